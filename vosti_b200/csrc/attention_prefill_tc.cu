@@ -33,7 +33,14 @@
 // kernels/triton_kernels/fattn_paged.py:176-252): out = acc / l, 0 if l = 0. A box brings
 // whole groups of 16 keys; keys of a group beyond the last visible one are overwritten with
 // zeros in shared memory, so what unused cache slots hold never reaches the arithmetic.
+//
+// A cache of 8 bits (e4m3.cuh) differs in the loaders alone: a loader warp's 16 keys are a block with one scale. It reads
+// the block's payloads into registers while the stage is still in use, makes them bfloat16 (exactly: the scale is a power
+// of two) and stores them swizzled. Values lie feature-major in the cache, so the second MMA reads them K-major.
+#include <type_traits>
+
 #include "common.cuh"
+#include "e4m3.cuh"
 #include "mma_util.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
@@ -62,16 +69,21 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 
 // score; keys before `bias_last` are visible whatever the window (tiles of them come first, in ascending key
 // order like all tiles); and every head's row is multiplied by the sigmoid of head_gate[token, head] (or null).
 // Without BIASED the arithmetic is what it was before the flag existed, bit for bit.
-template <int D, bool BIASED, bool CAPPED, bool SLOPED>
+// Side: how keys, or values, are held: a tensor map of a bfloat16 cache, or an E4m3Side.
+struct E4m3Side {
+  const uint8_t *payload, *scale;
+};
+template <int D, bool BIASED, bool CAPPED, bool SLOPED, typename Side = CUtensorMap>
 __global__ void __launch_bounds__(THREADS, 1)
-attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                            const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out,
+attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Side map_k,
+                            const __grid_constant__ Side map_v, bf16* __restrict__ out,
                             const int* __restrict__ row_list, const int* __restrict__ cu_q,
                             const int* __restrict__ kv_len, const int* __restrict__ block_table, int max_pages,
                             int page_size, int page_shift, int num_pages, int nq, int nkv, float scale_log2_in,
                             int window, const float* __restrict__ bias, int bias_last,
                             const float* __restrict__ sink, float softcap, const float* __restrict__ head_gate, unsigned* status) {
   const float scale_log2 = BIASED ? 1.f : scale_log2_in;      // BIASED: scores are scaled where the bias is added
+  constexpr bool EIGHT = std::is_same<Side, E4m3Side>::value;
   constexpr int NB = D / 64;                          // 64-element blocks of the head size
   constexpr int STAGES = kv_stages<D>();
   constexpr int Q_BYTES = NB * ROWS * 128;            // one row tile of Q
@@ -146,7 +158,9 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax and accumulation
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // (8 bits: the loaders hold payloads in registers)
+    if constexpr (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int wg = warp >> 2;                                    // its row tile
     const int r = threadIdx.x & 127;                             // row of the tile and lane of tensor memory
     const int token = token0 + wg * tokens_per_tile + r / group;
@@ -317,7 +331,8 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     tc_fence_before();
   } else if (warp < MMA_WARP) {
     // ------------------------------------------------------------ loaders
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (EIGHT) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int w = warp - 8;                              // keys 16 w .. 16 w + 15 of every tile
     if (w == 0 && lane == 0) {
       // Q rows: row r is token r / group, head r % group: a box [tokens][heads of the group][64]
@@ -331,6 +346,67 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int* table = block_table + (int64_t)b * max_pages;
     bool ok = true;
     uint32_t edges = 0;
+    if constexpr (EIGHT) {
+      constexpr int UNITS = D / 32;                      // 16-byte pieces of a block's keys, or values, that a lane moves
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int stage = j % STAGES;
+        const int lo = tile_key(j) + w * GROUP_KEYS;
+        uint4 piece[2][UNITS];
+        int k_scale = 0, v_scale = 0, seen = 0;          // tokens of the block before the last visible one's end
+        if (lo + GROUP_KEYS - 1 >= first_key && lo < key_end) {
+          const int index = page_shift >= 0 ? lo >> page_shift : lo / page_size;
+          const int page = index < max_pages ? table[index] : -1;
+          if (page < 0 || page >= num_pages) {
+            raise_fault(status, VOSTI_FAULT_PAGE_RANGE);
+          } else {
+            const int64_t block = ((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (lo - index * page_size) / GROUP_KEYS;
+            seen = min(GROUP_KEYS, key_end - lo);
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+              piece[0][i] = *reinterpret_cast<const uint4*>(map_k.payload + block * (GROUP_KEYS * D) + (lane + 32 * i) * 16);
+              piece[1][i] = *reinterpret_cast<const uint4*>(map_v.payload + block * (GROUP_KEYS * D) + (lane + 32 * i) * 16);
+            }
+            k_scale = map_k.scale[block];
+            v_scale = map_v.scale[block];
+          }
+        }
+        if (j >= STAGES) ok = mbar_wait(smem_u32(&kv_empty[stage]), ((j / STAGES) - 1) & 1, &abort_flag, status);
+        if (!ok) break;
+        // A block that is no number makes its scores no number: those are left out where they are not visible, while such a
+        // value would meet weights of zero in rows that do not see it.
+        const bool none = k_scale == E4M3_NAN_SCALE || v_scale == E4M3_NAN_SCALE;
+        uint8_t* const kd = kv_s + stage * STAGE_BYTES;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          const E4m3Factor f = e4m3_factor(side == 0 ? (none ? E4M3_NAN_SCALE : k_scale) : none ? 0 : v_scale);
+#pragma unroll
+          for (int i = 0; i < UNITS; ++i) {
+            const int u = lane + 32 * i;                 // keys: row u / (D / 16), 16 features; values: feature u
+            uint4 v = piece[side][i];
+            if (seen == 0 || (side == 1 && none)) v = make_uint4(0, 0, 0, 0);
+            if (side == 1 && seen < GROUP_KEYS) {        // bytes past the last visible token: zeros, as above
+              v.x &= e4m3_first_bytes(seen);
+              v.y &= e4m3_first_bytes(seen - 4);
+              v.z &= e4m3_first_bytes(seen - 8);
+              v.w &= e4m3_first_bytes(seen - 12);
+            }
+            uint4 lower = make_uint4(e4m3_widen<0>(v.x, f), e4m3_widen<1>(v.x, f), e4m3_widen<0>(v.y, f), e4m3_widen<1>(v.y, f));
+            uint4 upper = make_uint4(e4m3_widen<0>(v.z, f), e4m3_widen<1>(v.z, f), e4m3_widen<0>(v.w, f), e4m3_widen<1>(v.w, f));
+            if (f.second != E4M3_ONE) {
+              lower = make_uint4(bf16x2_times(lower.x, f.second), bf16x2_times(lower.y, f.second), bf16x2_times(lower.z, f.second), bf16x2_times(lower.w, f.second));
+              upper = make_uint4(bf16x2_times(upper.x, f.second), bf16x2_times(upper.y, f.second), bf16x2_times(upper.z, f.second), bf16x2_times(upper.w, f.second));
+            }
+            const int row = side == 0 ? w * GROUP_KEYS + u / (D / 16) : u, at = side == 0 ? u % (D / 16) : w;
+            uint8_t* const dst = kd + (side == 0 ? (at >> 2) * (KT * 128) : K_BYTES);
+            *reinterpret_cast<uint4*>(dst + swizzled(row, (at & 3) * 2)) = lower;
+            *reinterpret_cast<uint4*>(dst + swizzled(row, (at & 3) * 2 + 1)) = upper;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&kv_full[stage]));
+      }
+    } else
     for (int j = 0; j < tiles && ok; ++j) {
       const int stage = j % STAGES;
       if (j >= STAGES) ok = mbar_wait(smem_u32(&kv_empty[stage]), ((j / STAGES) - 1) & 1, &abort_flag, status);
@@ -357,8 +433,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const uint32_t bar = edge ? smem_u32(&edge_bar[w]) : smem_u32(&kv_full[stage]);
       if (lane == 0) mbar_expect_tx(bar, (uint32_t)(2 * NB * GROUP_KEYS * 128));
       __syncwarp();
+      if constexpr (!EIGHT) {
       if (lane < 2 * NB)
         tma_load_2d(smem_u32(dst + lane * (KT * 128)), lane < NB ? &map_k : &map_v, (lane < NB ? lane : lane - NB) * 64, row, bar);
+      }
       if (edge) {
         ok = mbar_wait(bar, edges & 1, &abort_flag, status);
         ++edges;
@@ -382,10 +460,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int role = warp - MMA_WARP, wg = role & 1;
     const int my_tiles = wg ? tiles_of[1] : tiles_of[0];
     constexpr uint32_t idesc_s = umma_instr_desc(ROWS, KT, false);
-    constexpr uint32_t idesc_pv = umma_instr_desc(ROWS, D, true);
+    constexpr uint32_t idesc_pv = umma_instr_desc(ROWS, D, !EIGHT);
     // descriptors differ in their start address only: bits [0,14) in units of 16 bytes
     const uint64_t q_desc = smem_desc_sw128(smem_u32(q_s) + wg * Q_BYTES), k_desc = smem_desc_sw128(smem_u32(kv_s));
-    const uint64_t v_desc = smem_desc_sw128_mn(smem_u32(kv_s) + K_BYTES, KT * 128);
+    const uint64_t v_desc = EIGHT ? smem_desc_sw128(smem_u32(kv_s) + K_BYTES) : smem_desc_sw128_mn(smem_u32(kv_s) + K_BYTES, KT * 128);
     bool ok = true;
     auto arrived = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &abort_flag, status)) != 0;
@@ -433,7 +511,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 #pragma unroll
           for (int ks = 0; ks < KT / 16; ++ks)
             umma_bf16(tmem_base + PV_COL + wg * D, p_desc + (uint64_t)((ks * 32) >> 4),
-                      vd + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv, (t | ks) ? 1u : 0u);
+                      vd + (uint64_t)((EIGHT ? ks * 32 : ks * 16 * 128) >> 4), idesc_pv, (t | ks) ? 1u : 0u);
           umma_commit(smem_u32(&p_empty[wg][t & 1]));
           umma_commit(smem_u32(&kv_empty[stage]));
         }
@@ -571,4 +649,44 @@ VOSTI_API int vosti_attention_prefill_tc_sloped(const void* q, const void* k_cac
   return launch_prefill_tc(q, k_cache, v_cache, out, row_list, count, cu_q, kv_len, block_table, max_pages, page_size,
                            num_pages, nq, nkv, d, max_q_len, tokens_total, scale, window, true, slopes, keep, sink, 0.f, status,
                            stream, true, head_gate);
+}
+
+// The same over a cache of 8 bits (e4m3.cuh); q and out as above.
+VOSTI_API int vosti_attention_prefill_tc_e4m3(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, void* out,
+                                              const int* row_list, int count, const int* cu_q, const int* kv_len, const int* block_table,
+                                              int max_pages, int page_size, int num_pages, int nq, int nkv, int d, int max_q_len,
+                                              int tokens_total, float scale, int window, unsigned* status, cudaStream_t stream) {
+  VOSTI_REQUIRE(count >= 0 && count <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0 && nq / nkv <= 16,
+                "attention_prefill_tc_e4m3: bad request or head counts (%d requests, nq=%d nkv=%d)", count, nq, nkv);
+  VOSTI_REQUIRE(vosti_attention_prefill_tc_supported(d, page_size),
+                "attention_prefill_tc_e4m3: head_dim %d must be 64 or 128 and page_size %d a multiple of 16", d, page_size);
+  VOSTI_REQUIRE(max_pages > 0 && num_pages > 0 && tokens_total > 0 && window >= 0 && scale > 0.f, "attention_prefill_tc_e4m3: bad geometry");
+  VOSTI_REQUIRE(k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr && (((uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0,
+                "attention_prefill_tc_e4m3: the cache is missing, or it or the output does not start on 16 bytes");
+  if (count == 0 || max_q_len <= 0) return VOSTI_OK;
+  const int group = nq / nkv, tokens_per_tile = ROWS / group, tokens_per_cta = ROW_TILES * tokens_per_tile;
+  CUtensorMap map_q;
+  const cuuint64_t dims[4] = {64, (cuuint64_t)nq, (cuuint64_t)tokens_total, (cuuint64_t)(d / 64)};
+  const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)nq * d * 2, 128};
+  const cuuint32_t box[4] = {64, (cuuint32_t)group, (cuuint32_t)tokens_per_tile, 1};
+  VOSTI_REQUIRE(encode_tensor_map_nd(&map_q, q, 4, dims, strides, box), "attention_prefill_tc_e4m3: cuTensorMapEncodeTiled failed (q)");
+  const E4m3Side keys = {(const uint8_t*)k, (const uint8_t*)k_scale}, values = {(const uint8_t*)v, (const uint8_t*)v_scale};
+  const dim3 grid((unsigned)((max_q_len + tokens_per_cta - 1) / tokens_per_cta) * nkv, count);
+  int page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (page_shift = 0; (1 << page_shift) < page_size; ++page_shift) {}
+#define LAUNCH_PREFILL_TC_E4M3(D)                                                                                     \
+  do {                                                                                                                \
+    auto kernel = attention_prefill_tc_kernel<D, false, false, false, E4m3Side>;                                      \
+    const cudaError_t raised =                                                                                        \
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prefill_tc_smem_bytes<D>());   \
+    VOSTI_REQUIRE(raised == cudaSuccess, "attention_prefill_tc_e4m3: %s", cudaGetErrorString(raised));                \
+    vosti_launch(kernel, grid, dim3(THREADS), prefill_tc_smem_bytes<D>(), stream, map_q, keys, values, (bf16*)out,    \
+                 row_list, cu_q, kv_len, block_table, max_pages, page_size, page_shift, num_pages, nq, nkv,           \
+                 scale * LOG2E, window, nullptr, 0, nullptr, 0.f, nullptr, status);                                   \
+  } while (0)
+  if (d == 64) LAUNCH_PREFILL_TC_E4M3(64);
+  else LAUNCH_PREFILL_TC_E4M3(128);
+#undef LAUNCH_PREFILL_TC_E4M3
+  VOSTI_LAUNCH_CHECK();
 }

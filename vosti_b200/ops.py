@@ -2280,3 +2280,178 @@ def moe_combine(y: torch.Tensor, where: torch.Tensor, weights: torch.Tensor) -> 
     _check(library().vosti_moe_combine(_p(y), _p(where), _p(weights), _p(out), tokens, top, y.shape[1], _stream()),
            "moe_combine")
     return out
+
+
+# ---------------------------------------------------------------- serving in few bits
+def _bound(name: str, kinds: str):
+    """The library's function `name` with its argument types set once, so that plain ints and floats may be handed to it: p a
+    pointer (an int or None), i int32, l int64, f float32."""
+    fn = getattr(library(), name)
+    if fn.argtypes is None:
+        fn.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float}[k] for k in kinds]
+    return fn
+
+
+def _here(what: str, *tensors) -> int:
+    """The current stream, if every tensor (or None) is contiguous and on the current CUDA device."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is None:
+            continue
+        if t.get_device() != device:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
+        if not t.is_contiguous():
+            raise KernelError("kernels take contiguous tensors")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _ints(what: str, count: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.numel() < count:
+            raise KernelError(f"{what}: {name} is int32 with {count} entries, got {t.dtype} {tuple(t.shape)}")
+
+
+E4M3_BLOCK = 16      # tokens of a block with one scale
+
+
+class PagedE4M3:
+    """One layer's keys and values in 8 bits (csrc/e4m3.cuh): float8_e4m3fn payloads, `k` [pages, kv heads, page, d] and `v`
+    [pages, kv heads, page / 16, d, 16], with a power of two (float8_e8m0fnu) per block of 16 tokens and kv head in `k_scale` and
+    `v_scale` [pages, kv heads, page / 16]. A block that was handed a value that is not finite, or 2^96
+    or more in size (sums of weights times values have to fit float32), has the scale 255 and is no number. `zeros` makes an empty one; `dequantized` gives keys and values [pages, kv heads, page, d] in float32."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "head_dim", "pointers")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 4 or k.shape[2] % E4M3_BLOCK or k.shape[3] % 16 or not 0 < k.shape[3] <= 256:
+            raise KernelError("a cache of 8 bits has keys [pages, kv heads, page, d], the page a multiple of 16 tokens, d of 16 up to 256; "
+                              f"got {tuple(k.shape)}")
+        pages, heads, page, d = k.shape
+        scales = (pages, heads, page // E4M3_BLOCK)
+        if tuple(v.shape) != (*scales, d, E4M3_BLOCK) or tuple(k_scale.shape) != scales or tuple(v_scale.shape) != scales:
+            raise KernelError(f"a cache of 8 bits with keys {tuple(k.shape)} has values {(*scales, d, E4M3_BLOCK)} and scales {scales}; got "
+                              f"{tuple(v.shape)}, {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+        if k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or k_scale.dtype != torch.float8_e8m0fnu or v_scale.dtype != k_scale.dtype:
+            raise KernelError("a cache of 8 bits has float8_e4m3fn payloads and float8_e8m0fnu scales")
+        if not all(t.is_cuda and t.is_contiguous() and t.device == k.device for t in (k, v, k_scale, v_scale)):
+            raise KernelError("a cache of 8 bits is contiguous, on one CUDA device")
+        if (k.data_ptr() | v.data_ptr()) % 16 or pages * page > 0x7fffffff:
+            raise KernelError("a cache of 8 bits starts on 16 bytes and has fewer than 2^31 slots")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page, d
+        self.pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+
+    @staticmethod
+    def tensors(pages: int, heads: int, page_size: int, head_dim: int, device) -> tuple:
+        """(k, v, k_scale, v_scale) of an empty cache."""
+        if page_size <= 0 or page_size % E4M3_BLOCK:
+            raise KernelError(f"a cache of 8 bits needs pages of a multiple of {E4M3_BLOCK} tokens, got {page_size}")
+        blocks = page_size // E4M3_BLOCK
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device)
+        return (zeros(pages, heads, page_size, head_dim).view(torch.float8_e4m3fn), zeros(pages, heads, blocks, head_dim, E4M3_BLOCK).view(torch.float8_e4m3fn),
+                zeros(pages, heads, blocks).view(torch.float8_e8m0fnu), zeros(pages, heads, blocks).view(torch.float8_e8m0fnu))
+
+    @classmethod
+    def zeros(cls, pages: int, heads: int, page_size: int, head_dim: int, device="cuda:0") -> "PagedE4M3":
+        return cls(*cls.tensors(pages, heads, page_size, head_dim, device))
+
+    def dequantized(self):
+        k_scale, v_scale = (s.float().repeat_interleave(E4M3_BLOCK, dim=2).unsqueeze(-1) for s in (self.k_scale, self.v_scale))
+        return self.k.float() * k_scale, self.v.float().transpose(-1, -2).reshape(self.k.shape) * v_scale
+
+
+def qkv_post_e4m3(qkv, cache: PagedE4M3, *, nq: int, nkv: int, head_dim: int, slot_mapping: torch.Tensor, status: torch.Tensor,
+                  q_norm_w: Optional[torch.Tensor] = None, k_norm_w: Optional[torch.Tensor] = None, eps: float = 1.0,
+                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                  rotary_dim: Optional[int] = None, interleaved: bool = False) -> torch.Tensor:
+    """`qkv_post` for a cache of 8 bits: head norm and rotation, queries returned [T, nq * d], keys and values rounded into
+    their blocks' payloads. Token t goes to slot slot_mapping[t] (-1: nowhere). The step's tokens of a block stand next to one
+    another in `qkv`, in the block's order; what the block holds before the first of them stays, under a larger scale where the
+    new ones need it, and what comes after the last of them is left as it was. No two requests of a step write to
+    one block."""
+    partial, splits = None, 0
+    if isinstance(qkv, PartialSum):
+        qkv.check()
+        partial, splits, dtype, (tokens, width) = qkv.partial, qkv.splits, qkv.dtype, qkv.shape
+        qkv = None
+    else:
+        if qkv.dim() != 2:
+            raise KernelError("qkv_post_e4m3: the projection is [tokens, (nq + 2 nkv) d]")
+        dtype, (tokens, width) = qkv.dtype, qkv.shape
+    if dtype != torch.bfloat16 and dtype != torch.float32:
+        raise KernelError(f"kernels take float32 or bfloat16 tensors, got {dtype}")
+    if width != (nq + 2 * nkv) * head_dim or cache.heads != nkv or cache.head_dim != head_dim:
+        raise KernelError("qkv_post_e4m3: input width, head counts and cache do not match")
+    rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+    _ints("qkv_post_e4m3", tokens, slot_mapping=slot_mapping)
+    _ints("qkv_post_e4m3", 1, status=status)
+    max_positions = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or positions is None:
+            raise KernelError("qkv_post_e4m3: rotation needs cos, sin and positions")
+        _ints("qkv_post_e4m3", tokens, positions=positions)
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or sin.shape != cos.shape:
+            raise KernelError("qkv_post_e4m3: rotation tables must be float32 [positions, rotary_dim/2]")
+        max_positions = cos.shape[0]
+    norm_flag = 0
+    for w in (q_norm_w, k_norm_w):
+        if w is not None:
+            norm_flag = _is_f32(w)
+            if w.numel() != head_dim or (k_norm_w is not None and w.dtype != k_norm_w.dtype):
+                raise KernelError("qkv_post_e4m3: norm weights have head_dim entries and share a dtype")
+    stream = _here("qkv_post_e4m3", qkv, partial, cache.k, q_norm_w, k_norm_w, cos, sin, positions, slot_mapping, status)
+    q_out = torch.empty((tokens, nq * head_dim), dtype=dtype, device=cache.k.device)
+    k, v, k_scale, v_scale = cache.pointers
+    _check(_bound("vosti_qkv_post_e4m3", "ppippppppp" "ifppippli" "iiiiiiipp")(
+        _address(qkv), _address(partial), splits, q_out.data_ptr(), k, v, k_scale, v_scale, _address(q_norm_w), _address(k_norm_w),
+        norm_flag, eps, _address(cos), _address(sin), max_positions, _address(positions), slot_mapping.data_ptr(), cache.pages * cache.page_size, cache.page_size,
+        tokens, nq, nkv, head_dim, rotary_dim, bool(interleaved), dtype == torch.float32, status.data_ptr(), stream), "qkv_post_e4m3")
+    return q_out
+
+
+def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nkv: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
+    """`attention` over a cache of 8 bits: every query row of the step over its request's keys, causal, the last `window` of them if
+    that is not 0. bfloat16 with heads of 64 or 128: single tokens on a kernel that cuts the keys into segments, portions on the tcgen05 kernel;
+    everything else on the CUDA cores in float32."""
+    tokens = q.shape[0]
+    if q.dim() != 2 or q.shape[1] != nq * head_dim or q.dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError("attention_e4m3: the queries are bfloat16 or float32 [tokens, nq * d]")
+    if nq <= 0 or nkv <= 0 or nq % nkv or cache.heads != nkv or cache.head_dim != head_dim or group.page_size != cache.page_size:
+        raise KernelError("attention_e4m3: head counts, page size and cache do not match")
+    table, status = group.block_table, ctx.status
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise KernelError("attention_e4m3: the block table is int32 [requests, pages]")
+    if window < 0 or not scale > 0:
+        raise KernelError("attention_e4m3: the score scale must be positive and the window not negative")
+    _ints("attention_e4m3", tokens, positions=ctx.positions, request_of=ctx.request_of)
+    stream = _here("attention_e4m3", q, cache.k, ctx.positions, ctx.request_of, table, status)
+    out = torch.empty_like(q)
+    geometry = (table.data_ptr(), table.shape[1], cache.page_size, cache.pages, nq, nkv, head_dim)
+    if q.dtype != torch.bfloat16 or head_dim not in (64, 128):
+        _check(_bound("vosti_attention_e4m3_simt", "pppppp" "ipp" "piiiiii" "fiipp")(
+            q.data_ptr(), *cache.pointers, out.data_ptr(), tokens, ctx.positions.data_ptr(), ctx.request_of.data_ptr(), *geometry, scale, window,
+            q.dtype == torch.float32, status.data_ptr(), stream), "attention_e4m3")
+        return out
+    lists = ctx.layout["attention"]
+    count, long_rows = lists["num_short_tokens"], lists["num_long_rows"]
+    if long_rows and nq // nkv > 16:                             # (more query heads than the portion kernel's tiles take)
+        count, long_rows, short = tokens, 0, None
+    else:
+        short = ctx.extras.get("attention.short_tokens")
+    if count:
+        if short is not None:
+            _here("attention_e4m3", short)
+        _check(_bound("vosti_attention_e4m3", "pppppp" "pipp" "piiiiii" "ifipp")(
+            q.data_ptr(), *cache.pointers, out.data_ptr(), _address(short), count, ctx.positions.data_ptr(), ctx.request_of.data_ptr(), *geometry,
+            ctx.max_kv_len, scale, window, status.data_ptr(), stream), "attention_e4m3")
+    if long_rows:
+        rows = ctx.extras.get("attention.long_rows")
+        _here("attention_e4m3", rows, ctx.cu_q, ctx.kv_len)
+        _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iifipp")(
+            q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
+            lists["max_long_q_len"], tokens, scale, window, status.data_ptr(), stream), "attention_prefill_tc_e4m3")
+    return out
