@@ -1,0 +1,119 @@
+"""Products with 4-bit weights on the GPU against 64 bits.
+
+Bounds. Up to 16 rows a group's codes meet the rows exactly, sums are float32: off by (k + group count) 2^-24 of sum |x||w| at most. With more
+rows codes times scales are rounded to bfloat16, 2^-8 of each product at most; then the same sums. The result's rounding is 2^-8 of it in
+bfloat16, 2^-24 in float32."""
+import pytest
+import torch
+
+from vosti_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEVICE = "cuda:0"
+
+
+def weight(features, k, group, seed=0):
+    gen = torch.Generator().manual_seed(seed + features + k)
+    codes = torch.randint(-8, 8, (features, k), generator=gen, dtype=torch.int8)
+    scales = (torch.rand(features, -(-k // group), generator=gen) * 0.01 + 0.001).bfloat16()
+    return ops.Int4Weight.from_codes(codes.to(DEVICE), scales.to(DEVICE), group), codes.double() * scales.double().repeat_interleave(group, dim=1)[:, :k], gen
+
+
+def check(y, x, w, rows):
+    want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+    bound = (x.shape[1] + 8) * 2.0 ** -24 * size + (2.0 ** -8 if y.dtype == torch.bfloat16 else 2.0 ** -24) * want.abs()
+    if rows > 16:
+        bound += 2.0 ** -8 * size
+    worst = float(((y.cpu().double() - want).abs() - bound).max())
+    assert worst <= 0, worst
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 33, 64, 65, 128, 129, 256, 300])
+@pytest.mark.parametrize("features,k,group", [(16, 128, 128), (1000, 1024, 128), (130, 640, 32), (4096, 512, 64), (33, 4096, 128), (257, 96, 32), (5000, 2048, 64),
+                                              (1, 64, 64), (640, 200, 32)])
+def test_products(rows, features, k, group):
+    w, numbers, gen = weight(features, k, group)
+    x = torch.randn(rows, k, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    for kind in (torch.bfloat16, torch.float32):
+        y = ops.gemm_int4(x.to(DEVICE), w, status, out_dtype=kind)
+        assert int(status) == 0 and y.dtype == kind and tuple(y.shape) == (rows, features)
+        check(y, x, numbers, rows)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 40])
+@pytest.mark.parametrize("k", [1, 7, 100, 129, 1003])
+def test_rows_that_start_inside_a_word(rows, k):
+    w, numbers, gen = weight(70, k, 32)
+    x = torch.randn(rows, k, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    check(ops.gemm_int4(x.to(DEVICE), w, status), x, numbers, 17)
+    # the same matrix from an odd address
+    odd = torch.zeros(rows * 128 + 1, dtype=torch.bfloat16, device=DEVICE)[1:].view(rows, 128)
+    w, numbers, gen = weight(70, 128, 32)
+    x = torch.randn(rows, 128, generator=gen).bfloat16()
+    odd.copy_(x)
+    check(ops.gemm_int4(odd, w, status), x, numbers, 17)
+
+
+def test_no_rows():
+    w, _, _ = weight(32, 128, 128)
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    assert tuple(ops.gemm_int4(torch.empty(0, 128, dtype=torch.bfloat16, device=DEVICE), w, status).shape) == (0, 32)
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+def test_what_stands_beyond_the_matrix_does_not_count(rows):
+    w, numbers, gen = weight(40, 200, 32)
+    w.codes.view(3, 2, 16, 4, 4, 4)[2, :, 8:] = 255                       # rows 40 .. 47
+    w.scales[2, :, 8:] = float("nan")
+    w.scales[:, 1, :, 3] = float("nan")                                   # k 224 .. 255
+    x = torch.randn(rows, 200, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    check(ops.gemm_int4(x.to(DEVICE), w, status), x, numbers, rows)
+
+
+@pytest.mark.parametrize("rows", [2, 20])
+def test_rows_do_not_mix(rows):
+    """A row that is no number leaves the others alone."""
+    w, numbers, gen = weight(200, 512, 128)
+    x = torch.randn(rows, 512, generator=gen).bfloat16()
+    x[1, 7] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    y = ops.gemm_int4(x.to(DEVICE), w, status).cpu()
+    assert y[1].isnan().all()
+    keep = [r for r in range(rows) if r != 1]
+    check(y[keep], x[keep], numbers, rows)
+
+
+def test_another_stream_and_a_graph():
+    w, _, gen = weight(512, 1024, 128)
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    for rows in (4, 70):
+        x = torch.randn(rows, 1024, generator=gen).bfloat16().to(DEVICE)
+        want = ops.gemm_int4(x, w, status)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = ops.gemm_int4(x, w, status)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = ops.gemm_int4(x, w, status)
+        kept.zero_()
+        graph.replay()
+        assert torch.equal(kept, want)
+
+
+def test_quantized_on_the_device():
+    gen = torch.Generator().manual_seed(5)
+    w = torch.randn(130, 300, generator=gen) * 0.02
+    a, b = ops.Int4Weight.quantize(w, 64), ops.Int4Weight.quantize(w.to(DEVICE), 64)
+    assert torch.equal(a.codes, b.codes.cpu()) and torch.equal(a.scales, b.scales.cpu())
+
+
+def test_tiles_ask_for_no_more_tensor_memory_than_an_sm_has():
+    for tile in range(4):
+        assert 0 < ops.library().vosti_gemm_int4_columns_an_sm(tile) <= 512
+    assert ops.library().vosti_gemm_int4_columns_an_sm(4) == -1

@@ -1,0 +1,511 @@
+// Product with weights in 4 bits and a scale for each group along k:
+//   Y[t, f] = sum_k X[t, k] * c[f, k] * s[f, k / group]       c in -8 .. 7, X and s bfloat16, sums float32
+// Layout (what a reader wants next to one another lies next to one another):
+//   codes   [features / 16][k / 128][16 rows][4 j][4 i][4 bytes]     a row's 128 codes in 64 bytes; the 32-bit word (j, i) holds k = 32 i +
+//                                                                    8 j .. + 7, nibble p the code c + 8 of k offset 2 p (p < 4) or 2 p - 7
+//   scales  [features / 16][k / 128][16 rows][128 / group]           bfloat16, group 32, 64 or 128
+// A word shifted by 4 p and masked holds the codes of neighbouring k in its halves; with the exponent of 128 or'ed in they are 128 + c + 8 in
+// bfloat16, exactly, and minus 136 the codes.
+//
+// Up to 16 tokens: mma.sync, weights as the 16 rows (int4_few_kernel). What bounds it is the weights' bytes. More tokens: tcgen05
+// (int4_tiles_kernel), weights made bfloat16 in tensor memory.
+#include "common.cuh"
+#include "mma_util.cuh"
+#include "tcgen05.cuh"
+#include "tensor_map.cuh"
+
+namespace {
+
+constexpr int KB = 128;                    // k of a block of codes: 64 bytes a row
+constexpr int TILE_BYTES = 16 * KB / 2;    // codes of 16 rows
+
+// Codes of k offsets 2 P and 2 P + 1 of a word, in bfloat16.
+template <int P>
+__device__ __forceinline__ uint32_t int4_codes(uint32_t w) {
+  const uint32_t t = ((w >> (4 * P)) & 0x000f000fu) | 0x43004300u;
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0xc308c308u));
+  return r;
+}
+__device__ __forceinline__ uint32_t int4_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// A row's scales of a block of 128 k (N = 1, 2 or 4), two to a word, of which `left` k are the matrix's: what stands for groups beyond
+// them (k < 128 in the last block) may be no number and becomes zero.
+template <int N>
+__device__ __forceinline__ void load_scales(const bf16* p, int left, uint32_t (&s)[(N + 1) / 2]) {
+  if constexpr (N == 1) {
+    s[0] = *reinterpret_cast<const unsigned short*>(p);
+  } else if constexpr (N == 2) {
+    s[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    s[0] = v.x;
+    s[1] = v.y;
+  }
+  if (N > 1 && left < KB) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * (KB / N) >= left) s[i / 2] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
+  }
+}
+__device__ __forceinline__ float scale_of(uint32_t word, int i) { return __uint_as_float((i & 1) ? word & 0xffff0000u : word << 16); }
+
+// ---------------------------------------------------------------------------------------------- up to 16 tokens
+// A CTA takes FT tiles of 16 features over all of k, its eight warps every eighth block of 128 k, straight from memory into registers
+// one block ahead. The order of k inside an instruction is free: lane j of a row takes offsets 8 j .. 8 j + 7 of every 32 k, so that four of
+// them are a word's half and the tokens' 8 are one 16-byte load. An instruction never mixes groups: a group's codes are summed exactly, then
+// multiplied by its scale in float32. The warps' sums meet in shared memory, in warp order.
+constexpr int FEW_WARPS = 8, FEW_THREADS = FEW_WARPS * 32;
+
+// 16 bytes of a token's row from element kk on; rows that do not start on whole words are read element by element, zeros beyond k.
+template <bool WORDS>
+__device__ __forceinline__ uint4 load_tokens(const bf16* row, int kk, int k) {
+  if constexpr (WORDS) {
+    return kk < k ? *reinterpret_cast<const uint4*>(row + kk) : make_uint4(0, 0, 0, 0);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = kk + 2 * i < k ? reinterpret_cast<const unsigned short*>(row)[kk + 2 * i] : 0;
+      const uint32_t hi = kk + 2 * i + 1 < k ? reinterpret_cast<const unsigned short*>(row)[kk + 2 * i + 1] : 0;
+      w[i] = lo | hi << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <int FT, int NT, int GROUPS, bool WORDS>
+__global__ void __launch_bounds__(FEW_THREADS)
+int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y, int y_is_f32,
+                int rows, int n, int k, int tiles, int deep) {
+  constexpr int SW = (GROUPS + 1) / 2;
+  __shared__ float sums[FEW_WARPS][NT * 8][FT * 16 + 4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r8 = lane >> 2, j = lane & 3;
+  const int tile0 = blockIdx.x * FT;
+  uint4 c[FT][2];
+  uint32_t s[FT][2][SW];
+  auto load = [&](int kb) {
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+      const int64_t at = ((int64_t)min(tile0 + f, tiles - 1) * deep + kb) * 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[f][h] = load_codes(codes + (at + r8 + 8 * h) * (KB / 2) + 16 * j);
+        load_scales<GROUPS>(scales + (at + r8 + 8 * h) * GROUPS, k - kb * KB, s[f][h]);
+      }
+    }
+  };
+  // the first weights do not depend on the kernel before this one
+  if (warp < deep) load(warp);
+  pdl_wait();
+  pdl_launch_dependents();
+  float acc[FT][NT][4];
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[f][t][0] = acc[f][t][1] = acc[f][t][2] = acc[f][t][3] = 0.f;
+  for (int kb = warp; kb < deep; kb += FEW_WARPS) {
+    uint4 b[NT][4];                                              // [8 tokens][32 k]
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        b[t][i] = t * 8 + r8 < rows ? load_tokens<WORDS>(x + (int64_t)(t * 8 + r8) * k, kb * KB + 32 * i + 8 * j, k) : make_uint4(0, 0, 0, 0);
+    uint4 now[FT][2];
+    uint32_t s_now[FT][2][SW];
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        now[f][h] = c[f][h];
+#pragma unroll
+        for (int w = 0; w < SW; ++w) s_now[f][h][w] = s[f][h][w];
+      }
+    if (kb + FEW_WARPS < deep) load(kb + FEW_WARPS);
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        float part[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
+#pragma unroll
+        for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
+          const uint32_t lo = int4_word(now[f][0], i), hi = int4_word(now[f][1], i);
+          const uint32_t first[4] = {int4_codes<0>(lo), int4_codes<0>(hi), int4_codes<1>(lo), int4_codes<1>(hi)};
+          const uint32_t second[4] = {int4_codes<2>(lo), int4_codes<2>(hi), int4_codes<3>(lo), int4_codes<3>(hi)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma_bf16(part[t], first, b[t][i].x, b[t][i].y);
+            mma_bf16(part[t], second, b[t][i].z, b[t][i].w);
+          }
+        }
+        const float s0 = scale_of(s_now[f][0][g / 2], g), s1 = scale_of(s_now[f][1][g / 2], g);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          acc[f][t][0] = fmaf(part[t][0], s0, acc[f][t][0]);
+          acc[f][t][1] = fmaf(part[t][1], s0, acc[f][t][1]);
+          acc[f][t][2] = fmaf(part[t][2], s1, acc[f][t][2]);
+          acc[f][t][3] = fmaf(part[t][3], s1, acc[f][t][3]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[warp][t * 8 + 2 * j + (e & 1)][f * 16 + r8 + 8 * (e >> 1)] = acc[f][t][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * FT * 16; i += FEW_THREADS) {
+    const int t = i / (FT * 16), f = i % (FT * 16);
+    if (tile0 * 16 + f >= n) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < FEW_WARPS; ++w) v += sums[w][t][f];
+    const int64_t at = (int64_t)t * n + tile0 * 16 + f;
+    if (y_is_f32) reinterpret_cast<float*>(y)[at] = v;
+    else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- more tokens
+// Features on M = 128, TOK tokens on N; k in `segments`, one CTA of a cluster each, summed in their order through distributed shared
+// memory. Eight warps read the codes into registers DEPTH blocks ahead (a thread: half a feature's block, one 32-byte sector), make them
+// bfloat16 times their scale (rounded once: codes of 1, 2, 4 and 8 are exact) and store them to one of two stages in tensor memory; a
+// ninth warp issues the MMAs, a tenth brings the tokens by TMA.
+constexpr int WORKERS = 256, TILE_THREADS = WORKERS + 64;
+constexpr int FEATURES = 128;
+constexpr int A_STAGES = 2, A_COLS = KB / 2;
+constexpr int DEPTH = 4;
+
+template <int TOK>
+struct Int4Tile {
+  static constexpr int X_STAGE = TOK * KB * 2;
+  static constexpr int X_STAGES = TOK >= 128 ? 3 : 4;
+  static constexpr int COLS = TOK + A_STAGES * A_COLS <= 256 ? 256 : 512;
+  static constexpr int RING = X_STAGES * X_STAGE, SUMS = TOK * FEATURES * 4;
+  // no more CTAs an SM than tensor memory has columns for: shared memory (228 KB, 1 KB of it with every CTA) is padded until that many fit
+  static constexpr int FEWEST = 228 * 1024 / (512 / COLS + 1);
+  static constexpr int NEEDED = (RING > SUMS ? RING : SUMS) + 1024;
+  static constexpr int SMEM = NEEDED > FEWEST ? NEEDED : FEWEST;
+  static constexpr int CTAS = 512 / COLS;
+};
+
+__device__ __forceinline__ void int4_tmem_store8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ uint32_t int4_times(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float4 int4_load_rank(uint32_t smem_at, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_at), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, status);
+  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  __syncwarp();
+  return ok;
+}
+__device__ __forceinline__ void int4_workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
+
+template <int TOK, int GROUPS>
+__global__ void __launch_bounds__(TILE_THREADS, Int4Tile<TOK>::CTAS)
+int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y,
+                  int y_is_f32, int rows, int n, int k, int tiles, int deep, int token_tiles, int segments, unsigned* status) {
+  using Tile = Int4Tile<TOK>;
+  constexpr int SW = (GROUPS + 1) / 2, COLS = TOK / 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t x_full[Tile::X_STAGES], x_empty[Tile::X_STAGES], a_full[A_STAGES], a_empty[A_STAGES];
+  __shared__ uint32_t tmem_base_holder;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int segment = blockIdx.x % segments;
+  const int t0 = (blockIdx.x / segments) % token_tiles * TOK, f0 = blockIdx.x / (segments * token_tiles) * FEATURES;
+  const int kb_begin = (int)((int64_t)deep * segment / segments), blocks = (int)((int64_t)deep * (segment + 1) / segments) - kb_begin;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < Tile::X_STAGES; ++s) {
+      mbar_init(smem_u32(&x_full[s]), 1);
+      mbar_init(smem_u32(&x_empty[s]), 1);
+    }
+    for (int s = 0; s < A_STAGES; ++s) {
+      mbar_init(smem_u32(&a_full[s]), WORKERS / 32);
+      mbar_init(smem_u32(&a_empty[s]), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc(smem_u32(&tmem_base_holder), Tile::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();               // (after this CTA's tensor memory is its own)
+  const uint32_t tmem_sum = tmem_base_holder, tmem_a = tmem_sum + TOK;
+
+  if (warp == WORKERS / 32 + 1) {
+    if (lane == 0) {
+      pdl_wait();
+      for (int b = 0; b < blocks; ++b) {
+        const int s = b % Tile::X_STAGES;
+        if (b >= Tile::X_STAGES && !mbar_wait(smem_u32(&x_empty[s]), (b / Tile::X_STAGES - 1) & 1, &abort_flag, status)) break;
+        mbar_expect_tx(smem_u32(&x_full[s]), (uint32_t)Tile::X_STAGE);
+        for (int h = 0; h < 2; ++h)
+          tma_load_2d(smem_u32(smem + s * Tile::X_STAGE + h * (TOK * 128)), &map_x, (kb_begin + b) * KB + h * 64, t0, smem_u32(&x_full[s]));
+      }
+    }
+    return;
+  }
+  if (warp == WORKERS / 32) {
+    constexpr uint32_t idesc = umma_instr_desc(FEATURES, TOK, false);
+    bool ok = true;
+    auto arrived = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &abort_flag, status)) != 0;
+    };
+    for (int b = 0; b < blocks && ok; ++b) {
+      const int s = b % A_STAGES, xs = b % Tile::X_STAGES;
+      ok = arrived(&x_full[xs], (b / Tile::X_STAGES) & 1) && arrived(&a_full[s], (b / A_STAGES) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t desc = smem_desc_sw128(smem_u32(smem + xs * Tile::X_STAGE));
+      if (elect_one()) {
+#pragma unroll
+        for (int q = 0; q < KB / 16; ++q)
+          umma_bf16_ts(tmem_sum, tmem_a + s * A_COLS + 8 * q, desc + (uint64_t)(((q >> 2) * (TOK * 128) + (q & 3) * 32) >> 4), idesc, b > 0 || q > 0);
+        umma_commit(smem_u32(&a_empty[s]));
+        umma_commit(smem_u32(&x_empty[xs]));
+      }
+      __syncwarp();
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- workers
+  const int quarter = warp & 3, half = warp >> 2, feature = quarter * 32 + lane;
+  const int tile = min(f0 / 16 + feature / 16, tiles - 1);       // (rows beyond the matrix are never stored)
+  const int64_t row = ((int64_t)tile * deep + kb_begin) * 16 + feature % 16;
+  const uint8_t* const my_codes = codes + row * (KB / 2) + 32 * half;
+  const bf16* const my_scales = scales + row * GROUPS;
+  const uint32_t my_a = tmem_a + ((uint32_t)(quarter * 32) << 16) + 8 * half;
+  uint4 c[DEPTH][2];
+  uint32_t sc[DEPTH][SW];
+  auto load = [&](int b, int d) {
+    const uint8_t* const at = my_codes + (int64_t)b * TILE_BYTES;
+    c[d][0] = load_codes(at);
+    c[d][1] = load_codes(at + 16);
+    load_scales<GROUPS>(my_scales + (int64_t)b * 16 * GROUPS, k - (kb_begin + b) * KB, sc[d]);
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (d < blocks) load(d, d);
+  bool ok = true;
+  for (int b0 = 0; b0 < blocks && ok; b0 += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int b = b0 + d, s = b % A_STAGES;
+      if (b >= blocks || !ok) break;
+      if (b >= A_STAGES) {
+        ok = int4_wait(smem_u32(&a_empty[s]), (b / A_STAGES - 1) & 1, &abort_flag, status);
+        if (!ok) break;
+        tc_fence_after();                                        // (the MMAs that read the stage)
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int g = i * GROUPS / 4;
+        const uint32_t two = __byte_perm(sc[d][g / 2], 0, (g & 1) ? 0x3232 : 0x1010);
+        const uint32_t lo = int4_word(c[d][0], i), hi = int4_word(c[d][1], i);
+        const uint32_t r[8] = {int4_times(int4_codes<0>(lo), two), int4_times(int4_codes<1>(lo), two), int4_times(int4_codes<2>(lo), two),
+                               int4_times(int4_codes<3>(lo), two), int4_times(int4_codes<0>(hi), two), int4_times(int4_codes<1>(hi), two),
+                               int4_times(int4_codes<2>(hi), two), int4_times(int4_codes<3>(hi), two)};
+        int4_tmem_store8(my_a + s * A_COLS + 16 * i, r);
+      }
+      if (b + DEPTH < blocks) load(b + DEPTH, d);
+      tmem_wait_stores();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&a_full[s]));
+    }
+  }
+  if (ok && blocks > 0) ok = int4_wait(smem_u32(&a_empty[(blocks - 1) % A_STAGES]), ((blocks - 1) / A_STAGES) & 1, &abort_flag, status);
+  tc_fence_after();
+  pdl_wait();                                                    // (what this kernel writes may still be read before that)
+
+  const uint32_t my_sums = tmem_sum + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+  auto store = [&](int t, int f, float v) {
+    if (t0 + t >= rows || f0 + f >= n) return;
+    const int64_t at = (int64_t)(t0 + t) * n + f0 + f;
+    if (y_is_f32) reinterpret_cast<float*>(y)[at] = v;
+    else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
+  };
+  float* const part = reinterpret_cast<float*>(smem);            // (every MMA that read the ring is complete)
+  // [TOK][128] sums; 16 columns at a time where there are fewer than 32
+  constexpr int STEP = COLS < 32 ? COLS : 32;
+  for (int c0 = 0; c0 < COLS && blocks > 0; c0 += STEP) {
+    uint32_t r[32];
+    if constexpr (STEP == 32) {
+      tmem_load32(my_sums + c0, r);
+    } else {
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+            "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          : "r"(my_sums + c0));
+      tmem_wait_loads();
+    }
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) {
+      const int t = half * COLS + c0 + i;
+      if (segments == 1) store(t, feature, __uint_as_float(r[i]));
+      else part[t * FEATURES + feature] = __uint_as_float(r[i]);
+    }
+  }
+  tc_fence_before();
+  if (segments > 1) {
+    // The roles that bring and issue have ended: every thread of the cluster that is left takes part
+    cluster_sync_all();
+    const int lo = TOK * segment / segments, hi = TOK * (segment + 1) / segments;
+    for (int word = threadIdx.x; word < (hi - lo) * (FEATURES / 4); word += WORKERS) {
+      const int t = lo + word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
+      if (t0 + t >= rows) break;
+      const uint32_t at = smem_u32(&part[t * FEATURES + f]);
+      float4 v = int4_load_rank(at, 0);
+      for (int r = 1; r < segments; ++r) {
+        const float4 u = int4_load_rank(at, r);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+      }
+      store(t, f, v.x);
+      store(t, f + 1, v.y);
+      store(t, f + 2, v.z);
+      store(t, f + 3, v.w);
+    }
+    cluster_sync_all();                                          // nobody reads this CTA's sums after this
+  }
+  int4_workers_sync();
+  if (abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    int4_workers_sync();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem_sum, Tile::COLS);
+  }
+}
+
+// Segments of k: as many as still find an SM, each of four blocks at least.
+int int4_segments(int64_t ctas, int deep, int at_once) {
+  int s = 1;
+  while (s < 8 && ctas * s * 2 <= at_once && deep >= 8 * s) s *= 2;
+  return s;
+}
+
+struct Int4Args {
+  const bf16* x;
+  const uint8_t* codes;
+  const bf16* scales;
+  void* y;
+  int y_is_f32, rows, n, k, tiles, deep;
+  unsigned* status;
+  cudaStream_t stream;
+};
+
+template <int FT, int NT, int GROUPS>
+cudaError_t launch_few(const Int4Args& a, bool words) {
+  const dim3 grid((a.tiles + FT - 1) / FT);
+  if (words)
+    return vosti_launch(int4_few_kernel<FT, NT, GROUPS, true>, grid, dim3(FEW_THREADS), 0, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n,
+                        a.k, a.tiles, a.deep);
+  return vosti_launch(int4_few_kernel<FT, NT, GROUPS, false>, grid, dim3(FEW_THREADS), 0, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n,
+                      a.k, a.tiles, a.deep);
+}
+template <int GROUPS>
+cudaError_t launch_few_as(const Int4Args& a, bool words) {
+  const bool wide = a.tiles > 2 * 148;
+  if (a.rows <= 8) return wide ? launch_few<2, 1, GROUPS>(a, words) : launch_few<1, 1, GROUPS>(a, words);
+  return wide ? launch_few<2, 2, GROUPS>(a, words) : launch_few<1, 2, GROUPS>(a, words);
+}
+
+template <int TOK, int GROUPS>
+int launch_tiles(const Int4Args& a) {
+  auto kernel = int4_tiles_kernel<TOK, GROUPS>;
+  constexpr int SMEM = Int4Tile<TOK>::SMEM;
+  const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  VOSTI_REQUIRE(raised == cudaSuccess, "gemm_int4: %s", cudaGetErrorString(raised));
+  CUtensorMap map;
+  VOSTI_REQUIRE(encode_tensor_map_2d(&map, a.x, a.rows, a.k, TOK, 64), "gemm_int4: cuTensorMapEncodeTiled failed");
+  const int token_tiles = (a.rows + TOK - 1) / TOK;
+  const int64_t whole = (int64_t)((a.n + FEATURES - 1) / FEATURES) * token_tiles;
+  const int segments = int4_segments(whole, a.deep, 140 * Int4Tile<TOK>::CTAS);
+  VOSTI_REQUIRE(whole * segments <= 0x7fffffff, "gemm_int4: too many tiles for one launch");
+  const cudaError_t e = vosti_launch_clusters(kernel, dim3((unsigned)(whole * segments)), dim3(TILE_THREADS), (unsigned)segments, SMEM, a.stream, map,
+                                              a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n, a.k, a.tiles, a.deep, token_tiles, segments, a.status);
+  VOSTI_REQUIRE(e == cudaSuccess, "gemm_int4: %s", cudaGetErrorString(e));
+  return VOSTI_OK;
+}
+template <int GROUPS>
+int launch_tiles_as(const Int4Args& a) {
+  if (a.rows <= 32) return launch_tiles<32, GROUPS>(a);
+  if (a.rows <= 64) return launch_tiles<64, GROUPS>(a);
+  if (a.rows <= 128) return launch_tiles<128, GROUPS>(a);
+  return launch_tiles<256, GROUPS>(a);
+}
+
+}  // namespace
+
+// Tensor memory columns that the CTAs of a token tile (0 .. 3, -1 beyond) may ask for on one SM.
+VOSTI_API int vosti_gemm_int4_columns_an_sm(int tile) {
+  auto of = [](int smem, int cols) { return 228 * 1024 / (smem + 1024) * cols; };
+  switch (tile) {
+    case 0: return of(Int4Tile<32>::SMEM, Int4Tile<32>::COLS);
+    case 1: return of(Int4Tile<64>::SMEM, Int4Tile<64>::COLS);
+    case 2: return of(Int4Tile<128>::SMEM, Int4Tile<128>::COLS);
+    case 3: return of(Int4Tile<256>::SMEM, Int4Tile<256>::COLS);
+  }
+  return -1;
+}
+
+// x: bfloat16 [rows, k]; codes, scales: as at the top of this file, for n features and k, group 32, 64 or 128; y: [rows, n] bfloat16, or
+// float32 with y_is_f32.
+VOSTI_API int vosti_gemm_int4(const void* x, const void* codes, const void* scales, void* y, int y_is_f32, int rows, int n, int k, int group,
+                              unsigned* status, cudaStream_t stream) {
+  VOSTI_REQUIRE(rows >= 0 && n > 0 && k > 0, "gemm_int4: bad sizes rows=%d n=%d k=%d", rows, n, k);
+  VOSTI_REQUIRE(group == 32 || group == 64 || group == 128, "gemm_int4: the group is 32, 64 or 128, not %d", group);
+  VOSTI_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 7) == 0, "gemm_int4: the weights must start on whole words");
+  if (rows == 0) return VOSTI_OK;
+  Int4Args a = {(const bf16*)x, (const uint8_t*)codes, (const bf16*)scales, y, y_is_f32, rows, n, k, (n + 15) / 16, (k + KB - 1) / KB, status, stream};
+  // whole words of eight tokens' elements: every row starts on 16 bytes
+  const bool words = k % 8 == 0 && ((uintptr_t)x & 15) == 0;
+  if (rows > 16 && words) {
+    const int code = group == 32 ? launch_tiles_as<4>(a) : group == 64 ? launch_tiles_as<2>(a) : launch_tiles_as<1>(a);
+    if (code != VOSTI_OK) return code;
+    VOSTI_LAUNCH_CHECK();
+  }
+  for (int t = 0; t < rows; t += 16) {                           // (more than one turn only where rows do not start on whole words)
+    a.x = (const bf16*)x + (int64_t)t * k;
+    a.y = (uint8_t*)y + (int64_t)t * n * (y_is_f32 ? 4 : 2);
+    a.rows = rows - t < 16 ? rows - t : 16;
+    const cudaError_t e = group == 32 ? launch_few_as<4>(a, words) : group == 64 ? launch_few_as<2>(a, words) : launch_few_as<1>(a, words);
+    if (e != cudaSuccess) {
+      vosti_set_error("gemm_int4: %s", cudaGetErrorString(e));
+      return (int)e;
+    }
+  }
+  VOSTI_LAUNCH_CHECK();
+}

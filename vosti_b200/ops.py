@@ -2455,3 +2455,98 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
             lists["max_long_q_len"], tokens, scale, window, status.data_ptr(), stream), "attention_prefill_tc_e4m3")
     return out
+
+
+class Int4Weight:
+    """A [features, k] weight in 4 bits with a bfloat16 scale for each group of 32, 64 or 128 neighbouring k: codes -8 .. 7 times their
+    scale. `codes` uint8 [features / 16, k / 128, 16 rows, 4 j, 4 i, 4 bytes] (rounded up): the 32-bit word (j, i) of a row holds its k =
+    32 i + 8 j .. + 7 of the block, nibble p the code + 8 of k offset 2 p (p < 4) or 2 p - 7. `scales` bfloat16 [features / 16, k / 128,
+    16 rows, 128 / group]. Made by `quantize` from a matrix or by `from_codes` from codes and scales of another quantizer."""
+
+    __slots__ = ("codes", "scales", "shape", "group", "device")
+    dtype = torch.uint8
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
+        features, k = (int(s) for s in shape)
+        tiles, deep = -(-features // 16), -(-k // 128)
+        if features <= 0 or k <= 0 or codes.dtype != torch.uint8 or tuple(codes.shape) != (tiles, deep, 16, 4, 4, 4):
+            raise KernelError(f"Int4Weight: codes are uint8 {(tiles, deep, 16, 4, 4, 4)} for a {features} x {k} matrix, got {codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype != torch.bfloat16 or scales.dim() != 4 or tuple(scales.shape[:3]) != (tiles, deep, 16) or scales.shape[3] not in (1, 2, 4):
+            raise KernelError(f"Int4Weight: scales are bfloat16 {(tiles, deep, 16)} x (128 / group), the group 32, 64 or 128, got {scales.dtype} {tuple(scales.shape)}")
+        if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
+            raise KernelError("Int4Weight: codes and scales are contiguous, on one device")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 8:
+            raise KernelError("Int4Weight: codes start on 16 bytes, scales on 8")
+        self.codes, self.scales, self.shape, self.group, self.device = codes, scales, (features, k), 128 // scales.shape[3], codes.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.codes.is_cuda
+
+    def numel(self) -> int:
+        return self.shape[0] * self.shape[1]
+
+    @staticmethod
+    def check_group(group: int) -> int:
+        if group not in (32, 64, 128):
+            raise KernelError(f"Int4Weight: the group is 32, 64 or 128, not {group!r}")
+        return int(group)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, group: int) -> "Int4Weight":
+        """From integer codes [features, k] in -8 .. 7 and scales [features, k / group] (rounded up), which become bfloat16."""
+        cls.check_group(group)
+        if codes.dim() != 2 or codes.dtype.is_floating_point or tuple(scales.shape) != (codes.shape[0], -(-codes.shape[1] // group)):
+            raise KernelError(f"Int4Weight: integer codes [features, k] and scales [features, k / {group}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        features, k = codes.shape
+        tiles, deep = -(-features // 16), -(-k // 128)
+        padded = torch.full((tiles * 16, deep * 128), 8, dtype=torch.uint8, device=codes.device)
+        padded[:features, :k] = (codes + 8).to(torch.uint8)
+        # [tile, row, block, i, j, offset] -> [tile, block, row, j, i, offset]; a byte holds two nibbles of the word
+        at = padded.view(tiles, 16, deep, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)
+        nibble = at[..., [0, 2, 4, 6, 1, 3, 5, 7]]
+        packed = (nibble[..., 0::2] | nibble[..., 1::2] << 4).contiguous()
+        groups = 128 // group
+        wide = torch.zeros((tiles * 16, deep * groups), dtype=torch.bfloat16, device=codes.device)
+        wide[:features, :scales.shape[1]] = scales.to(torch.bfloat16)
+        return cls(packed, wide.view(tiles, 16, deep, groups).transpose(1, 2).contiguous(), (features, k))
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, group: int = 128) -> "Int4Weight":
+        """Round to nearest: a group's scale is its largest size over 7 (in bfloat16), its codes the nearest of -8 .. 7."""
+        cls.check_group(group)
+        if w.dim() != 2 or w.dtype not in (torch.bfloat16, torch.float32):
+            raise KernelError("Int4Weight: quantize takes a 2-d bfloat16 or float32 matrix")
+        features, k = w.shape
+        padded = torch.nn.functional.pad(w.float(), (0, -k % group)).view(features, -1, group)
+        if not bool(torch.isfinite(padded).all()):
+            raise KernelError("Int4Weight: the matrix holds values that are not finite")
+        scales = (padded.abs().amax(-1) / 7).to(torch.bfloat16)
+        safe = torch.where(scales > 0, scales, torch.ones_like(scales)).float().unsqueeze(-1)
+        codes = torch.round(padded / safe).clamp_(-8, 7).to(torch.int8)
+        return cls.from_codes(codes.view(features, -1)[:, :k], scales, group)
+
+    def dequantized(self) -> torch.Tensor:
+        """The float32 [features, k] matrix that codes and scales stand for."""
+        tiles, deep = self.codes.shape[:2]
+        nibble = torch.stack([self.codes & 15, self.codes >> 4], dim=-1).flatten(-2)[..., [0, 4, 1, 5, 2, 6, 3, 7]]
+        codes = nibble.permute(0, 2, 1, 4, 3, 5).reshape(tiles, 16, deep, 128 // self.group, self.group).float() - 8
+        scales = self.scales.transpose(1, 2).float().unsqueeze(-1)
+        return (codes * scales).reshape(tiles * 16, deep * 128)[:self.shape[0], :self.shape[1]].contiguous()
+
+
+def gemm_int4(x: torch.Tensor, w: Int4Weight, status: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x @ w.T for bfloat16 rows and a weight in 4 bits, rounded once to `out_dtype` (bfloat16 or float32). Up to 16 rows a group's codes
+    are summed exactly and scaled in float32; more rows multiply codes times scales rounded to bfloat16."""
+    rows, k = x.shape
+    features = w.shape[0]
+    if x.dtype != torch.bfloat16 or k != w.shape[1]:
+        raise KernelError(f"gemm_int4: x is bfloat16 [rows, {w.shape[1]}], got {x.dtype} {tuple(x.shape)}")
+    out_dtype = out_dtype or torch.bfloat16
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"gemm_int4: the result is bfloat16 or float32, not {out_dtype}")
+    stream = _here("gemm_int4", x, w.codes, status)
+    out = torch.empty((rows, features), dtype=out_dtype, device=x.device)
+    _check(_bound("vosti_gemm_int4", "pppp" "iiiii" "pp")(x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), out_dtype == torch.float32,
+                                                          rows, features, k, w.group, status.data_ptr(), stream), "gemm_int4")
+    return out
