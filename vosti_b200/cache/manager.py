@@ -23,7 +23,7 @@ import ctypes
 
 import torch
 
-from .. import host
+from .. import host, ops
 from ..host import OutOfSlots
 from ..parts.base import PagedCacheSpec, StateSpec
 from .pages import OutOfPages, PageAccountingError, PagePool
@@ -39,6 +39,7 @@ class LayerCache:
     tensors: Tuple[torch.Tensor, ...] = ()
     state: Optional[torch.Tensor] = None
     page_size: int = 0
+    e4m3: Optional["ops.PagedE4M3"] = None       # keys and values in 8 bits, if that is how they are held
 
     @property
     def k(self):
@@ -129,7 +130,13 @@ class CacheManager:
                     layers_of.append([])
                 cache.group = by_window[reach]
                 layers_of[cache.group].append(layer)
-                if device is not None:
+                if spec.storage == "e4m3":
+                    if page_size % ops.E4M3_BLOCK:
+                        raise ValueError(f"a cache of 8 bits needs pages of a multiple of {ops.E4M3_BLOCK} tokens, got {page_size}")
+                    if device is not None:
+                        cache.tensors = ops.PagedE4M3.tensors(num_pages, spec.heads, page_size, spec.width, device)
+                        cache.e4m3 = ops.PagedE4M3(*cache.tensors)
+                elif device is not None:
                     # zeros, not empty: the decode kernel reads whole boxes of 16 keys and masks
                     # afterwards, so slots nobody wrote yet must hold finite values
                     cache.tensors = tuple(
@@ -227,11 +234,8 @@ class CacheManager:
         return list(buf[:n])
 
     def bytes_per_token(self) -> int:
-        total = 0
-        for cache in self.layer_caches:
-            for t in cache.tensors:
-                total += t.shape[1] * t.shape[3] * t.element_size()      # heads * width
-        return total
+        total = sum(t.numel() * t.element_size() for cache in self.layer_caches for t in cache.tensors)
+        return -(-total // (self.num_pages * self.page_size))      # (scales of 8-bit caches are shared by 16 tokens)
 
     def pages_for(self, tokens: int) -> int:
         return (tokens + self.page_size - 1) // self.page_size

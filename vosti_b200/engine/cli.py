@@ -19,7 +19,8 @@ meaning here, and every one also has a flag (the flag wins):
   VOSTI_ENGINE_STEP_TRACE   --step-trace       one JSON line per step
   VOSTI_CUDA_GRAPH          --cuda-graph       0/1: replay decode steps as CUDA graphs (default 1 here)
 
-Added here: --dtype {bfloat16,float32} (VOSTI_DTYPE), --block-size (VOSTI_BLOCK_SIZE, the
+Added here: --cache-dtype e4m3 (VOSTI_CACHE_DTYPE) and --weights int4 (VOSTI_WEIGHTS, --weight-group, VOSTI_WEIGHT_GROUP): keys and
+values in 8 bits, the layers' matrices in 4; --dtype {bfloat16,float32} (VOSTI_DTYPE), --block-size (VOSTI_BLOCK_SIZE, the
 reference's page size is the constant 64), --temperature, --seed, --chunk-size, and
 --random-config FILE --random-seed N [--random-shapes FILE], which first writes a random-weights
 model folder to --model. Prints MODEL_OUTPUT_TOKEN_IDS=[...] or, for a prepared workload, the BENCH and
@@ -151,6 +152,12 @@ def main(argv: Optional[List[str]] = None) -> int:
                                                               _env("VOSTI_BATCH_INVARIANT", "off")),
                         help="full: a token's bits do not depend on how the work is cut into steps and batches "
                              "(slower decoding); decode: decode steps of up to 64 rows do not depend on the batch")
+    parser.add_argument("--cache-dtype", choices=["e4m3"], default=_env("VOSTI_CACHE_DTYPE") or None,
+                        help="hold keys and values in 8 bits (pages of a multiple of 16 tokens)")
+    parser.add_argument("--weights", choices=["int4"], default=_env("VOSTI_WEIGHTS") or None,
+                        help="hold the layers' matrices in 4 bits (bfloat16 serving)")
+    parser.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=int(_env("VOSTI_WEIGHT_GROUP", 128)),
+                        help="neighbouring inputs that share a scale")
     parser.add_argument("--random-config", help="config.json to draw a random-weights model from")
     parser.add_argument("--random-seed", type=int, default=0)
     parser.add_argument("--random-shapes", help="JSON file, tensor name -> shape: the sizes an architecture's config.json "
@@ -181,7 +188,8 @@ def main(argv: Optional[List[str]] = None) -> int:
                     max_num_batched_tokens=args.max_batched_tokens, prefill_chunk_size=args.chunk_size,
                     enable_prefix_caching=not args.no_prefix_caching, step_trace=args.step_trace,
                     cuda_graphs=bool(args.cuda_graph), batch_invariant=args.batch_invariant,
-                    async_scheduling=bool(args.async_scheduling))
+                    async_scheduling=bool(args.async_scheduling), cache_dtype=args.cache_dtype, weights=args.weights,
+                    weight_group=args.weight_group)
     print(f"MODEL_RUNTIME architecture={engine.runner.spec.architecture} dtype={args.dtype} "
           f"device={args.device}", flush=True)
 

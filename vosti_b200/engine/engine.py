@@ -54,7 +54,8 @@ class Engine:
                  max_num_batched_tokens: int = 4096, prefill_chunk_size: int = 0,
                  enable_prefix_caching: bool = True, step_trace: Optional[str] = None,
                  cuda_graphs: bool = True, batch_invariant=False, async_scheduling: bool = False, spec=None,
-                 tensors=None, consume_tensors: bool = False):
+                 tensors=None, consume_tensors: bool = False, cache_dtype: Optional[str] = None,
+                 weights: Optional[str] = None, weight_group: int = 128):
         """`num_blocks` pages of `block_size` tokens; `max_num_seqs` rows and
         `max_num_batched_tokens` tokens per step at most (the reference's VOSTI_NUM_BLOCKS,
         VOSTI_MAX_SEQS, VOSTI_MAX_BATCHED_TOKENS; its page size is fixed at 64).
@@ -68,13 +69,22 @@ class Engine:
         `async_scheduling`: `step` launches the next step before it reads the last one's tokens,
         so the GPU does not idle while the host plans; the tokens a call returns are then those
         of the step launched by the call before (one call later than without it).
+        `cache_dtype` "e4m3" holds keys and values in 8 bits, with a power of two for each block of 16 tokens and head
+        (pages are then a multiple of 16 tokens); `weights` "int4" holds the layers' matrices in 4 bits, rounded to
+        nearest when they are loaded, with a scale for each `weight_group` (32, 64 or 128) inputs (bfloat16 only). A block's scale
+        follows the tokens that are in it, and the products' kernels the number of rows, so both refuse `batch_invariant`.
         `cuda_graphs`: decode steps are recorded once per shape and replayed; it is switched
         off by itself for a model with a part that declares `capture_safe = False`."""
         from .. import ops
+        if (cache_dtype or weights) and batch_invariant not in (False, None, "off", "0", ""):
+            raise ValueError("serving in few bits rounds keys, values and products by how the work is cut: not with batch_invariant")
+        if weights and not _is_bfloat16(dtype) and str(dtype) != "bf16":
+            raise ValueError("weights in 4 bits serve bfloat16 activations only")
         self.invariance = ops.set_invariance(batch_invariant) if _is_bfloat16(dtype) else None
         self.runner = ModelRunner(model, dtype=dtype, device=device, num_pages=num_blocks, page_size=block_size,
                                   max_requests=max_num_seqs, prefix_reuse=enable_prefix_caching, spec=spec,
-                                  tensors=tensors, consume_tensors=consume_tensors)
+                                  tensors=tensors, consume_tensors=consume_tensors, cache_dtype=cache_dtype, weights=weights,
+                                  weight_group=weight_group)
         spec = self.runner.spec
         self.scheduler = Scheduler(self.runner.cache, SchedulerConfig(
             max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens,

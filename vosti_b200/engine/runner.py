@@ -18,7 +18,7 @@ import torch
 
 from .. import ops
 from ..cache import CacheManager, OutOfPages
-from ..config import model_spec_from_dir, ModelSpec
+from ..config import in_few_bits, model_spec_from_dir, ModelSpec
 from ..models import build_model
 from ..weights import check_tensors, load_weights
 from .batch import StagingBuffer, StepContext, StepEntry, build_context
@@ -49,11 +49,12 @@ class ModelRunner:
     def __init__(self, model_dir: Optional[str | Path] = None, *, dtype="bfloat16", device="cuda:0",
                  num_pages: int, page_size: int = 16, max_requests: int = 64, prefix_reuse: bool = False,
                  spec: Optional[ModelSpec] = None, tensors: Optional[Dict[str, torch.Tensor]] = None,
-                 consume_tensors: bool = False):
+                 consume_tensors: bool = False, cache_dtype: Optional[str] = None, weights: Optional[str] = None,
+                 weight_group: int = 128):
         """`tensors` (name -> tensor, already on the device) stands in for a model folder.
         With `consume_tensors` the dictionary is emptied once the parts have taken what they
         keep, before the cache is allocated, so that weights the parts re-packed do not stay in
-        memory twice."""
+        memory twice. `cache_dtype`, `weights`, `weight_group`: see `config.in_few_bits`."""
         self.device = torch.device(device)
         self.dtype = parse_dtype(dtype)
         ops.require_device(self.device)
@@ -61,7 +62,8 @@ class ModelRunner:
         torch.cuda.set_device(self.device)
         if torch.backends.cuda.matmul.allow_tf32:
             torch.backends.cuda.matmul.allow_tf32 = False
-        self.spec = spec if spec is not None else model_spec_from_dir(model_dir)
+        self.spec = in_few_bits(spec if spec is not None else model_spec_from_dir(model_dir), cache=cache_dtype, weights=weights,
+                                weight_group=weight_group)
         self.model = build_model(self.spec)
         expected = self.model.expected_weights()
         if tensors is None:

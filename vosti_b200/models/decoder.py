@@ -172,6 +172,8 @@ class DecoderModel:
             for value in vars(obj).values():
                 if isinstance(value, ops.PackedWeight):
                     value = value.data
+                if isinstance(value, ops.Int4Weight):
+                    value = [value.codes, value.scales]
                 if isinstance(value, torch.Tensor) and value.is_cuda:
                     base = value.untyped_storage().data_ptr()
                     if base not in seen:

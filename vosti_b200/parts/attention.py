@@ -9,7 +9,8 @@ limited to a window; output projection. Sizes and constants are parameters of th
 num_heads, num_kv_heads, head_dim, scale, window (0 = all keys), head_norm_eps (None =
 no head norm), qkv_bias and o_bias (false for Qwen3, whose configuration must say
 attention_bias=false; true adds `{q,k,v}_proj.bias` / `o_proj.bias` to the tensors the part
-asks for, added to the float32 products before they are rounded).
+asks for, added to the float32 products before they are rounded). `cache` "e4m3" holds keys and values in
+8 bits (ops.PagedE4M3), `weights` "int4" the two matrices in 4 (ops.Int4Weight, `weight_group` inputs a scale).
 """
 from __future__ import annotations
 
@@ -21,7 +22,7 @@ from .. import ops
 from ..config.schema import ConfigError, PartSpec
 from ..weights.loader import WeightSpec
 from .base import Mixer, PagedCacheSpec, PositionEncoding, register_part, register_step_layout
-from .linear import linear, prepare_weight
+from .linear import linear, prepare_weight, weight_group_of
 
 
 class Attention(Mixer):
@@ -41,6 +42,9 @@ class Attention(Mixer):
             raise ConfigError(f"attention: head_dim {self.d} must be a multiple of 16, at most 256")
         if self.window < 0:
             raise ConfigError("attention: window must be >= 0")
+        if spec.get("cache") not in (None, "e4m3"):
+            raise ConfigError(f"attention: the cache is 'e4m3' or left out, not {spec.get('cache')!r}")
+        self.eight_bits, self.weight_group = spec.get("cache") == "e4m3", weight_group_of(spec)
         self.qkv_bias, self.o_bias = bool(spec.get("qkv_bias", False)), bool(spec.get("o_bias", False))
         self.w_qkv = self.w_q = self.w_o = self.q_norm = self.k_norm = self.b_qkv = self.b_o = None
 
@@ -65,11 +69,11 @@ class Attention(Mixer):
         common = torch.float32 if any(p.dtype == torch.float32 for p in parts) else parts[0].dtype
         # one [ (nq + 2 nkv) d, hidden ] matrix: the projection is a single product
         w_qkv = torch.cat([p.to(common) for p in parts], dim=0).contiguous()
-        self.w_qkv = prepare_weight(w_qkv, dtype)
+        self.w_qkv = prepare_weight(w_qkv, dtype, self.weight_group)
         # a layer that reads another layer's cache needs q only: the first rows of the matrix,
         # or (tile-packed weight) the whole product, whose k and v are then dropped
         self.w_q = w_qkv[: self.nq * self.d] if self.w_qkv is w_qkv else None
-        self.w_o = prepare_weight(tensors["o_proj.weight"], dtype)
+        self.w_o = prepare_weight(tensors["o_proj.weight"], dtype, self.weight_group)
         if self.qkv_bias:
             self.b_qkv = torch.cat([tensors[f"{p}_proj.bias"].float() for p in "qkv"]).contiguous()
         if self.o_bias:
@@ -87,7 +91,7 @@ class Attention(Mixer):
         return self.w_qkv
 
     def cache_spec(self) -> PagedCacheSpec:
-        return PagedCacheSpec(entries=2, heads=self.nkv, width=self.d, window=self.window)
+        return PagedCacheSpec(entries=2, heads=self.nkv, width=self.d, window=self.window, storage="e4m3" if self.eight_bits else "")
 
     def forward(self, ctx, x, cache, writes_cache: bool = True):
         group = ctx.group(cache.group)
@@ -100,6 +104,10 @@ class Attention(Mixer):
                       positions=ctx.positions, status=ctx.status, rotary_dim=rotary_dim, interleaved=interleaved)
         if writes_cache:
             qkv = linear(ctx, x, self.w_qkv, allow_partial=True, bias=self.b_qkv)   # summed inside qkv_post
+            if self.eight_bits:
+                common.pop("page_size")
+                q = ops.qkv_post_e4m3(qkv, cache.e4m3, nkv=self.nkv, k_norm_w=self.k_norm, slot_mapping=group.slot_mapping, **common)
+                return self._out(ctx, q, cache, group)
             if (ops.DECODE_FUSION and isinstance(qkv, ops.PartialSum) and qkv.dtype == torch.bfloat16
                     and ctx.layout["attention"]["num_short_tokens"] == ctx.num_tokens == ctx.num_requests
                     and self.nq // self.nkv <= 16 and cache.k.dtype == torch.bfloat16
@@ -122,8 +130,15 @@ class Attention(Mixer):
         else:
             q = ops.qkv_post(linear(ctx, x, self.w_qkv, allow_partial=True, bias=self.b_qkv), None, None, nkv=self.nkv,
                              k_norm_w=self.k_norm, slot_mapping=None, **common)
-        attn = ops.attention(ctx, q, cache.k, cache.v, group, nq=self.nq, nkv=self.nkv, head_dim=self.d,
-                             scale=self.scale, window=self.window)
+        return self._out(ctx, q, cache, group)
+
+    def _out(self, ctx, q, cache, group):
+        """Attention of the rotated queries and the output projection."""
+        sizes = dict(nq=self.nq, nkv=self.nkv, head_dim=self.d, scale=self.scale, window=self.window)
+        if self.eight_bits:
+            attn = ops.attention_e4m3(ctx, q, cache.e4m3, group, **sizes)
+        else:
+            attn = ops.attention(ctx, q, cache.k, cache.v, group, **sizes)
         return linear(ctx, attn, self.w_o, allow_partial=True, bias=self.b_o)   # summed by the norm that follows
 
 

@@ -40,7 +40,8 @@ class PagedCacheSpec:
     """Per-token cache of a mixer: `entries` tensors (keys and values: 2), each
     [tokens, heads, width] per token; `window` > 0 means only the last `window`
     tokens, and a request's first `keep_first`, are ever read again, so the pages
-    between them may be given back."""
+    between them may be given back. `storage` "e4m3": the two entries are keys and values in 8 bits with
+    their scales (ops.PagedE4M3) instead of tensors of the serving type."""
 
     entries: int
     heads: int
@@ -48,6 +49,7 @@ class PagedCacheSpec:
     window: int = 0
     keep_first: int = 0
     widths: Tuple[int, ...] = ()      # width of every entry where they differ (else `width` for all)
+    storage: str = ""
 
     def entry_widths(self) -> Tuple[int, ...]:
         return tuple(self.widths) if self.widths else (self.width,) * self.entries

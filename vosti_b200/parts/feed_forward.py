@@ -11,7 +11,8 @@ float32: the down projection is then not rounded to the serving type, and `activ
 (the default), "relu" or "relu2" (the square of relu) on the gate, or with `bias` "clamped": g sigmoid(`sigmoid_scale` g)
 (u + 1) of g = min(gate x + bg, `limit`) and u = up x + bu clamped to [-limit, limit]. `bias`: all three projections have
 biases (the tensor's name with ".b"); the down projection's joins in the kernel that reads the product next
-(an arrangement that asks for `out_bias`), the others in the activation.
+(an arrangement that asks for `out_bias`), the others in the activation. `weights` "int4" (without `bias`): the matrices in 4 bits,
+with a scale for each `weight_group` inputs (ops.Int4Weight).
 
 `ExpertMixture` is the same feed-forward as `experts` small ones, of which each token uses
 the `top` with the largest router logits, weighted by the softmax over the chosen logits only.
@@ -31,7 +32,7 @@ from .. import ops
 from ..config.schema import ConfigError, PartSpec
 from ..weights.loader import WeightSpec
 from .base import FeedForward, register_part
-from .linear import linear, prepare_weight, uses_tensor_cores
+from .linear import linear, prepare_weight, uses_tensor_cores, weight_group_of
 
 
 def stack_gate_up(gate: torch.Tensor, up: torch.Tensor, dtype: torch.dtype, activation: str = "silu"):
@@ -81,6 +82,9 @@ class SwiGLU(FeedForward):
                 raise ConfigError("swiglu: the clamped activation's limit must be positive")
         if self.activation not in ops.GLU_ACTIVATIONS:
             raise ConfigError(f"swiglu: activation is one of {sorted(ops.GLU_ACTIVATIONS)}")
+        self.weight_group = weight_group_of(spec)
+        if self.weight_group and self.has_bias:
+            raise ConfigError("swiglu: matrices in 4 bits go without biases")
         self.w_gate_up = self.w_down = None
         self.fused = self.fused_packed = False
 
@@ -94,7 +98,11 @@ class SwiGLU(FeedForward):
 
     def load(self, tensors, dtype):
         gate, up, down = self.names
-        self.w_down = prepare_weight(tensors[down], dtype)
+        self.w_down = prepare_weight(tensors[down], dtype, self.weight_group)
+        if self.weight_group:
+            common = torch.float32 if torch.float32 in (tensors[gate].dtype, tensors[up].dtype) else tensors[gate].dtype
+            self.w_gate_up = prepare_weight(torch.cat([tensors[gate].to(common), tensors[up].to(common)]), dtype, self.weight_group)
+            return
         if self.has_bias:
             pair, biases = (tensors[gate], tensors[up]), (tensors[gate + ".b"].float(), tensors[up + ".b"].float())
             # blocks of 16 gate and 16 up rows where the tensor-core product may apply the activation itself

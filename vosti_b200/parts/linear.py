@@ -1,5 +1,6 @@
 """Matrix product y = x @ w.T for the parts, choosing the kernel by operand types.
 
+A weight in 4 bits (`ops.Int4Weight`) has a product of its own.
 bfloat16 x bfloat16 goes to the tensor-core kernel when it takes the sizes, float32 x float32 to the
 tensor-core kernel that splits every operand into three bfloat16 terms (float32 results, no reduced precision);
 every other combination (a 32-bit weight under bfloat16 serving, sizes those kernels refuse) goes to the
@@ -14,6 +15,7 @@ from typing import Optional
 import torch
 
 from .. import ops
+from ..config.schema import ConfigError
 
 # VOSTI_PACK_WEIGHTS=0 keeps weights row-major (for comparisons; the results are the same bits).
 PACK_WEIGHTS = os.environ.get("VOSTI_PACK_WEIGHTS", "1") != "0"
@@ -29,10 +31,26 @@ def uses_split_float32(x_dtype: torch.dtype, w) -> bool:
             and ops.gemm_f32_supported(w.shape[0], w.shape[1]))
 
 
-def prepare_weight(w: torch.Tensor, serving_dtype: torch.dtype):
+def weight_group_of(spec) -> int:
+    """Neighbouring inputs with one scale, for a part whose spec asks for weights in 4 bits (parameters `weights` "int4" and
+    `weight_group`); 0 for one whose weights stay in the serving type."""
+    kind = spec.get("weights")
+    if kind is None:
+        return 0
+    if kind != "int4":
+        raise ConfigError(f"part '{spec.kind}': weights are 'int4' or left out, not {kind!r}")
+    return ops.Int4Weight.check_group(int(spec.get("weight_group", 128)))
+
+
+def prepare_weight(w: torch.Tensor, serving_dtype: torch.dtype, group: int = 0):
     """What a part keeps of a [features, k] weight it only ever multiplies with: the
     tile-packed copy if the tensor-core product will read it, else the tensor itself. A
-    weight that is also read by rows (a tied embedding table) must stay a tensor."""
+    weight that is also read by rows (a tied embedding table) must stay a tensor. With `group` the weight is rounded to
+    4 bits with a scale for each group of so many inputs."""
+    if group:
+        if serving_dtype != torch.bfloat16:
+            raise ops.KernelError("weights in 4 bits serve bfloat16 activations only")
+        return ops.Int4Weight.quantize(w, group)
     if PACK_WEIGHTS and isinstance(w, torch.Tensor) and uses_tensor_cores(serving_dtype, w):
         return ops.PackedWeight(w)
     return w
@@ -53,6 +71,10 @@ def linear(ctx, x: torch.Tensor, w: torch.Tensor, *, out_dtype: Optional[torch.d
             raise ops.KernelError(f"linear: bias has shape {tuple(bias.shape)}, the weight has {w.shape[0]} rows")
         product = linear(ctx, x, w, out_dtype=torch.float32, row_index=row_index)
         return ops.affine_rows(product, bias=bias, out_dtype=out_dtype or x.dtype)
+    if isinstance(w, ops.Int4Weight):
+        if row_index is not None:
+            x = ops.gather_rows(x, row_index, ctx.status)
+        return ops.gemm_int4(x, w, ctx.status, out_dtype=out_dtype)
     if isinstance(w, ops.PackedWeight) and x.dtype != torch.bfloat16:
         raise ops.KernelError("a tile-packed weight serves bfloat16 activations only")
     if uses_tensor_cores(x.dtype, w):
