@@ -29,13 +29,21 @@ struct CacheArgs {
 //     64 c + 16 j .. + 15 (j = lane % 4): four k-steps of four features. Rows of S^T are chosen so that the weights come out
 //     where the second product wants them: row r of step s is token 4 s + r % 2 (+ 2 for rows 8 to 15) of block r % 8 / 2.
 //   * a lane's 16 bytes of a value row are one feature's 16 tokens of block j: four k-steps of four tokens.
-//   * the weights turn from (key, head) into (head, key) by movmatrix on pairs rounded to bfloat16.
-// Payloads become bfloat16 by moving their bits and one multiplication by the block's scale, which is exact.
-// What bounds it is the cache's bytes; the conversion is some five instructions for two values.
-constexpr int WARPS = 4, THREADS = WARPS * 32;
+//   * the weights turn from (key, head) into (head, key) by movmatrix on pairs rounded to float16.
+// Payloads become float16, exactly, by one conversion for two of them; scales never touch them. A lane's scores are all of one block, so the
+// keys' scale is a factor of the scores, and the values' one joins the weights in the exponent: the products sum
+// 2^(s_j + log2 scale_j - M + 15) payload_j with a running maximum M of s_j + log2 scale_j of their own, so that a weight is 2^15 at
+// most whatever the scales are, and full float16 precision reaches 2^-29 of the largest (2^-39 of it is the smallest), while the denominator sums
+// 2^(s_j - m) under the scores' own maximum. Queries become float16 too, a row times the power of two that brings
+// its largest to 2^14 .. 2^15: exact down to 2^-28 of it.
+// What bounds it is the cache's bytes. (Payloads made bfloat16 by moving their bits, four integer instructions and a multiplication for two, kept
+// the integer pipe busy: 96 us for 64 tokens at 600 to 3,500 keys, 75 for eight at 16,384.)
+constexpr int RESIDENT = 8;                // warps an SM holds of the kernel's registers
+constexpr int MAX_WARPS = 4;
 constexpr int TILE = 64;                   // keys of a warp's step: four blocks
 constexpr int HEADS = 8;                   // query heads of a CTA
 constexpr int MAX_SEGMENTS = 16;
+constexpr int MAX_ORDERED = 256;           // tokens of a launch that starts with the longest
 
 __device__ __forceinline__ uint4 load_line(const uint8_t* p) {
   uint4 v;
@@ -44,6 +52,28 @@ __device__ __forceinline__ uint4 load_line(const uint8_t* p) {
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Payload bytes 0 and 1 (2 and 3) of a word in float16.
+__device__ __forceinline__ uint32_t lower_f16(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t upper_f16(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -54,27 +84,26 @@ __device__ __forceinline__ uint32_t cluster_rank_of() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float load_of_rank(const float* p, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_at_rank(float* p, uint32_t rank, float v) {
   uint32_t at;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
-template <int D>
-__global__ void __launch_bounds__(THREADS, 2)
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, RESIDENT / WARPS)
 attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const CacheArgs c, const int* __restrict__ token_list,
                       const int* __restrict__ positions, const int* __restrict__ request_of, int nq, int nkv, float scale_log2, int window,
-                      int segments, unsigned* status) {
-  constexpr int CHUNKS = D / 64, FT = D / 16;
-  constexpr int REC = D + 2;                                   // a head's record: largest score, sum, products
-  __shared__ float part[WARPS][HEADS][REC];
-  __shared__ float whole[HEADS][REC];
+                      int segments, int ordered, unsigned* status) {
+  constexpr int CHUNKS = D / 64, FT = D / 16, THREADS = WARPS * 32;
+  constexpr int RAISED = 15;
+  __shared__ float part[WARPS][HEADS][D + 4];                  // the warps' products, under the CTA's maximum
+  __shared__ float stats[WARPS][HEADS][3];                     // m, sum, M
+  __shared__ float inbox[HEADS * D + MAX_SEGMENTS];            // of each segment, its products of this CTA's share of the row
+  __shared__ float inbox_stats[MAX_SEGMENTS][HEADS][3];
+  if (segments > 1) cluster_arrive();                          // (waited for before the first store to another CTA)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = lane & 3, r8 = lane >> 2;
   const int group = nq / nkv, halves = (group + HEADS - 1) / HEADS;
@@ -82,7 +111,31 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   int item = blockIdx.x / segments;
   const int part_of_group = item % halves;
   item /= halves;
-  const int g = item % nkv, t = token_list ? token_list[item / nkv] : item / nkv;
+  const int g = item % nkv;
+  item /= nkv;
+  if (ordered > 0) {
+    // CTAs that start later than others take the tokens with fewer keys: the item's place is a rank among all tokens
+    __shared__ __align__(16) int keys_of[MAX_ORDERED];
+    __shared__ int chosen;
+    for (int i = threadIdx.x; i < (ordered + 3) / 4 * 4; i += THREADS) {
+      const int p = i < ordered ? positions[token_list ? token_list[i] : i] : -1;
+      keys_of[i] = i < ordered ? p - first_visible_key(p, window) : -0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ordered; i += THREADS) {
+      const int mine = keys_of[i];
+      int rank = 0;
+      for (int k = 0; k < ordered; k += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(keys_of + k);
+        rank += (v.x > mine || (v.x == mine && k < i)) + (v.y > mine || (v.y == mine && k + 1 < i)) + (v.z > mine || (v.z == mine && k + 2 < i)) +
+                (v.w > mine || (v.w == mine && k + 3 < i));
+      }
+      if (rank == item) chosen = i;
+    }
+    __syncthreads();
+    item = chosen;
+  }
+  const int t = token_list ? token_list[item] : item;
   const int heads = min(HEADS, group - part_of_group * HEADS);
   const int64_t q_at = ((int64_t)t * nq + g * group + part_of_group * HEADS) * D;
   const int pos = positions[t], req = request_of[t];
@@ -107,7 +160,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   };
 
   uint4 kk[4][2][CHUNKS];                                      // [step][rows 0-7, 8-15][chunk]
-  int k_exp = 0, v_exp = 0;
+  int k_exp = 0, v_exp = 0;                                    // scales of block lane / 8, the block of this lane's scores
   auto load_keys = [&](int64_t block) {
     const int64_t mine = __shfl_sync(0xffffffffu, block, lane >> 3);
     const uint8_t* const at = c.k + mine * (E4M3_BLOCK * D) + (r8 & 1) * D + 16 * j;
@@ -118,29 +171,53 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ++ch) kk[s][h][ch] = load_line(at + (4 * s + 2 * h) * D + 64 * ch);
     k_exp = c.k_scale[mine];
+    v_exp = c.v_scale[mine];
   };
 
   int64_t block = begin + warp < end ? block_of(begin + warp) : 0;
   pdl_wait();
   pdl_launch_dependents();
+  if (begin + warp < end) load_keys(block);
   uint32_t qb[CHUNKS][4][2];                                   // Q^T: [chunk][k-step][features 4 w, + 2]
+  float q_scale[2];                                            // what heads 2 j and 2 j + 1 were divided by, times scale_log2
+  {
+    uint4 raw[CHUNKS][2];
+    uint32_t top = 0;                                          // largest size of the row, as bits of a bfloat16
 #pragma unroll
-  for (int ch = 0; ch < CHUNKS; ++ch) {
-    uint4 u = make_uint4(0, 0, 0, 0), v = u;
-    if (r8 < heads) {
-      const uint4* const at = reinterpret_cast<const uint4*>(q + q_at + (int64_t)r8 * D + 64 * ch + 16 * j);
-      u = at[0];
-      v = at[1];
+    for (int ch = 0; ch < CHUNKS; ++ch) {
+      raw[ch][0] = raw[ch][1] = make_uint4(0, 0, 0, 0);
+      if (r8 < heads) {
+        const uint4* const at = reinterpret_cast<const uint4*>(q + q_at + (int64_t)r8 * D + 64 * ch + 16 * j);
+        raw[ch][0] = at[0];
+        raw[ch][1] = at[1];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = word_of(raw[ch][i >> 2], i & 3) & 0x7fff7fffu;
+        top = max(top, max(w & 0xffffu, w >> 16));
+      }
     }
-    qb[ch][0][0] = u.x, qb[ch][0][1] = u.y, qb[ch][1][0] = u.z, qb[ch][1][1] = u.w;
-    qb[ch][2][0] = v.x, qb[ch][2][1] = v.y, qb[ch][3][0] = v.z, qb[ch][3][1] = v.w;
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^(14 - exponent) as exponent bits, and its inverse
+    const int biased = min(max((int)(top >> 7), 15), 254);
+    const float up = __uint_as_float((uint32_t)(268 - biased) << 23), down = __uint_as_float((uint32_t)(biased - 14) << 23);
+#pragma unroll
+    for (int ch = 0; ch < CHUNKS; ++ch)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = word_of(raw[ch][i >> 2], i & 3);
+        qb[ch][i >> 1][i & 1] = pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) q_scale[h] = __shfl_sync(0xffffffffu, down, (2 * j + h) * 4) * scale_log2;
   }
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // of heads 2 j and 2 j + 1
+  float mv[2] = {-INFINITY, -INFINITY};                        // the products' M
   float o[FT][4];
 #pragma unroll
   for (int i = 0; i < FT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  if (begin + warp < end) load_keys(block);
   for (int tile = begin + warp; tile < end; tile += WARPS) {
     // this tile's values, and where the next one lies
     uint4 vv[FT][2];                                           // [16 features][rows 0-7, 8-15]
@@ -150,63 +227,77 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
       vv[i][0] = load_line(v_at + i * 16 * E4M3_BLOCK);
       vv[i][1] = load_line(v_at + i * 16 * E4M3_BLOCK + 8 * E4M3_BLOCK);
     }
-    v_exp = c.v_scale[block];
     const int64_t next = block_of(tile + WARPS);
 
     // ---- S^T = K Q^T
     float s[4][4];
-    {
-      const E4m3Factor f = e4m3_factor(k_exp);
-      const bool twice = __any_sync(0xffffffffu, f.second != E4M3_ONE);
+    const float k_times = e4m3_scale(k_exp);
+    float v_log = v_exp == E4M3_NAN_SCALE ? __uint_as_float(0x7fffffffu) : (float)(v_exp - 127);
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        s[st][0] = s[st][1] = s[st][2] = s[st][3] = 0.f;
+    for (int st = 0; st < 4; ++st) {
+      s[st][0] = s[st][1] = s[st][2] = s[st][3] = 0.f;
 #pragma unroll
-        for (int ch = 0; ch < CHUNKS; ++ch)
+      for (int ch = 0; ch < CHUNKS; ++ch)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t lo = word_of(kk[st][0][ch], w), hi = word_of(kk[st][1][ch], w);
-            uint32_t a[4] = {e4m3_widen<0>(lo, f), e4m3_widen<0>(hi, f), e4m3_widen<1>(lo, f), e4m3_widen<1>(hi, f)};
-            if (twice)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) a[i] = bf16x2_times(a[i], f.second);
-            mma_bf16(s[st], a, qb[ch][w][0], qb[ch][w][1]);
-          }
-      }
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t lo = word_of(kk[st][0][ch], w), hi = word_of(kk[st][1][ch], w);
+          const uint32_t a[4] = {lower_f16(lo), lower_f16(hi), upper_f16(lo), upper_f16(hi)};
+          mma_f16(s[st], a, qb[ch][w][0], qb[ch][w][1]);
+        }
     }
     if (tile + WARPS < end) load_keys(next);
 
     // ---- online softmax of the lane's two heads over the warp's 64 keys
     const int key_lane = tile * TILE + (lane >> 3) * E4M3_BLOCK + (r8 & 1);        // + 4 st (+ 2)
     const bool edge = tile * TILE < kstart || tile * TILE + TILE - 1 > pos;
+    const float factor[2] = {q_scale[0] * k_times, q_scale[1] * k_times};
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[st][e] *= scale_log2;
+        s[st][e] *= factor[e & 1];
         if (edge) {
           const int key = key_lane + 4 * st + (e >> 1) * 2;
           if (key < kstart || key > pos) s[st][e] = -INFINITY;
         }
         top[e & 1] = fmaxf(top[e & 1], s[st][e]);
       }
+    if (edge && top[0] == -INFINITY && top[1] == -INFINITY) v_log = 0.f;        // (nothing of this lane's block is visible, whatever it holds)
     float alpha[2];
+    uint32_t p[4][2];                                          // P^T: [step][tokens 4 s, + 2]
+    {
+      float w[4][4];                                           // the products' weights
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
+        float top_v = top[h] + v_log;
 #pragma unroll
-      for (int x = 4; x <= 16; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
-      const float m_new = fmaxf(m[h], top[h]), safe = m_new == -INFINITY ? 0.f : m_new;
-      alpha[h] = fast_exp2(m[h] - safe);
-      m[h] = m_new;
-      float sum = 0.f;
+        for (int x = 4; x <= 16; x <<= 1) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
+          top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, x));
+        }
+        const float m_new = fmaxf(m[h], top[h]), safe = m_new == -INFINITY ? 0.f : m_new;
+        const float mv_new = fmaxf(mv[h], top_v), less = v_log + RAISED - (mv_new == -INFINITY ? 0.f : mv_new);
+        const float keep = fast_exp2(m[h] - safe);
+        alpha[h] = mv_new == mv[h] ? 1.f : fast_exp2(mv[h] - mv_new);
+        m[h] = m_new;
+        mv[h] = mv_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int e = h; e < 4; e += 2) {
+            sum += fast_exp2(s[st][e] - safe);
+            w[st][e] = fast_exp2(s[st][e] + less);
+            if (edge && s[st][e] == -INFINITY) w[st][e] = 0.f;  // (a scale that is no number)
+          }
+        l[h] = l[h] * keep + sum;                              // the lane's share; added up at the end
+      }
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
-        s[st][h] = fast_exp2(s[st][h] - safe);
-        s[st][h + 2] = fast_exp2(s[st][h + 2] - safe);
-        sum += s[st][h] + s[st][h + 2];
+        p[st][0] = turn8x8(pack_f16(w[st][0], w[st][1]));
+        p[st][1] = turn8x8(pack_f16(w[st][2], w[st][3]));
       }
-      l[h] = l[h] * alpha[h] + sum;                            // the lane's share; added up at the end
     }
     if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -216,12 +307,6 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
         o[i][2] *= alpha[0];
         o[i][3] *= alpha[1];
       }
-    }
-    uint32_t p[4][2];                                          // P^T: [step][tokens 4 s, + 2]
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      p[st][0] = turn8x8(pack_bf16(s[st][0], s[st][1]));
-      p[st][1] = turn8x8(pack_bf16(s[st][2], s[st][3]));
     }
 
     // ---- O^T += V^T P^T
@@ -236,7 +321,6 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
         for (int b = 0; b < 4; ++b)
           if (key0 + 4 * w + b >= kstart && key0 + 4 * w + b <= pos) keep[w] |= 0xffu << (8 * b);
       }
-      if ((keep[0] | keep[1] | keep[2] | keep[3]) == 0) v_exp = 0;
 #pragma unroll
       for (int i = 0; i < FT; ++i)
 #pragma unroll
@@ -247,107 +331,125 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
           vv[i][h].w &= keep[3];
         }
     }
-    {
-      const E4m3Factor f = e4m3_factor(v_exp);
-      const bool twice = __any_sync(0xffffffffu, f.second != E4M3_ONE);
 #pragma unroll
-      for (int i = 0; i < FT; ++i)
+    for (int i = 0; i < FT; ++i)
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const uint32_t lo = word_of(vv[i][0], st), hi = word_of(vv[i][1], st);
-          uint32_t a[4] = {e4m3_widen<0>(lo, f), e4m3_widen<0>(hi, f), e4m3_widen<1>(lo, f), e4m3_widen<1>(hi, f)};
-          if (twice)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) a[x] = bf16x2_times(a[x], f.second);
-          mma_bf16(o[i], a, p[st][0], p[st][1]);
-        }
-    }
+      for (int st = 0; st < 4; ++st) {
+        const uint32_t lo = word_of(vv[i][0], st), hi = word_of(vv[i][1], st);
+        const uint32_t a[4] = {lower_f16(lo), lower_f16(hi), upper_f16(lo), upper_f16(hi)};
+        mma_f16(o[i], a, p[st][0], p[st][1]);
+      }
     block = next;
   }
 
-  // ---- the four warps' records into one, in warp order
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int x = 4; x <= 16; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+  // ---- the warps' sums into one, in warp order
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float* const rec = part[warp][2 * j + h];
-    if (r8 == 0) {
-      rec[0] = m[h];
-      rec[1] = l[h];
-    }
 #pragma unroll
-    for (int i = 0; i < FT; ++i) {
-      rec[2 + 16 * i + r8] = o[i][h];
-      rec[2 + 16 * i + 8 + r8] = o[i][h + 2];
+    for (int x = 4; x <= 16; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+    if (r8 == 0) {
+      stats[warp][2 * j + h][0] = m[h];
+      stats[warp][2 * j + h][1] = l[h];
+      stats[warp][2 * j + h][2] = mv[h];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += THREADS) {
-    const int h = i / D, f = i % D;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w][h][0]);
-    const float safe = top == -INFINITY ? 0.f : top;
+  for (int h = 0; h < 2; ++h) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float weight = fast_exp2(part[w][h][0] - safe);
-      sum += part[w][h][1] * weight;
-      v += part[w][h][2 + f] * weight;
-    }
-    if (segments == 1) {
-      out[q_at + i] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
-    } else {
-      whole[h][2 + f] = v;
-      if (f == 0) {
-        whole[h][0] = top;
-        whole[h][1] = sum;
-      }
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, stats[w][2 * j + h][2]);
+    const float weight = fast_exp2(mv[h] - (top == -INFINITY ? 0.f : top));
+    float* const to = part[warp][2 * j + h];
+#pragma unroll
+    for (int i = 0; i < FT; ++i) {
+      to[16 * i + r8] = o[i][h] * weight;
+      to[16 * i + 8 + r8] = o[i][h + 2] * weight;
     }
   }
-  if (segments == 1) return;
-  // ---- the segments' records, in their order; each CTA of the cluster takes a share of the row
-  cluster_sync();
-  for (int i = seg * THREADS + threadIdx.x; i < heads * D; i += segments * THREADS) {
-    const int h = i / D, f = i % D;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
-    for (int s = 0; s < segments; ++s) top = fmaxf(top, load_of_rank(&whole[h][0], s));
-    const float safe = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < segments; ++s) {
-      const float weight = fast_exp2(load_of_rank(&whole[h][0], s) - safe);
-      sum += load_of_rank(&whole[h][1], s) * weight;
-      v += load_of_rank(&whole[h][2 + f], s) * weight;
+  __syncthreads();
+  // (m, sum, M) of a head over all records of `from`
+  struct Stats { float m, sum, mv; };
+  auto joined = [](const float (*from)[HEADS][3], int count, int h) {
+    Stats r = {-INFINITY, 0.f, -INFINITY};
+    for (int w = 0; w < count; ++w) {
+      r.m = fmaxf(r.m, from[w][h][0]);
+      r.mv = fmaxf(r.mv, from[w][h][2]);
     }
-    out[q_at + i] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
+    const float safe = r.m == -INFINITY ? 0.f : r.m;
+    for (int w = 0; w < count; ++w) r.sum += from[w][h][1] * fast_exp2(from[w][h][0] - safe);
+    return r;
+  };
+  // products / 2^RAISED, divided by the sum, their maximum against the scores'
+  auto finish = [](float v, const Stats& r) {
+    const float safe = r.m == -INFINITY ? 0.f : r.m, safe_v = r.mv == -INFINITY ? 0.f : r.mv;
+    return __float2bfloat16_rn(r.sum == 0.f ? 0.f : v * (1.f / (1 << RAISED)) / r.sum * exp2f(safe_v - safe));
+  };
+  const int total = heads * D;
+  if (segments == 1) {
+    for (int i = threadIdx.x; i < total; i += THREADS) {
+      const int h = i / D, f = i % D;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) v += part[w][h][f];
+      out[q_at + i] = finish(v, joined(stats, WARPS, h));
+    }
+    return;
   }
-  cluster_sync();                                              // nobody reads this CTA's record after this
+  // ---- the segments' sums into one, in their order: each CTA of the cluster is sent its share of the row by all of them
+  const int share = (total + segments - 1) / segments;
+  cluster_wait();
+  for (int i = threadIdx.x; i < total; i += THREADS) {
+    const int h = i / D, f = i % D;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v += part[w][h][f];
+    store_at_rank(&inbox[seg * share + i % share], i / share, v);
+  }
+  for (int i = threadIdx.x; i < heads * segments; i += THREADS) {
+    const int h = i / segments;
+    const Stats r = joined(stats, WARPS, h);
+    store_at_rank(&inbox_stats[seg][h][0], i % segments, r.m);
+    store_at_rank(&inbox_stats[seg][h][1], i % segments, r.sum);
+    store_at_rank(&inbox_stats[seg][h][2], i % segments, r.mv);
+  }
+  cluster_arrive();
+  cluster_wait();                                              // all of it has arrived; nobody stores to this CTA after this
+  for (int i = threadIdx.x; i < share && seg * share + i < total; i += THREADS) {
+    const int h = (seg * share + i) / D;
+    const Stats r = joined(inbox_stats, segments, h);
+    const float safe_v = r.mv == -INFINITY ? 0.f : r.mv;
+    float v = 0.f;
+    for (int s = 0; s < segments; ++s) v += inbox[s * share + i] * fast_exp2(inbox_stats[s][h][2] - safe_v);
+    out[q_at + seg * share + i] = finish(v, r);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- CUDA cores
+constexpr int SIMT_WARPS = 4, SIMT_THREADS = SIMT_WARPS * 32;
 // One CTA for (token, query head), four warps that take 32 keys in turn: a lane multiplies a whole key (its row is contiguous),
 // then takes features, whose 16 values of a block are contiguous. All of it float32.
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(SIMT_THREADS)
 attention_e4m3_simt_kernel(const T* __restrict__ q, T* __restrict__ out, const CacheArgs c, const int* __restrict__ positions,
                            const int* __restrict__ request_of, int nq, int nkv, int d, float scale_log2, int window, unsigned* status) {
   constexpr int STEP = 2 * E4M3_BLOCK, MAX_D = 256;
   __shared__ __align__(16) float q_s[MAX_D];
-  __shared__ __align__(16) float p_s[WARPS][STEP];
-  __shared__ float rec[WARPS][MAX_D + 2];
+  __shared__ __align__(16) float p_s[SIMT_WARPS][STEP];
+  __shared__ float rec[SIMT_WARPS][MAX_D + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = blockIdx.x, head = blockIdx.y, g = head / (nq / nkv);
   pdl_wait();
   pdl_launch_dependents();
   const int64_t at = ((int64_t)t * nq + head) * d;
-  for (int i = threadIdx.x; i < d; i += THREADS) q_s[i] = to_f32(q[at + i]);
+  for (int i = threadIdx.x; i < d; i += SIMT_THREADS) q_s[i] = to_f32(q[at + i]);
   __syncthreads();
   const int pos = positions[t], req = request_of[t], kstart = first_visible_key(pos, window);
   const int blocks_a_page = c.page_size / E4M3_BLOCK;
   float m = -INFINITY, l = 0.f, o[MAX_D / 32];
 #pragma unroll
   for (int i = 0; i < MAX_D / 32; ++i) o[i] = 0.f;
-  for (int key0 = kstart / STEP * STEP + warp * STEP; key0 <= pos; key0 += WARPS * STEP) {
+  for (int key0 = kstart / STEP * STEP + warp * STEP; key0 <= pos; key0 += SIMT_WARPS * STEP) {
     // lane < 16: the first block of the two, else the second
     int64_t block = -1;
     {
@@ -425,13 +527,13 @@ attention_e4m3_simt_kernel(const T* __restrict__ q, T* __restrict__ out, const C
   for (int i = 0; i < MAX_D / 32; ++i)
     if (lane + 32 * i < d) rec[warp][2 + lane + 32 * i] = o[i];
   __syncthreads();
-  for (int f = threadIdx.x; f < d; f += THREADS) {
+  for (int f = threadIdx.x; f < d; f += SIMT_THREADS) {
     float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, rec[w][0]);
+    for (int w = 0; w < SIMT_WARPS; ++w) top = fmaxf(top, rec[w][0]);
     const float safe = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < SIMT_WARPS; ++w) {
       const float weight = exp2f(rec[w][0] - safe);
       sum += rec[w][1] * weight;
       v += rec[w][2 + f] * weight;
@@ -440,9 +542,23 @@ attention_e4m3_simt_kernel(const T* __restrict__ q, T* __restrict__ out, const C
   }
 }
 
+// How a launch cuts its work: warps a CTA, and segments of the keys (CTAs a cluster).
+struct Cut { int warps, segments; bool ordered; };
+// All items at once where the warps allow it (RESIDENT an SM): few items get four warps each and their keys cut into segments, as long as
+// every warp still has two tiles; many get two or one. us, 64 tokens at 600 to 3,500 keys (512 items): one warp 1W, two 2W, four 4W; eight
+// at 16,384 (64 items) with 2, 4 and 8 segments 80, 51 and 57; one at 2,048 (8 items) with 4, 8 and 16 7.3, 6.0 and 7.3.
+Cut cut_of(int64_t items, int max_kv_len) {
+  const int slots = 148 * RESIDENT, tiles = (max_kv_len + TILE - 1) / TILE;
+  int segments = 1;
+  while (segments < MAX_SEGMENTS && items * MAX_WARPS * segments * 2 <= slots && tiles >= segments * 2 * MAX_WARPS) segments *= 2;
+  int warps = MAX_WARPS;
+  while (segments == 1 && warps > 1 && items * warps > slots) warps /= 2;
+  return {warps, segments, items * warps * segments > slots};
+}
+
 // Whether clusters of `size` CTAs can run at all; asked once per device, kernel and size.
 template <typename Kernel>
-bool cluster_runs(Kernel kernel, int size) {
+bool cluster_runs(Kernel kernel, int threads, int size) {
   static std::unordered_map<uint64_t, bool> known;
   static std::mutex mutex;
   std::lock_guard<std::mutex> lock(mutex);
@@ -454,7 +570,7 @@ bool cluster_runs(Kernel kernel, int size) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)size);
-  config.blockDim = dim3(THREADS);
+  config.blockDim = dim3((unsigned)threads);
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
   attribute[0].val.clusterDim.x = (unsigned)size;
@@ -470,17 +586,33 @@ bool cluster_runs(Kernel kernel, int size) {
   return clusters > 0;
 }
 
-template <int D>
-cudaError_t launch_e4m3(const bf16* q, bf16* out, const CacheArgs& c, const int* token_list, int count, const int* positions, const int* request_of,
-                        int nq, int nkv, float scale_log2, int window, int segments, unsigned* status, cudaStream_t stream) {
-  auto kernel = attention_e4m3_kernel<D>;
-  while (segments > 1 && !cluster_runs(kernel, segments)) segments /= 2;
-  const int halves = (nq / nkv + HEADS - 1) / HEADS;
-  const dim3 grid((unsigned)((int64_t)count * nkv * halves * segments));
+struct Launch {
+  const bf16* q;
+  bf16* out;
+  CacheArgs c;
+  const int *token_list, *positions, *request_of;
+  int64_t items;
+  int nq, nkv, window, segments, ordered;
+  float scale_log2;
+  unsigned* status;
+  cudaStream_t stream;
+};
+
+template <int D, int WARPS>
+cudaError_t launch_e4m3(const Launch& a) {
+  auto kernel = attention_e4m3_kernel<D, WARPS>;
+  int segments = a.segments;
+  while (segments > 1 && !cluster_runs(kernel, WARPS * 32, segments)) segments /= 2;
+  const dim3 grid((unsigned)(a.items * segments));
   if (segments == 1)
-    return vosti_launch(kernel, grid, dim3(THREADS), 0, stream, q, out, c, token_list, positions, request_of, nq, nkv, scale_log2, window, 1, status);
-  return vosti_launch_clusters(kernel, grid, dim3(THREADS), (unsigned)segments, 0, stream, q, out, c, token_list, positions, request_of, nq, nkv,
-                               scale_log2, window, segments, status);
+    return vosti_launch(kernel, grid, dim3(WARPS * 32), 0, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,
+                        a.window, 1, a.ordered, a.status);
+  return vosti_launch_clusters(kernel, grid, dim3(WARPS * 32), (unsigned)segments, 0, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of,
+                               a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.status);
+}
+template <int D>
+cudaError_t launch_e4m3_as(const Launch& a, int warps) {
+  return warps == 4 ? launch_e4m3<D, 4>(a) : warps == 2 ? launch_e4m3<D, 2>(a) : launch_e4m3<D, 1>(a);
 }
 
 int check_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, const int* block_table, int max_pages, int page_size,
@@ -496,15 +628,6 @@ int check_cache(const void* k, const void* v, const void* k_scale, const void* v
 
 }  // namespace
 
-// How many segments the visible keys of a token are cut into: `count` tokens, the longest of them with max_kv_len keys.
-VOSTI_API int vosti_attention_e4m3_segments(int count, int nq, int nkv, int max_kv_len) {
-  const int64_t items = (int64_t)count * nkv * ((nq / nkv + HEADS - 1) / HEADS);
-  const int tiles = (max_kv_len + TILE - 1) / TILE;
-  int segments = 1;
-  while (segments < MAX_SEGMENTS && items * segments * 2 <= 296 && tiles >= segments * 2 * WARPS) segments *= 2;
-  return segments;
-}
-
 // q, out: bfloat16 [tokens, nq * d]; the cache as in e4m3.cuh. `token_list` (or null: 0 .. count - 1) names the tokens; d is 64 or 128.
 VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, void* out,
                                    const int* token_list, int count, const int* positions, const int* request_of, const int* block_table,
@@ -516,11 +639,11 @@ VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, 
   VOSTI_REQUIRE(count >= 0 && (int64_t)count * nq * MAX_SEGMENTS <= 0x7fffffff, "attention_e4m3: bad token count %d", count);
   if (count == 0) return VOSTI_OK;
   const CacheArgs c = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, max_pages, page_size, num_pages};
-  const int segments = vosti_attention_e4m3_segments(count, nq, nkv, max_kv_len);
-  const cudaError_t e = d == 64 ? launch_e4m3<64>((const bf16*)q, (bf16*)out, c, token_list, count, positions, request_of, nq, nkv, scale * LOG2E, window,
-                                                  segments, status, stream)
-                                : launch_e4m3<128>((const bf16*)q, (bf16*)out, c, token_list, count, positions, request_of, nq, nkv, scale * LOG2E,
-                                                   window, segments, status, stream);
+  const int64_t items = (int64_t)count * nkv * ((nq / nkv + HEADS - 1) / HEADS);
+  const Cut cut = cut_of(items, max_kv_len);
+  const Launch launch = {(const bf16*)q, (bf16*)out, c, token_list, positions, request_of, items, nq, nkv, window, cut.segments,
+                         cut.ordered && count > 1 && count <= MAX_ORDERED ? count : 0, scale * LOG2E, status, stream};
+  const cudaError_t e = d == 64 ? launch_e4m3_as<64>(launch, cut.warps) : launch_e4m3_as<128>(launch, cut.warps);
   if (e != cudaSuccess) {
     vosti_set_error("attention_e4m3: %s", cudaGetErrorString(e));
     return (int)e;
@@ -539,9 +662,9 @@ VOSTI_API int vosti_attention_e4m3_simt(const void* q, const void* k, const void
   if (tokens == 0) return VOSTI_OK;
   const CacheArgs c = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, max_pages, page_size, num_pages};
   const dim3 grid(tokens, nq);
-  const cudaError_t e = is_f32 ? vosti_launch(attention_e4m3_simt_kernel<float>, grid, dim3(THREADS), 0, stream, (const float*)q, (float*)out, c, positions,
+  const cudaError_t e = is_f32 ? vosti_launch(attention_e4m3_simt_kernel<float>, grid, dim3(SIMT_THREADS), 0, stream, (const float*)q, (float*)out, c, positions,
                                               request_of, nq, nkv, d, scale * LOG2E, window, status)
-                               : vosti_launch(attention_e4m3_simt_kernel<bf16>, grid, dim3(THREADS), 0, stream, (const bf16*)q, (bf16*)out, c, positions,
+                               : vosti_launch(attention_e4m3_simt_kernel<bf16>, grid, dim3(SIMT_THREADS), 0, stream, (const bf16*)q, (bf16*)out, c, positions,
                                               request_of, nq, nkv, d, scale * LOG2E, window, status);
   if (e != cudaSuccess) {
     vosti_set_error("attention_e4m3: %s", cudaGetErrorString(e));
