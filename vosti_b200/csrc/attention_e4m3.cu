@@ -24,7 +24,10 @@ struct CacheArgs {
 // ---------------------------------------------------------------------------------------------- tensor cores
 // One CTA for (token, kv head, up to 8 of its query heads, segment of the visible keys); the segments of a token and kv head form a cluster.
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an m16n8k16 instruction are keys and
-// features, all of them needed, and the 8 columns query heads. A warp takes 64 keys at a time, straight from memory into registers, no staging:
+// features, all of them needed, and the 8 columns query heads. A warp takes 64 keys at a time, by bulk copies (a block's keys, or
+// values, are contiguous) into a buffer of its own for each, refilled as soon as it has been read: what is in flight costs no registers, so an
+// SM holds twelve warps instead of eight and ends of CTAs overlap others' middles (us, straight into registers / so, 8 kv heads: 48 tokens at 512
+// keys 18.8 / 12.3, at 2,048 52 / 37, 96 at 600 to 3,500 80 / 65, eight at 16,384 51 / 48).
 //   * the order of the summed index is free as long as both operands share it. A lane's 16 bytes of a key row are features
 //     64 c + 16 j .. + 15 (j = lane % 4): four k-steps of four features. Rows of S^T are chosen so that the weights come out
 //     where the second product wants them: row r of step s is token 4 s + r % 2 (+ 2 for rows 8 to 15) of block r % 8 / 2.
@@ -38,18 +41,13 @@ struct CacheArgs {
 // its largest to 2^14 .. 2^15: exact down to 2^-28 of it.
 // What bounds it is the cache's bytes. (Payloads made bfloat16 by moving their bits, four integer instructions and a multiplication for two, kept
 // the integer pipe busy: 96 us for 64 tokens at 600 to 3,500 keys, 75 for eight at 16,384.)
-constexpr int RESIDENT = 8;                // warps an SM holds of the kernel's registers
-constexpr int MAX_WARPS = 4;
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int RESIDENT = 3;                // CTAs an SM holds of the kernel's registers and buffers
 constexpr int TILE = 64;                   // keys of a warp's step: four blocks
 constexpr int HEADS = 8;                   // query heads of a CTA
 constexpr int MAX_SEGMENTS = 16;
 constexpr int MAX_ORDERED = 256;           // tokens of a launch that starts with the longest
 
-__device__ __forceinline__ uint4 load_line(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -92,14 +90,18 @@ __device__ __forceinline__ void store_at_rank(float* p, uint32_t rank, float v) 
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
-template <int D, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, RESIDENT / WARPS)
+template <int D>
+__global__ void __launch_bounds__(THREADS, RESIDENT)
 attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const CacheArgs c, const int* __restrict__ token_list,
                       const int* __restrict__ positions, const int* __restrict__ request_of, int nq, int nkv, float scale_log2, int window,
                       int segments, int ordered, unsigned* status) {
-  constexpr int CHUNKS = D / 64, FT = D / 16, THREADS = WARPS * 32;
+  constexpr int CHUNKS = D / 64, FT = D / 16;
   constexpr int RAISED = 15;
-  __shared__ float part[WARPS][HEADS][D + 4];                  // the warps' products, under the CTA's maximum
+  // a warp's buffers: four blocks of keys, and four of values whose starts lie 32 bytes apart in the banks (lanes read all four at once)
+  constexpr int BLOCK_BYTES = E4M3_BLOCK * D, V_STRIDE = BLOCK_BYTES + 32, WARP_BYTES = 4 * (BLOCK_BYTES + V_STRIDE);
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full[WARPS][2];             // a warp's keys, its values
+  float (*const part)[HEADS][D + 4] = reinterpret_cast<float (*)[HEADS][D + 4]>(ring);      // at the end: the warps' products, under the CTA's maximum
   __shared__ float stats[WARPS][HEADS][3];                     // m, sum, M
   __shared__ float inbox[HEADS * D + MAX_SEGMENTS];            // of each segment, its products of this CTA's share of the row
   __shared__ float inbox_stats[MAX_SEGMENTS][HEADS][3];
@@ -146,10 +148,10 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   const int blocks_a_page = c.page_size / E4M3_BLOCK;
   const int* const table = c.block_table + (int64_t)req * c.max_pages;
 
-  // index of block `lane % 4` of a tile among the cache's blocks of this kv head, 0 where nothing of it is visible
+  // index of block `lane % 4` of a tile among the cache's blocks, -1 where nothing of it is visible
   auto block_of = [&](int tile) {
     const int key0 = tile * TILE + j * E4M3_BLOCK;
-    if (tile >= end || key0 > pos || key0 + E4M3_BLOCK <= kstart) return (int64_t)g * blocks_a_page;
+    if (tile >= end || key0 > pos || key0 + E4M3_BLOCK <= kstart) return (int64_t)-1;
     const int index = key0 / c.page_size;
     int page = index < c.max_pages ? table[index] : -1;
     if (page < 0 || page >= c.num_pages) {
@@ -159,25 +161,47 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
     return ((int64_t)page * nkv + g) * blocks_a_page + (key0 - index * c.page_size) / E4M3_BLOCK;
   };
 
-  uint4 kk[4][2][CHUNKS];                                      // [step][rows 0-7, 8-15][chunk]
+  uint8_t* const keys_s = ring + warp * WARP_BYTES;
+  uint8_t* const values_s = keys_s + 4 * BLOCK_BYTES;
+  const uint32_t bar[2] = {smem_addr(&full[warp][0]), smem_addr(&full[warp][1])};
+  if (lane == 0) {
+    mb_init(bar[0], 1);
+    mb_init(bar[1], 1);
+    mb_fence_init();
+  }
+  __syncwarp();
+  // the visible blocks of a tile (lane j < 4 names block j) into the keys' or the values' buffer
+  auto request = [&](int side, int64_t block) {
+    const unsigned some = __ballot_sync(0xffffffffu, lane < 4 && block >= 0);
+    if (lane == 0) mb_expect_tx(bar[side], (uint32_t)(__popc(some) * BLOCK_BYTES));
+    __syncwarp();
+    if (lane < 4 && block >= 0)
+      bulk_copy_g2s(smem_addr(side == 0 ? keys_s + lane * BLOCK_BYTES : values_s + lane * V_STRIDE), (side == 0 ? c.k : c.v) + block * BLOCK_BYTES,
+                    BLOCK_BYTES, bar[side]);
+  };
   int k_exp = 0, v_exp = 0;                                    // scales of block lane / 8, the block of this lane's scores
-  auto load_keys = [&](int64_t block) {
+  auto load_scales = [&](int64_t block) {
     const int64_t mine = __shfl_sync(0xffffffffu, block, lane >> 3);
-    const uint8_t* const at = c.k + mine * (E4M3_BLOCK * D) + (r8 & 1) * D + 16 * j;
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int ch = 0; ch < CHUNKS; ++ch) kk[s][h][ch] = load_line(at + (4 * s + 2 * h) * D + 64 * ch);
-    k_exp = c.k_scale[mine];
-    v_exp = c.v_scale[mine];
+    k_exp = mine >= 0 ? c.k_scale[mine] : 0;
+    v_exp = mine >= 0 ? c.v_scale[mine] : 0;
+  };
+  // A wait that runs out is reported, and the warp stops; before, it waits once more for what it has in flight (`other`: the other side too).
+  auto arrived = [&](int side, uint32_t parity, bool other, uint32_t other_parity) {
+    const bool ok = mb_wait(bar[side], parity, status);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    (void)mb_wait(bar[side], parity, status);
+    if (other) (void)mb_wait(bar[side ^ 1], other_parity, status);
+    return false;
   };
 
-  int64_t block = begin + warp < end ? block_of(begin + warp) : 0;
+  int64_t next = block_of(begin + warp);
   pdl_wait();
   pdl_launch_dependents();
-  if (begin + warp < end) load_keys(block);
+  if (begin + warp < end) {
+    request(0, next);
+    request(1, next);
+    load_scales(next);
+  }
   uint32_t qb[CHUNKS][4][2];                                   // Q^T: [chunk][k-step][features 4 w, + 2]
   float q_scale[2];                                            // what heads 2 j and 2 j + 1 were divided by, times scale_log2
   {
@@ -218,34 +242,35 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
 #pragma unroll
   for (int i = 0; i < FT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  for (int tile = begin + warp; tile < end; tile += WARPS) {
-    // this tile's values, and where the next one lies
-    uint4 vv[FT][2];                                           // [16 features][rows 0-7, 8-15]
-    const uint8_t* const v_at = c.v + block * (E4M3_BLOCK * D) + r8 * E4M3_BLOCK;
-#pragma unroll
-    for (int i = 0; i < FT; ++i) {
-      vv[i][0] = load_line(v_at + i * 16 * E4M3_BLOCK);
-      vv[i][1] = load_line(v_at + i * 16 * E4M3_BLOCK + 8 * E4M3_BLOCK);
-    }
-    const int64_t next = block_of(tile + WARPS);
+  uint32_t parity = 0;
+  for (int tile = begin + warp; tile < end; tile += WARPS, parity ^= 1) {
+    next = block_of(tile + WARPS);
+    if (!arrived(0, parity, true, parity)) break;
 
     // ---- S^T = K Q^T
     float s[4][4];
     const float k_times = e4m3_scale(k_exp);
-    float v_log = v_exp == E4M3_NAN_SCALE ? __uint_as_float(0x7fffffffu) : (float)(v_exp - 127);
+    const float v_log = v_exp == E4M3_NAN_SCALE ? __uint_as_float(0x7fffffffu) : (float)(v_exp - 127);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       s[st][0] = s[st][1] = s[st][2] = s[st][3] = 0.f;
 #pragma unroll
-      for (int ch = 0; ch < CHUNKS; ++ch)
+      for (int ch = 0; ch < CHUNKS; ++ch) {
+        const uint8_t* const at = keys_s + (lane >> 3) * BLOCK_BYTES + (4 * st + (r8 & 1)) * D + 64 * ch + 16 * j;
+        const uint4 rows[2] = {*reinterpret_cast<const uint4*>(at), *reinterpret_cast<const uint4*>(at + 2 * D)};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t lo = word_of(kk[st][0][ch], w), hi = word_of(kk[st][1][ch], w);
+          const uint32_t lo = word_of(rows[0], w), hi = word_of(rows[1], w);
           const uint32_t a[4] = {lower_f16(lo), lower_f16(hi), upper_f16(lo), upper_f16(hi)};
           mma_f16(s[st], a, qb[ch][w][0], qb[ch][w][1]);
         }
+      }
     }
-    if (tile + WARPS < end) load_keys(next);
+    __syncwarp();                                              // every lane has read the keys
+    if (tile + WARPS < end) {
+      request(0, next);
+      load_scales(next);
+    }
 
     // ---- online softmax of the lane's two heads over the warp's 64 keys
     const int key_lane = tile * TILE + (lane >> 3) * E4M3_BLOCK + (r8 & 1);        // + 4 st (+ 2)
@@ -263,7 +288,6 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
         }
         top[e & 1] = fmaxf(top[e & 1], s[st][e]);
       }
-    if (edge && top[0] == -INFINITY && top[1] == -INFINITY) v_log = 0.f;        // (nothing of this lane's block is visible, whatever it holds)
     float alpha[2];
     uint32_t p[4][2];                                          // P^T: [step][tokens 4 s, + 2]
     {
@@ -310,36 +334,40 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
     }
 
     // ---- O^T += V^T P^T
+    // (bytes of tokens that are not visible become zeros: whatever they hold must not meet a weight of zero)
+    const int key0 = tile * TILE + j * E4M3_BLOCK;
+    uint32_t seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
     if (edge) {
-      // bytes of tokens that are not visible become zeros: whatever they hold must not meet a weight of zero
-      const int key0 = tile * TILE + j * E4M3_BLOCK;
-      uint32_t keep[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        keep[w] = 0;
+        seen[w] = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-          if (key0 + 4 * w + b >= kstart && key0 + 4 * w + b <= pos) keep[w] |= 0xffu << (8 * b);
+          if (key0 + 4 * w + b >= kstart && key0 + 4 * w + b <= pos) seen[w] |= 0xffu << (8 * b);
       }
-#pragma unroll
-      for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          vv[i][h].x &= keep[0];
-          vv[i][h].y &= keep[1];
-          vv[i][h].z &= keep[2];
-          vv[i][h].w &= keep[3];
-        }
     }
+    if (!arrived(1, parity, tile + WARPS < end, parity ^ 1)) break;
+    auto product = [&](bool masked) {
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
+      for (int i = 0; i < FT; ++i) {
+        const uint8_t* const at = values_s + j * V_STRIDE + (16 * i + r8) * E4M3_BLOCK;
+        const uint4 rows[2] = {*reinterpret_cast<const uint4*>(at), *reinterpret_cast<const uint4*>(at + 8 * E4M3_BLOCK)};
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const uint32_t lo = word_of(vv[i][0], st), hi = word_of(vv[i][1], st);
-        const uint32_t a[4] = {lower_f16(lo), lower_f16(hi), upper_f16(lo), upper_f16(hi)};
-        mma_f16(o[i], a, p[st][0], p[st][1]);
+        for (int st = 0; st < 4; ++st) {
+          uint32_t lo = word_of(rows[0], st), hi = word_of(rows[1], st);
+          if (masked) {
+            lo &= seen[st];
+            hi &= seen[st];
+          }
+          const uint32_t a[4] = {lower_f16(lo), lower_f16(hi), upper_f16(lo), upper_f16(hi)};
+          mma_f16(o[i], a, p[st][0], p[st][1]);
+        }
       }
-    block = next;
+    };
+    if (edge) product(true);
+    else product(false);
+    __syncwarp();                                              // every lane has read the values
+    if (tile + WARPS < end) request(1, next);
   }
 
   // ---- the warps' sums into one, in warp order
@@ -542,23 +570,20 @@ attention_e4m3_simt_kernel(const T* __restrict__ q, T* __restrict__ out, const C
   }
 }
 
-// How a launch cuts its work: warps a CTA, and segments of the keys (CTAs a cluster).
-struct Cut { int warps, segments; bool ordered; };
-// All items at once where the warps allow it (RESIDENT an SM): few items get four warps each and their keys cut into segments, as long as
-// every warp still has two tiles; many get two or one. us, 64 tokens at 600 to 3,500 keys (512 items): one warp 1W, two 2W, four 4W; eight
-// at 16,384 (64 items) with 2, 4 and 8 segments 80, 51 and 57; one at 2,048 (8 items) with 4, 8 and 16 7.3, 6.0 and 7.3.
-Cut cut_of(int64_t items, int max_kv_len) {
-  const int slots = 148 * RESIDENT, tiles = (max_kv_len + TILE - 1) / TILE;
-  int segments = 1;
-  while (segments < MAX_SEGMENTS && items * MAX_WARPS * segments * 2 <= slots && tiles >= segments * 2 * MAX_WARPS) segments *= 2;
-  int warps = MAX_WARPS;
-  while (segments == 1 && warps > 1 && items * warps > slots) warps /= 2;
-  return {warps, segments, items * warps * segments > slots};
+// Segments of a token's keys: as many as find an SM at once, each of a tile a warp at least, eight at most (what a cluster always may have); sixteen
+// where they are few and long. us at 1, 4, 8 and 16 segments: 8 kv heads, one token at 2,048 keys 18.7, 7.8, 6.1 and 7.2, at 8,192 67, 20, 12.3 and
+// 10.5; four at 8,192 72, 24, 18.8 and 25; eight at 8,192 with 4, 6 and 8 31, 28 and 37; sixteen at 2,048 with 1, 3 and 4 21.7, 17.6 and 23.8.
+int segments_of(int64_t items, int max_kv_len) {
+  const int64_t room = 148 * RESIDENT / items, work = (max_kv_len + TILE - 1) / TILE / WARPS;
+  if (items * MAX_SEGMENTS <= 2 * 148 && work >= 2 * MAX_SEGMENTS) return MAX_SEGMENTS;
+  int64_t most = room < work ? room : work;
+  most = most < 8 ? most : 8;
+  return most < 1 ? 1 : (int)most;
 }
 
 // Whether clusters of `size` CTAs can run at all; asked once per device, kernel and size.
 template <typename Kernel>
-bool cluster_runs(Kernel kernel, int threads, int size) {
+bool cluster_runs(Kernel kernel, int threads, int smem, int size) {
   static std::unordered_map<uint64_t, bool> known;
   static std::mutex mutex;
   std::lock_guard<std::mutex> lock(mutex);
@@ -571,6 +596,7 @@ bool cluster_runs(Kernel kernel, int threads, int size) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)size);
   config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = (size_t)smem;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
   attribute[0].val.clusterDim.x = (unsigned)size;
@@ -598,23 +624,21 @@ struct Launch {
   cudaStream_t stream;
 };
 
-template <int D, int WARPS>
+template <int D>
 cudaError_t launch_e4m3(const Launch& a) {
-  auto kernel = attention_e4m3_kernel<D, WARPS>;
+  auto kernel = attention_e4m3_kernel<D>;
+  constexpr int SMEM = WARPS * 4 * (2 * E4M3_BLOCK * D + 32);
+  const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (raised != cudaSuccess) return raised;
   int segments = a.segments;
-  while (segments > 1 && !cluster_runs(kernel, WARPS * 32, segments)) segments /= 2;
+  while (segments > 1 && !cluster_runs(kernel, THREADS, SMEM, segments)) --segments;
   const dim3 grid((unsigned)(a.items * segments));
   if (segments == 1)
-    return vosti_launch(kernel, grid, dim3(WARPS * 32), 0, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,
+    return vosti_launch(kernel, grid, dim3(THREADS), SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,
                         a.window, 1, a.ordered, a.status);
-  return vosti_launch_clusters(kernel, grid, dim3(WARPS * 32), (unsigned)segments, 0, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of,
+  return vosti_launch_clusters(kernel, grid, dim3(THREADS), (unsigned)segments, SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of,
                                a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.status);
 }
-template <int D>
-cudaError_t launch_e4m3_as(const Launch& a, int warps) {
-  return warps == 4 ? launch_e4m3<D, 4>(a) : warps == 2 ? launch_e4m3<D, 2>(a) : launch_e4m3<D, 1>(a);
-}
-
 int check_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, const int* block_table, int max_pages, int page_size,
                 int num_pages, int nq, int nkv, float scale, int window) {
   VOSTI_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_e4m3: bad head counts nq=%d nkv=%d", nq, nkv);
@@ -640,10 +664,11 @@ VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, 
   if (count == 0) return VOSTI_OK;
   const CacheArgs c = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, max_pages, page_size, num_pages};
   const int64_t items = (int64_t)count * nkv * ((nq / nkv + HEADS - 1) / HEADS);
-  const Cut cut = cut_of(items, max_kv_len);
-  const Launch launch = {(const bf16*)q, (bf16*)out, c, token_list, positions, request_of, items, nq, nkv, window, cut.segments,
-                         cut.ordered && count > 1 && count <= MAX_ORDERED ? count : 0, scale * LOG2E, status, stream};
-  const cudaError_t e = d == 64 ? launch_e4m3_as<64>(launch, cut.warps) : launch_e4m3_as<128>(launch, cut.warps);
+  // more CTAs than run at once: those of the tokens with most keys first
+  const bool ordered = items > 148 * RESIDENT && count > 1 && count <= MAX_ORDERED;
+  const Launch launch = {(const bf16*)q, (bf16*)out, c, token_list, positions, request_of, items, nq, nkv, window, segments_of(items, max_kv_len),
+                         ordered ? count : 0, scale * LOG2E, status, stream};
+  const cudaError_t e = d == 64 ? launch_e4m3<64>(launch) : launch_e4m3<128>(launch);
   if (e != cudaSuccess) {
     vosti_set_error("attention_e4m3: %s", cudaGetErrorString(e));
     return (int)e;

@@ -18,6 +18,8 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int PER_WARP = E4M3_BLOCK / WARPS;   // tokens of a run, or q heads, that a warp holds
 constexpr int V_PITCH = 20;                    // bytes between a feature's rows of values in shared memory (banks apart)
+constexpr int FEW = 64;                        // up to so many tokens: one a CTA
+constexpr int Q_TOKENS = 2;                    // of a CTA of query heads, with more
 
 struct PostArgs {
   const void* qkv;               // [tokens, (nq + 2 nkv) d], or null with
@@ -168,6 +170,34 @@ __device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, fl
   }
 }
 
+template <typename T, int PAIRS, bool FAST>
+__device__ __forceinline__ void store_head(const PostArgs& a, T* dst, int lane, const float (&x)[PAIRS], const float (&y)[PAIRS]) {
+  const int half = a.d >> 1;
+  if constexpr (FAST && PAIRS > 1) {
+#pragma unroll
+    for (int j = 0; j < PAIRS; j += 2) {
+      const int p = pair_index<PAIRS, FAST>(lane, j);
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(dst + p) = make_float2(x[j], x[j + 1]);
+        *reinterpret_cast<float2*>(dst + p + half) = make_float2(y[j], y[j + 1]);
+      } else {
+        *reinterpret_cast<__nv_bfloat162*>(dst + p) = __floats2bfloat162_rn(x[j], x[j + 1]);
+        *reinterpret_cast<__nv_bfloat162*>(dst + p + half) = __floats2bfloat162_rn(y[j], y[j + 1]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      const int p = pair_index<PAIRS, FAST>(lane, j);
+      if (p >= half) continue;
+      int ia, ib;
+      pair_elements<FAST>(p, a, ia, ib);
+      dst[ia] = from_f32<T>(x[j]);
+      dst[ib] = from_f32<T>(y[j]);
+    }
+  }
+}
+
 __device__ __forceinline__ int position_of(const PostArgs& a, int t) {
   if (a.cos_table == nullptr) return 0;
   const int pos = a.positions[t];
@@ -176,64 +206,51 @@ __device__ __forceinline__ int position_of(const PostArgs& a, int t) {
   return 0;
 }
 
-// grid: x: `tile` neighbouring tokens, y: kv heads, then groups of 16 q heads.
+// Blocks: `tile` neighbouring tokens' keys and values of a kv head, then 16 query heads of one or two tokens (what is in flight is what
+// counts for a prompt: a warp has four heads of two tokens, or keys and values of four, on their way, 32 warps an SM).
 template <typename T, int PAIRS, bool FAST>
-__global__ void __launch_bounds__(THREADS) qkv_post_e4m3_kernel(const PostArgs a) {
+__global__ void __launch_bounds__(THREADS, PAIRS >= 4 ? 4 : 8) qkv_post_e4m3_kernel(const PostArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = a.nq + 2 * a.nkv, half = a.d >> 1;
-  const int t_begin = blockIdx.x * a.tile, t_end = min(a.tokens, t_begin + a.tile);
+  const int kv_blocks = (a.tokens + a.tile - 1) / a.tile * a.nkv;
 
-  if ((int)blockIdx.y >= a.nkv) {
-    // ------------------------------------------------------------ queries: a warp takes four heads of a token at a time
-    const int h0 = ((int)blockIdx.y - a.nkv) * E4M3_BLOCK + warp * PER_WARP;
+  if ((int)blockIdx.x >= kv_blocks) {
+    // ------------------------------------------------------------ queries: a warp takes four heads
+    const int groups = (a.nq + E4M3_BLOCK - 1) / E4M3_BLOCK, block = (int)blockIdx.x - kv_blocks;
+    const int h0 = block % groups * E4M3_BLOCK + warp * PER_WARP;
+    const int step = a.tokens <= FEW ? 1 : Q_TOKENS, t0 = block / groups * step, count = min(step, a.tokens - t0);
     float wx[PAIRS], wy[PAIRS];
     load_norm<PAIRS, FAST>(a, a.q_norm_w, lane, wx, wy);
     pdl_wait();
     pdl_launch_dependents();
     if (h0 >= a.nq) return;
-    for (int t = t_begin; t < t_end; ++t) {
-      float x[PER_WARP][PAIRS], y[PER_WARP][PAIRS], c[PAIRS], s[PAIRS];
-      const int64_t at = ((int64_t)t * heads + h0) * a.d;
+    float x[Q_TOKENS][PER_WARP][PAIRS], y[Q_TOKENS][PER_WARP][PAIRS];
+#pragma unroll
+    for (int n = 0; n < Q_TOKENS; ++n)
 #pragma unroll
       for (int i = 0; i < PER_WARP; ++i)
-        if (h0 + i < a.nq) load_head<T, PAIRS, FAST>(a, at + (int64_t)i * a.d, lane, x[i], y[i]);
-      load_turn<PAIRS, FAST>(a, position_of(a, t), lane, c, s);
-      T* out = reinterpret_cast<T*>(a.q_out) + ((int64_t)t * a.nq + h0) * a.d;
+        if (n < count && h0 + i < a.nq) load_head<T, PAIRS, FAST>(a, ((int64_t)(t0 + n) * heads + h0 + i) * a.d, lane, x[n][i], y[n][i]);
+#pragma unroll
+    for (int n = 0; n < Q_TOKENS; ++n) {
+      if (n >= count) break;
+      float c[PAIRS], s[PAIRS];
+      load_turn<PAIRS, FAST>(a, position_of(a, t0 + n), lane, c, s);
+      T* out = reinterpret_cast<T*>(a.q_out) + ((int64_t)(t0 + n) * a.nq + h0) * a.d;
 #pragma unroll
       for (int i = 0; i < PER_WARP; ++i) {
         if (h0 + i >= a.nq) break;
-        norm_and_turn<PAIRS>(a, a.q_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
-        T* dst = out + (int64_t)i * a.d;
-#pragma unroll
-        for (int j = 0; j < PAIRS; ++j) {
-          const int p = pair_index<PAIRS, FAST>(lane, j);
-          if (FAST && PAIRS > 1) {
-            if (j & 1) continue;
-            if (sizeof(T) == 4) {
-              *reinterpret_cast<float2*>(reinterpret_cast<float*>(dst) + p) = make_float2(x[i][j], x[i][(j + 1) % PAIRS]);
-              *reinterpret_cast<float2*>(reinterpret_cast<float*>(dst) + p + half) = make_float2(y[i][j], y[i][(j + 1) % PAIRS]);
-            } else {
-              *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(dst) + p) = __floats2bfloat162_rn(x[i][j], x[i][(j + 1) % PAIRS]);
-              *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(dst) + p + half) = __floats2bfloat162_rn(y[i][j], y[i][(j + 1) % PAIRS]);
-            }
-            continue;
-          }
-          if (p >= half) continue;
-          int ia, ib;
-          pair_elements<FAST>(p, a, ia, ib);
-          dst[ia] = from_f32<T>(x[i][j]);
-          dst[ib] = from_f32<T>(y[i][j]);
-        }
+        norm_and_turn<PAIRS>(a, a.q_norm_w != nullptr, x[n][i], y[n][i], wx, wy, c, s);
+        store_head<T, PAIRS, FAST>(a, out + (int64_t)i * a.d, lane, x[n][i], y[n][i]);
       }
     }
     return;
   }
 
   // -------------------------------------------------------------- keys and values of one kv head, run by run
-  extern __shared__ __align__(16) uint8_t v_rows[];             // [d][V_PITCH]: the run's values, feature-major
+  extern __shared__ __align__(16) uint8_t v_rows[];             // [d][V_PITCH]: the run's values, feature-major, at their places in the block
   __shared__ float most[2][WARPS];
   __shared__ int broken[2][WARPS];
-  const int g = blockIdx.y;
+  const int g = (int)blockIdx.x % a.nkv, t_begin = (int)blockIdx.x / a.nkv * a.tile, t_end = min(a.tokens, t_begin + a.tile);
   float wx[PAIRS], wy[PAIRS];
   load_norm<PAIRS, FAST>(a, a.k_norm_w, lane, wx, wy);
   // slots were written before the step began
@@ -349,8 +366,8 @@ __global__ void __launch_bounds__(THREADS) qkv_post_e4m3_kernel(const PostArgs a
         int ia, ib;
         pair_elements<FAST>(p, a, ia, ib);
         const uint16_t vv = e4m3_pack(vx[i][j] * v_times, vy[i][j] * v_times);
-        v_rows[ia * V_PITCH + r] = (uint8_t)vv;
-        v_rows[ib * V_PITCH + r] = (uint8_t)(vv >> 8);
+        v_rows[ia * V_PITCH + offset + r] = (uint8_t)vv;
+        v_rows[ib * V_PITCH + offset + r] = (uint8_t)(vv >> 8);
         if (FAST && PAIRS > 1) {
           if (j & 1) continue;
           *reinterpret_cast<uint16_t*>(key + p) = e4m3_pack(kx[i][j] * k_times, kx[i][(j + 1) % PAIRS] * k_times);
@@ -370,18 +387,16 @@ __global__ void __launch_bounds__(THREADS) qkv_post_e4m3_kernel(const PostArgs a
       const int feature = i >> 2, w0 = (i & 3) * 4;              // tokens w0 .. w0 + 3 of the block
       if (w0 >= offset + n || (w0 + 4 <= offset && !regrow)) continue;
       uint32_t* const word = reinterpret_cast<uint32_t*>(v_block + feature * E4M3_BLOCK) + (i & 3);
-      const bool whole = w0 >= offset && w0 + 4 <= offset + n;
-      uint32_t w = whole ? 0u : *word;
-      if (regrow && w0 < offset) {
-        const float2 lo = e4m3_unpack((uint16_t)w), hi = e4m3_unpack((uint16_t)(w >> 16));
-        const uint32_t again = (uint32_t)e4m3_pack(lo.x * f, lo.y * f) | (uint32_t)e4m3_pack(hi.x * f, hi.y * f) << 16;
-        const uint32_t mine = w0 + 4 <= offset ? 0xffffffffu : (1u << (8 * (offset - w0))) - 1u;     // earlier tokens' bytes
-        w = (w & ~mine) | (again & mine);
-      }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int r = w0 + b - offset;
-        if (r >= 0 && r < n) w = (w & ~(0xffu << (8 * b))) | (uint32_t)v_rows[feature * V_PITCH + r] << (8 * b);
+      const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
+      uint32_t w = *reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH + w0) & new_bytes;
+      if (new_bytes != 0xffffffffu) {
+        uint32_t there = *word;
+        if (regrow) {
+          const float2 lo = e4m3_unpack((uint16_t)there), hi = e4m3_unpack((uint16_t)(there >> 16));
+          const uint32_t again = (uint32_t)e4m3_pack(lo.x * f, lo.y * f) | (uint32_t)e4m3_pack(hi.x * f, hi.y * f) << 16;
+          there = (there & ~old_bytes) | (again & old_bytes);
+        }
+        w |= there & ~new_bytes;
       }
       *word = w;
     }
@@ -395,7 +410,8 @@ __global__ void __launch_bounds__(THREADS) qkv_post_e4m3_kernel(const PostArgs a
 
 template <typename T, int PAIRS, bool FAST>
 cudaError_t launch_post(const PostArgs& a, cudaStream_t stream) {
-  const dim3 grid((a.tokens + a.tile - 1) / a.tile, a.nkv + (a.nq + E4M3_BLOCK - 1) / E4M3_BLOCK);
+  const int64_t q_steps = a.tokens <= FEW ? a.tokens : (a.tokens + Q_TOKENS - 1) / Q_TOKENS;
+  const dim3 grid((unsigned)((int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv + q_steps * ((a.nq + E4M3_BLOCK - 1) / E4M3_BLOCK)));
   return vosti_launch(qkv_post_e4m3_kernel<T, PAIRS, FAST>, grid, dim3(THREADS), (size_t)a.d * V_PITCH, stream, a);
 }
 template <typename T>
@@ -433,9 +449,9 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
   VOSTI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qkv_post_e4m3: the cache must start on 16 bytes");
   VOSTI_REQUIRE(slot_mapping != nullptr && k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr, "qkv_post_e4m3: the cache is missing");
   if (tokens == 0) return VOSTI_OK;
-  VOSTI_REQUIRE(nkv + (nq + E4M3_BLOCK - 1) / E4M3_BLOCK <= 65535, "qkv_post_e4m3: too many heads for one launch");
+  VOSTI_REQUIRE((int64_t)tokens * (nkv + (nq + E4M3_BLOCK - 1) / E4M3_BLOCK) <= 0x7fffffff, "qkv_post_e4m3: too many tokens and heads for one launch");
   // few tokens: a CTA for each, so that none waits for another's run; many (prompts): a CTA for 16, one or two runs
-  const int tile = tokens <= 64 ? 1 : E4M3_BLOCK;
+  const int tile = tokens <= FEW ? 1 : E4M3_BLOCK;
   const PostArgs a = {qkv, partial, splits, (int64_t)tokens * (nq + 2 * nkv) * d, q_out, (uint8_t*)k, (uint8_t*)v, (uint8_t*)k_scale,
                       (uint8_t*)v_scale, q_norm_w, k_norm_w, norm_w_is_f32, eps, cos_table, sin_table, max_positions, positions, slot_mapping,
                       num_slots, page_size, tokens, nq, nkv, d, cos_table != nullptr ? rotary_dim : d, interleaved, tile, status};
