@@ -6,20 +6,26 @@
 // the one rounding at the store.
 //
 // A scale belongs to a block, so the unit of work for keys and values is a run: the step's tokens of one block and kv head, which stand
-// next to one another in the batch and in the block. One CTA takes a run: it holds the run's keys and values in
-// registers, finds their largest size, takes the larger of what they need and (a block that holds earlier tokens) the
-// scale that is there, rounds the earlier tokens again where the scale grew, and stores. Nothing of another CTA's is read.
+// next to one another in the batch and in the block. A CTA (runs of more than four tokens) or a warp (shorter ones) takes a run: it holds
+// the run's keys and values in registers, finds their largest size, takes the larger of what they need and (a block that holds earlier
+// tokens) the scale that is there, rounds the earlier tokens again where the scale grew, and stores. Nothing of another run's is read.
 // A value that is not finite, or not below 2^96, makes its block's scale 255: the block is no number from then on.
+//
+// A head of 64, 128 or 256 that turns as a whole in pairs (i, i + d/2), or not at all, is d / 8 lanes with four neighbouring elements of each half;
+// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 21.6 us, a third of what its bytes need: blocks are
+// short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (blocks that walked on over query
+// heads were slower: 22.1 us with six an SM, 27 with three; a head on a whole warp 22.4 with half as many instructions again).
 #include "common.cuh"
 #include "e4m3.cuh"
 
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int PER_WARP = E4M3_BLOCK / WARPS;   // tokens of a run, or q heads, that a warp holds
+constexpr int SHORT = 4;                       // tokens of a run that one warp takes
 constexpr int V_PITCH = 20;                    // bytes between a feature's rows of values in shared memory (banks apart)
 constexpr int FEW = 64;                        // up to so many tokens: one a CTA
-constexpr int Q_TOKENS = 2;                    // of a CTA of query heads, with more
+constexpr int TILE = 8;                        // neighbouring tokens whose runs a CTA takes, with more
+constexpr int Q_ITEMS = 4;                     // query heads that a lane holds at a time
 
 struct PostArgs {
   const void* qkv;               // [tokens, (nq + 2 nkv) d], or null with
@@ -30,7 +36,7 @@ struct PostArgs {
   uint8_t *k, *v, *k_scale, *v_scale;
   const void *q_norm_w, *k_norm_w;
   int norm_w_is_f32;
-  float eps;
+  float eps, inverse_d;
   const float *cos_table, *sin_table;
   int max_positions;
   const int *positions, *slot_mapping;
@@ -39,227 +45,380 @@ struct PostArgs {
   unsigned* status;
 };
 
-// A lane holds PAIRS pairs of a head's elements; those of a rotation turn with one another. FAST (the whole head turns in pairs
-// (i, i + d/2), or nothing turns; d a multiple of 64, of 128 above one pair): neighbouring pairs in neighbouring words.
-template <int PAIRS, bool FAST>
-__device__ __forceinline__ int pair_index(int lane, int j) {
-  return FAST && PAIRS > 1 ? 2 * lane + (j & 1) + 64 * (j >> 1) : lane + 32 * j;
-}
-// Elements of pair p: the first `rotary_dim` turn, the rest pair up with their neighbours.
-template <bool FAST>
-__device__ __forceinline__ void pair_elements(int p, const PostArgs& a, int& ia, int& ib) {
-  if (FAST) {
-    ia = p;
-    ib = p + (a.d >> 1);
-    return;
+// How a head lies on lanes: `LANES` of them with `PAIRS` pairs each; those of a rotation turn with one another.
+template <int LANES_, int PAIRS_, bool FAST_>
+struct Lay {
+  static constexpr int LANES = LANES_, PAIRS = PAIRS_, HEADS = 32 / LANES_;
+  static constexpr bool FAST = FAST_;
+  static __device__ __forceinline__ int pair(int sub, int j) { return FAST ? 4 * sub + j : sub + 32 * j; }
+  // Elements of pair p: the first `rotary_dim` turn, the rest pair up with their neighbours.
+  static __device__ __forceinline__ void elements(int p, const PostArgs& a, int& ia, int& ib) {
+    if (FAST) {
+      ia = p;
+      ib = p + (a.d >> 1);
+      return;
+    }
+    const int turning = a.rotary_dim >> 1;
+    const bool turns = p < turning;
+    ia = turns && !a.interleaved ? p : 2 * p;
+    ib = turns && !a.interleaved ? p + turning : 2 * p + 1;
   }
-  const int turning = a.rotary_dim >> 1;
-  if (p < turning) {
-    ia = a.interleaved ? 2 * p : p;
-    ib = a.interleaved ? 2 * p + 1 : p + turning;
-  } else {
-    ia = 2 * p;
-    ib = 2 * p + 1;
-  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_words(const T* p, float (&x)[4]) {
+  const float4 v = load_four(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
 
-template <typename T, int PAIRS, bool FAST>
-__device__ __forceinline__ void load_head(const PostArgs& a, int64_t at, int lane, float (&x)[PAIRS], float (&y)[PAIRS]) {
+// A head of the projection (or of its partial sums, added in split order) that begins at element `at`.
+template <typename T, typename L>
+__device__ __forceinline__ void load_head(const PostArgs& a, int64_t at, int sub, float (&x)[L::PAIRS], float (&y)[L::PAIRS]) {
   const int half = a.d >> 1;
-  if constexpr (FAST && PAIRS > 1) {
+  if constexpr (L::FAST) {
+    const int64_t i = at + 4 * sub;
+    if (a.partial == nullptr) {
+      load_words(reinterpret_cast<const T*>(a.qkv) + i, x);
+      load_words(reinterpret_cast<const T*>(a.qkv) + i + half, y);
+      return;
+    }
 #pragma unroll
-    for (int j = 0; j < PAIRS; j += 2) {
-      const int64_t i = at + 2 * lane + 32 * j;
-      if (a.partial != nullptr) {
-        float2 u = make_float2(0.f, 0.f), v = u;
+    for (int j = 0; j < 4; ++j) x[j] = y[j] = 0.f;
 #pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) {
-          const float2 p = *reinterpret_cast<const float2*>(a.partial + s * a.plane + i);
-          const float2 r = *reinterpret_cast<const float2*>(a.partial + s * a.plane + i + half);
-          u.x += p.x, u.y += p.y, v.x += r.x, v.y += r.y;
-        }
-        x[j] = u.x, x[j + 1] = u.y, y[j] = v.x, y[j + 1] = v.y;
-      } else if (sizeof(T) == 4) {
-        const float2 u = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.qkv) + i);
-        const float2 v = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.qkv) + i + half);
-        x[j] = u.x, x[j + 1] = u.y, y[j] = v.x, y[j + 1] = v.y;
-      } else {
-        const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(reinterpret_cast<const bf16*>(a.qkv) + i));
-        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(reinterpret_cast<const bf16*>(a.qkv) + i + half));
-        x[j] = u.x, x[j + 1] = u.y, y[j] = v.x, y[j + 1] = v.y;
+    for (int s = 0; s < a.splits; ++s) {
+      float u[4], v[4];
+      load_words(a.partial + s * a.plane + i, u);
+      load_words(a.partial + s * a.plane + i + half, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] += u[j];
+        y[j] += v[j];
       }
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < PAIRS; ++j) {
-      const int p = pair_index<PAIRS, FAST>(lane, j);
+    for (int j = 0; j < L::PAIRS; ++j) {
+      const int p = L::pair(sub, j);
       x[j] = y[j] = 0.f;
       if (p >= half) continue;
       int ia, ib;
-      pair_elements<FAST>(p, a, ia, ib);
-      if (a.partial != nullptr) {
-#pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) {
-          x[j] += a.partial[s * a.plane + at + ia];
-          y[j] += a.partial[s * a.plane + at + ib];
-        }
-      } else {
+      L::elements(p, a, ia, ib);
+      if (a.partial == nullptr) {
         x[j] = to_f32(reinterpret_cast<const T*>(a.qkv)[at + ia]);
         y[j] = to_f32(reinterpret_cast<const T*>(a.qkv)[at + ib]);
+        continue;
+      }
+#pragma unroll 4
+      for (int s = 0; s < a.splits; ++s) {
+        x[j] += a.partial[s * a.plane + at + ia];
+        y[j] += a.partial[s * a.plane + at + ib];
       }
     }
   }
 }
 
 // Norm weights of this lane's elements (ones without a norm).
-template <int PAIRS, bool FAST>
-__device__ __forceinline__ void load_norm(const PostArgs& a, const void* w, int lane, float (&wx)[PAIRS], float (&wy)[PAIRS]) {
+template <typename L>
+__device__ __forceinline__ void load_norm(const PostArgs& a, const void* w, int sub, float (&wx)[L::PAIRS], float (&wy)[L::PAIRS]) {
+  if constexpr (L::FAST) {
+    if (w != nullptr) {
+      if (a.norm_w_is_f32) {
+        load_words(reinterpret_cast<const float*>(w) + 4 * sub, wx);
+        load_words(reinterpret_cast<const float*>(w) + 4 * sub + (a.d >> 1), wy);
+      } else {
+        load_words(reinterpret_cast<const bf16*>(w) + 4 * sub, wx);
+        load_words(reinterpret_cast<const bf16*>(w) + 4 * sub + (a.d >> 1), wy);
+      }
+      return;
+    }
+  }
 #pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-    const int p = pair_index<PAIRS, FAST>(lane, j);
+  for (int j = 0; j < L::PAIRS; ++j) {
+    const int p = L::pair(sub, j);
     wx[j] = wy[j] = 1.f;
     if (w == nullptr || p >= (a.d >> 1)) continue;
     int ia, ib;
-    pair_elements<FAST>(p, a, ia, ib);
+    L::elements(p, a, ia, ib);
     wx[j] = load_flex(w, a.norm_w_is_f32, ia);
     wy[j] = load_flex(w, a.norm_w_is_f32, ib);
   }
 }
 
-// Cosines and sines of this lane's pairs at a position (no turn: 1 and 0).
-template <int PAIRS, bool FAST>
-__device__ __forceinline__ void load_turn(const PostArgs& a, int pos, int lane, float (&c)[PAIRS], float (&s)[PAIRS]) {
-  const int turning = a.cos_table != nullptr ? a.rotary_dim >> 1 : 0;
-  const int64_t at = (int64_t)pos * turning;
-  if (FAST && PAIRS > 1 && turning > 0) {
+// A token's position (0 without a rotation); positions were written before the step began.
+__device__ __forceinline__ int position_of(const PostArgs& a, int t) {
+  if (a.cos_table == nullptr) return 0;
+  const int pos = a.positions[t];
+  if (pos >= 0 && pos < a.max_positions) return pos;
+  raise_fault(a.status, VOSTI_FAULT_POSITION_RANGE);
+  return 0;
+}
+
+// Cosines and sines of this lane's pairs (no turn: 1 and 0).
+template <typename L>
+__device__ __forceinline__ void load_turn(const PostArgs& a, int pos, int sub, float (&c)[L::PAIRS], float (&s)[L::PAIRS]) {
 #pragma unroll
-    for (int j = 0; j < PAIRS; j += 2) {
-      const float2 u = *reinterpret_cast<const float2*>(a.cos_table + at + 2 * lane + 32 * j);
-      const float2 v = *reinterpret_cast<const float2*>(a.sin_table + at + 2 * lane + 32 * j);
-      c[j] = u.x, c[j + 1] = u.y, s[j] = v.x, s[j + 1] = v.y;
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-    const int p = pair_index<PAIRS, FAST>(lane, j);
+  for (int j = 0; j < L::PAIRS; ++j) {
     c[j] = 1.f;
     s[j] = 0.f;
-    if (p < turning) {
+  }
+  if (a.cos_table == nullptr) return;
+  const int turning = a.rotary_dim >> 1;
+  const int64_t at = (int64_t)pos * turning;
+  if constexpr (L::FAST) {
+    load_words(a.cos_table + at + 4 * sub, c);
+    load_words(a.sin_table + at + 4 * sub, s);
+  } else {
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) {
+      const int p = L::pair(sub, j);
+      if (p >= turning) continue;
       c[j] = a.cos_table[at + p];
       s[j] = a.sin_table[at + p];
     }
   }
 }
 
-template <int PAIRS>
-__device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, float (&x)[PAIRS], float (&y)[PAIRS], const float (&wx)[PAIRS],
-                                              const float (&wy)[PAIRS], const float (&c)[PAIRS], const float (&s)[PAIRS]) {
-  float r = 1.f;
+// All lanes of the warp take part: a head's sum of squares runs over its lanes.
+template <typename L>
+__device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, float (&x)[L::PAIRS], float (&y)[L::PAIRS], const float (&wx)[L::PAIRS],
+                                              const float (&wy)[L::PAIRS], const float (&c)[L::PAIRS], const float (&s)[L::PAIRS]) {
   if (normed) {
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < PAIRS; ++j) ss += x[j] * x[j] + y[j] * y[j];
-    r = rsqrtf(warp_sum(ss) / (float)a.d + a.eps);
-  }
+    for (int j = 0; j < L::PAIRS; ++j) ss = fmaf(x[j], x[j], fmaf(y[j], y[j], ss));
 #pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-    const float u = x[j] * r * wx[j], v = y[j] * r * wy[j];
+    for (int o = 1; o < L::LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(fmaf(ss, a.inverse_d, a.eps));
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) {
+      x[j] *= r * wx[j];
+      y[j] *= r * wy[j];
+    }
+  }
+  if (a.cos_table == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < L::PAIRS; ++j) {
+    const float u = x[j], v = y[j];
+    if (!L::FAST && c[j] == 1.f && s[j] == 0.f) continue;        // (not turned: whatever its neighbour is)
     x[j] = u * c[j] - v * s[j];
     y[j] = v * c[j] + u * s[j];
   }
 }
 
-template <typename T, int PAIRS, bool FAST>
-__device__ __forceinline__ void store_head(const PostArgs& a, T* dst, int lane, const float (&x)[PAIRS], const float (&y)[PAIRS]) {
-  const int half = a.d >> 1;
-  if constexpr (FAST && PAIRS > 1) {
-#pragma unroll
-    for (int j = 0; j < PAIRS; j += 2) {
-      const int p = pair_index<PAIRS, FAST>(lane, j);
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float2*>(dst + p) = make_float2(x[j], x[j + 1]);
-        *reinterpret_cast<float2*>(dst + p + half) = make_float2(y[j], y[j + 1]);
-      } else {
-        *reinterpret_cast<__nv_bfloat162*>(dst + p) = __floats2bfloat162_rn(x[j], x[j + 1]);
-        *reinterpret_cast<__nv_bfloat162*>(dst + p + half) = __floats2bfloat162_rn(y[j], y[j + 1]);
-      }
-    }
+template <typename T, typename L>
+__device__ __forceinline__ void store_head(const PostArgs& a, T* dst, int sub, const float (&x)[L::PAIRS], const float (&y)[L::PAIRS]) {
+  if constexpr (L::FAST) {
+    store_four(dst + 4 * sub, make_float4(x[0], x[1], x[2], x[3]));
+    store_four(dst + 4 * sub + (a.d >> 1), make_float4(y[0], y[1], y[2], y[3]));
   } else {
 #pragma unroll
-    for (int j = 0; j < PAIRS; ++j) {
-      const int p = pair_index<PAIRS, FAST>(lane, j);
-      if (p >= half) continue;
+    for (int j = 0; j < L::PAIRS; ++j) {
+      const int p = L::pair(sub, j);
+      if (p >= (a.d >> 1)) continue;
       int ia, ib;
-      pair_elements<FAST>(p, a, ia, ib);
+      L::elements(p, a, ia, ib);
       dst[ia] = from_f32<T>(x[j]);
       dst[ib] = from_f32<T>(y[j]);
     }
   }
 }
 
-__device__ __forceinline__ int position_of(const PostArgs& a, int t) {
-  if (a.cos_table == nullptr) return 0;
-  const int pos = a.positions[t];
-  if (pos >= 0 && pos < a.max_positions) return pos;
-  if ((threadIdx.x & 31) == 0) raise_fault(a.status, VOSTI_FAULT_POSITION_RANGE);
-  return 0;
+__device__ __forceinline__ uint32_t e4m3_pack4(float v0, float v1, float v2, float v3) {
+  return (uint32_t)e4m3_pack(v0, v1) | (uint32_t)e4m3_pack(v2, v3) << 16;
+}
+// A word's four payloads under a scale 2^-(shift) times larger.
+__device__ __forceinline__ uint32_t e4m3_again(uint32_t w, float f) {
+  const float2 lo = e4m3_unpack((uint16_t)w), hi = e4m3_unpack((uint16_t)(w >> 16));
+  return e4m3_pack4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
 }
 
-// Blocks: `tile` neighbouring tokens' keys and values of a kv head, then 16 query heads of one or two tokens (what is in flight is what
-// counts for a prompt: a warp has four heads of two tokens, or keys and values of four, on their way, 32 warps an SM).
-template <typename T, int PAIRS, bool FAST>
-__global__ void __launch_bounds__(THREADS, PAIRS >= 4 ? 4 : 8) qkv_post_e4m3_kernel(const PostArgs a) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ int slot_at(const PostArgs& a, int t) { return t >= 0 && t < a.tokens ? a.slot_mapping[t] : -1; }
+
+// The larger size; no number if either is none.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+struct RunStats {                 // of a CTA's warps: largest sizes of keys and values
+  float most[2][WARPS];
+};
+
+// One run: the tokens from t0 on of kv head g, by the whole CTA or by one warp (`v_rows`: [d][V_PITCH] of its own).
+template <typename T, typename L, bool WHOLE>
+__device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint8_t* v_rows, RunStats* shared, const float (&wx)[L::PAIRS], const float (&wy)[L::PAIRS]) {
+  constexpr int STEP = (WHOLE ? WARPS : 1) * L::HEADS, ROUNDS = ((WHOLE ? E4M3_BLOCK : SHORT) + STEP - 1) / STEP;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L::LANES;
+  const int me = (WHOLE ? warp * L::HEADS : 0) + lane / L::LANES, thread = WHOLE ? threadIdx.x : lane, threads = WHOLE ? THREADS : 32;
   const int heads = a.nq + 2 * a.nkv, half = a.d >> 1;
+  const int slot = slot_at(a, t0), offset = slot % E4M3_BLOCK;
+  // the neighbours that continue the run (lane 16 never does)
+  const unsigned gone = ~__ballot_sync(0xffffffffu, offset + lane < E4M3_BLOCK && slot_at(a, t0 + lane) == slot + lane);
+  const int n = __ffs(gone) - 1;
+  const int64_t page = slot / a.page_size, in_page = slot % a.page_size;
+  const int64_t block = (page * a.nkv + g) * (a.page_size / E4M3_BLOCK) + in_page / E4M3_BLOCK;
+  auto sync = [] {
+    if constexpr (WHOLE) __syncthreads();
+    else __syncwarp();
+  };
+
+  int pos[ROUNDS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) pos[i] = position_of(a, t0 + min(me + i * STEP, n - 1));
+  float kx[ROUNDS][L::PAIRS], ky[ROUNDS][L::PAIRS], vx[ROUNDS][L::PAIRS], vy[ROUNDS][L::PAIRS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int r = me + i * STEP;
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) kx[i][j] = ky[i][j] = vx[i][j] = vy[i][j] = 0.f;
+    if (r >= n) continue;
+    const int64_t at = ((int64_t)(t0 + r) * heads + a.nq + g) * a.d;
+    load_head<T, L>(a, at, sub, kx[i], ky[i]);
+    load_head<T, L>(a, at + (int64_t)a.nkv * a.d, sub, vx[i], vy[i]);
+  }
+  const int k_old = offset > 0 ? a.k_scale[block] : 0, v_old = offset > 0 ? a.v_scale[block] : 0;
+  float most[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    if (i * STEP >= n) break;                                    // (the same in all lanes)
+    float c[L::PAIRS], s[L::PAIRS];
+    load_turn<L>(a, pos[i], sub, c, s);
+    norm_and_turn<L>(a, a.k_norm_w != nullptr, kx[i], ky[i], wx, wy, c, s);      // (zeros beyond the run stay zeros)
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) {
+      most[0] = larger(larger(most[0], kx[i][j]), ky[i][j]);
+      most[1] = larger(larger(most[1], vx[i][j]), vy[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most[i] = larger(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+  if constexpr (WHOLE) {
+    if (lane == 0) {
+      shared->most[0][warp] = most[0];
+      shared->most[1][warp] = most[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) most[i] = larger(most[i], shared->most[i][w]);
+  }
+  const int k_new = !(most[0] < E4M3_LIMIT) ? E4M3_NAN_SCALE : max(e4m3_scale_for(most[0]), k_old);
+  const int v_new = !(most[1] < E4M3_LIMIT) ? E4M3_NAN_SCALE : max(e4m3_scale_for(most[1]), v_old);
+  // 2^-(scale - 127): the bits 254 - scale as an exponent (a scale that is no number: any payload will do)
+  const float k_times = __uint_as_float((uint32_t)max(254 - k_new, 1) << 23), v_times = __uint_as_float((uint32_t)max(254 - v_new, 1) << 23);
+  uint8_t* const k_rows = a.k + block * E4M3_BLOCK * a.d;
+  uint8_t* const v_block = a.v + block * E4M3_BLOCK * a.d;
+  // earlier keys under a larger scale, in whole words (beyond 2^-127 everything is zero)
+  if (offset > 0 && k_new > k_old && k_new != E4M3_NAN_SCALE) {
+    const float f = e4m3_scale(max(127 + k_old - k_new, 0));
+    for (int i = thread; i < offset * a.d / 4; i += threads) {
+      uint32_t* const word = reinterpret_cast<uint32_t*>(k_rows) + i;
+      *word = e4m3_again(*word, f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int r = me + i * STEP;
+    if (r >= n) continue;
+    uint8_t* const key = k_rows + (offset + r) * a.d;
+    uint8_t* const column = v_rows + offset + r;                 // a token's place in every feature's row
+    if constexpr (L::FAST) {
+      *reinterpret_cast<uint32_t*>(key + 4 * sub) = e4m3_pack4(kx[i][0] * k_times, kx[i][1] * k_times, kx[i][2] * k_times, kx[i][3] * k_times);
+      *reinterpret_cast<uint32_t*>(key + 4 * sub + half) = e4m3_pack4(ky[i][0] * k_times, ky[i][1] * k_times, ky[i][2] * k_times, ky[i][3] * k_times);
+    }
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) {
+      const int p = L::pair(sub, j);
+      if (p >= half) continue;
+      int ia, ib;
+      L::elements(p, a, ia, ib);
+      const uint16_t vv = e4m3_pack(vx[i][j] * v_times, vy[i][j] * v_times);
+      column[ia * V_PITCH] = (uint8_t)vv;
+      column[ib * V_PITCH] = (uint8_t)(vv >> 8);
+      if constexpr (!L::FAST) {
+        const uint16_t kk = e4m3_pack(kx[i][j] * k_times, ky[i][j] * k_times);
+        key[ia] = (uint8_t)kk;
+        key[ib] = (uint8_t)(kk >> 8);
+      }
+    }
+  }
+  sync();
+  // values: words of four tokens of a feature, those that hold a token of the run (or, under a larger scale, an earlier one)
+  const bool regrow = offset > 0 && v_new > v_old && v_new != E4M3_NAN_SCALE;
+  const float f = regrow ? e4m3_scale(max(127 + v_old - v_new, 0)) : 1.f;
+  const int w_first = regrow ? 0 : offset >> 2, w_count = ((offset + n - 1) >> 2) - w_first + 1;
+  if (w_count == 4 && n == E4M3_BLOCK) {
+    for (int feature = thread; feature < a.d; feature += threads) {
+      const uint32_t* const row = reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH);
+      *reinterpret_cast<uint4*>(v_block + feature * E4M3_BLOCK) = make_uint4(row[0], row[1], row[2], row[3]);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = thread; i < a.d * w_count; i += threads) {
+      const int feature = i % a.d, w0 = 4 * (w_first + i / a.d);
+      uint32_t* const word = reinterpret_cast<uint32_t*>(v_block + feature * E4M3_BLOCK + w0);
+      const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
+      uint32_t w = *reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH + w0) & new_bytes;
+      if (new_bytes != 0xffffffffu) {
+        uint32_t there = *word;
+        if (regrow) there = (there & ~old_bytes) | (e4m3_again(there, f) & old_bytes);
+        w |= there & ~new_bytes;
+      }
+      *word = w;
+    }
+  }
+  if (thread == 0) {
+    a.k_scale[block] = (uint8_t)k_new;
+    a.v_scale[block] = (uint8_t)v_new;
+  }
+  sync();                                                        // the next run takes the shared memory
+}
+
+// Blocks: `tile` neighbouring tokens' keys and values of a kv head, then query heads, WARPS * HEADS * Q_ITEMS of them.
+template <typename T, typename L>
+__global__ void __launch_bounds__(THREADS, L::LANES * L::PAIRS <= 64 ? 6 : 4) qkv_post_e4m3_kernel(const PostArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L::LANES;
   const int kv_blocks = (a.tokens + a.tile - 1) / a.tile * a.nkv;
 
   if ((int)blockIdx.x >= kv_blocks) {
-    // ------------------------------------------------------------ queries: a warp takes four heads
-    const int groups = (a.nq + E4M3_BLOCK - 1) / E4M3_BLOCK, block = (int)blockIdx.x - kv_blocks;
-    const int h0 = block % groups * E4M3_BLOCK + warp * PER_WARP;
-    const int step = a.tokens <= FEW ? 1 : Q_TOKENS, t0 = block / groups * step, count = min(step, a.tokens - t0);
-    float wx[PAIRS], wy[PAIRS];
-    load_norm<PAIRS, FAST>(a, a.q_norm_w, lane, wx, wy);
+    // ------------------------------------------------------------ queries: (token, head) pairs in their order
+    float wx[L::PAIRS], wy[L::PAIRS];
+    load_norm<L>(a, a.q_norm_w, sub, wx, wy);
+    constexpr int CHUNK = L::HEADS * Q_ITEMS;                    // heads of a token that a warp takes
+    const int of_token = (a.nq + CHUNK - 1) / CHUNK, chunk = ((int)blockIdx.x - kv_blocks) * WARPS + warp;
+    const int t = min(chunk / of_token, a.tokens - 1), h0 = chunk % of_token * CHUNK + lane / L::LANES;
+    const int pos = position_of(a, t);
     pdl_wait();
     pdl_launch_dependents();
-    if (h0 >= a.nq) return;
-    float x[Q_TOKENS][PER_WARP][PAIRS], y[Q_TOKENS][PER_WARP][PAIRS];
+    if (chunk >= a.tokens * of_token) return;
+    float x[Q_ITEMS][L::PAIRS], y[Q_ITEMS][L::PAIRS], c[L::PAIRS], s[L::PAIRS];
+    const int64_t in = (int64_t)t * (a.nq + 2 * a.nkv) * a.d, out = (int64_t)t * a.nq * a.d;
 #pragma unroll
-    for (int n = 0; n < Q_TOKENS; ++n)
+    for (int i = 0; i < Q_ITEMS; ++i)                            // (beyond the last head: the last one again, not stored)
+      load_head<T, L>(a, in + (int64_t)min(h0 + i * L::HEADS, a.nq - 1) * a.d, sub, x[i], y[i]);
+    load_turn<L>(a, pos, sub, c, s);                             // (behind the heads: the position has arrived by now)
 #pragma unroll
-      for (int i = 0; i < PER_WARP; ++i)
-        if (n < count && h0 + i < a.nq) load_head<T, PAIRS, FAST>(a, ((int64_t)(t0 + n) * heads + h0 + i) * a.d, lane, x[n][i], y[n][i]);
+    for (int i = 0; i < Q_ITEMS; ++i) norm_and_turn<L>(a, a.q_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
 #pragma unroll
-    for (int n = 0; n < Q_TOKENS; ++n) {
-      if (n >= count) break;
-      float c[PAIRS], s[PAIRS];
-      load_turn<PAIRS, FAST>(a, position_of(a, t0 + n), lane, c, s);
-      T* out = reinterpret_cast<T*>(a.q_out) + ((int64_t)(t0 + n) * a.nq + h0) * a.d;
-#pragma unroll
-      for (int i = 0; i < PER_WARP; ++i) {
-        if (h0 + i >= a.nq) break;
-        norm_and_turn<PAIRS>(a, a.q_norm_w != nullptr, x[n][i], y[n][i], wx, wy, c, s);
-        store_head<T, PAIRS, FAST>(a, out + (int64_t)i * a.d, lane, x[n][i], y[n][i]);
-      }
-    }
+    for (int i = 0; i < Q_ITEMS; ++i)
+      if (h0 + i * L::HEADS < a.nq) store_head<T, L>(a, reinterpret_cast<T*>(a.q_out) + out + (int64_t)(h0 + i * L::HEADS) * a.d, sub, x[i], y[i]);
     return;
   }
 
-  // -------------------------------------------------------------- keys and values of one kv head, run by run
-  extern __shared__ __align__(16) uint8_t v_rows[];             // [d][V_PITCH]: the run's values, feature-major, at their places in the block
-  __shared__ float most[2][WARPS];
-  __shared__ int broken[2][WARPS];
+  // -------------------------------------------------------------- keys and values of one kv head
+  extern __shared__ __align__(16) uint8_t rows_of_values[];     // [WARPS][d][V_PITCH]
+  __shared__ RunStats shared;
   const int g = (int)blockIdx.x % a.nkv, t_begin = (int)blockIdx.x / a.nkv * a.tile, t_end = min(a.tokens, t_begin + a.tile);
-  float wx[PAIRS], wy[PAIRS];
-  load_norm<PAIRS, FAST>(a, a.k_norm_w, lane, wx, wy);
-  // slots were written before the step began
+  float wx[L::PAIRS], wy[L::PAIRS];
+  load_norm<L>(a, a.k_norm_w, sub, wx, wy);
+  // which of the tile's tokens begin a run, and which runs are short (lane i: token t_begin + i; slots were written before the step)
   const int my_t = t_begin + lane;
-  auto slot_at = [&](int t) { return t >= 0 && t < a.tokens ? a.slot_mapping[t] : -1; };
-  // which of the tile's tokens begin a run (lane i: token t_begin + i)
-  bool begins = false;
+  bool begins = false, is_short = false;
   if (my_t < t_end) {
-    const int slot = slot_at(my_t), before = slot_at(my_t - 1);
+    const int slot = slot_at(a, my_t), before = slot_at(a, my_t - 1);
     if (slot < -1 || slot >= a.num_slots) {
       if (warp == 0 && g == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
     } else if (slot >= 0) {
@@ -267,161 +426,36 @@ __global__ void __launch_bounds__(THREADS, PAIRS >= 4 ? 4 : 8) qkv_post_e4m3_ker
       begins = !same;
       // a block's tokens of a step stand next to one another in its order; others are left out
       if (same && before != slot - 1 && warp == 0 && g == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
+      is_short = begins && !(slot % E4M3_BLOCK + SHORT < E4M3_BLOCK && slot_at(a, my_t + SHORT) == slot + SHORT);
     }
   }
-  unsigned runs = __ballot_sync(0xffffffffu, begins);
+  unsigned long_runs = __ballot_sync(0xffffffffu, begins && !is_short), short_runs = __ballot_sync(0xffffffffu, is_short);
   pdl_wait();
   pdl_launch_dependents();
-
-  for (; runs != 0; runs &= runs - 1) {                          // (the same in all warps)
-    const int t0 = t_begin + __ffs(runs) - 1;
-    const int slot = slot_at(t0), offset = slot % E4M3_BLOCK;
-    // the run's tokens: the neighbours that continue it
-    const int next = slot_at(t0 + lane);
-    const unsigned gone = ~__ballot_sync(0xffffffffu, offset + lane < E4M3_BLOCK && next == slot + lane);
-    const int n = __ffs(gone) - 1;                               // (lane 16 never continues it)
-    const int64_t page = slot / a.page_size, in_page = slot % a.page_size;
-    const int64_t block = (page * a.nkv + g) * (a.page_size / E4M3_BLOCK) + in_page / E4M3_BLOCK;
-
-    float kx[PER_WARP][PAIRS], ky[PER_WARP][PAIRS], vx[PER_WARP][PAIRS], vy[PER_WARP][PAIRS];
-    float k_most = 0.f, v_most = 0.f;
-    bool k_fine = true, v_fine = true;
-#pragma unroll
-    for (int i = 0; i < PER_WARP; ++i) {
-      const int r = warp + i * WARPS;
-      if (r >= n) break;
-      const int64_t at = ((int64_t)(t0 + r) * heads + a.nq + g) * a.d;
-      load_head<T, PAIRS, FAST>(a, at, lane, kx[i], ky[i]);
-      load_head<T, PAIRS, FAST>(a, at + (int64_t)a.nkv * a.d, lane, vx[i], vy[i]);
-    }
-    const int k_old = offset > 0 ? a.k_scale[block] : 0, v_old = offset > 0 ? a.v_scale[block] : 0;
-#pragma unroll
-    for (int i = 0; i < PER_WARP; ++i) {
-      const int r = warp + i * WARPS;
-      if (r >= n) break;
-      float c[PAIRS], s[PAIRS];
-      load_turn<PAIRS, FAST>(a, position_of(a, t0 + r), lane, c, s);
-      norm_and_turn<PAIRS>(a, a.k_norm_w != nullptr, kx[i], ky[i], wx, wy, c, s);
-      auto look = [](float v, float& top, bool& fine) {
-        const float size = fabsf(v);
-        const bool ok = size < E4M3_LIMIT;
-        fine = fine && ok;
-        if (ok) top = fmaxf(top, size);
-      };
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        look(kx[i][j], k_most, k_fine);
-        look(ky[i][j], k_most, k_fine);
-        look(vx[i][j], v_most, v_fine);
-        look(vy[i][j], v_most, v_fine);
-      }
-    }
-    k_most = warp_max(k_most);
-    v_most = warp_max(v_most);
-    const bool k_bad = __any_sync(0xffffffffu, !k_fine), v_bad = __any_sync(0xffffffffu, !v_fine);
-    if (lane == 0) {
-      most[0][warp] = k_most;
-      most[1][warp] = v_most;
-      broken[0][warp] = k_bad;
-      broken[1][warp] = v_bad;
-    }
-    __syncthreads();
-    int k_new, v_new;
-    {
-      float top[2] = {0.f, 0.f};
-      int bad[2] = {0, 0};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[i] = fmaxf(top[i], most[i][w]);
-          bad[i] |= broken[i][w];
-        }
-      k_new = bad[0] ? E4M3_NAN_SCALE : max(e4m3_scale_for(top[0]), k_old);
-      v_new = bad[1] ? E4M3_NAN_SCALE : max(e4m3_scale_for(top[1]), v_old);
-    }
-    // 2^-(scale - 127): the bits 254 - scale as an exponent (a scale that is no number: any payload will do)
-    const float k_times = __uint_as_float((uint32_t)max(254 - k_new, 1) << 23), v_times = __uint_as_float((uint32_t)max(254 - v_new, 1) << 23);
-    uint8_t* const k_rows = a.k + block * E4M3_BLOCK * a.d;
-    uint8_t* const v_block = a.v + block * E4M3_BLOCK * a.d;
-    // earlier keys under a larger scale: whole words, 2 tokens or more apart from the run's own rows
-    if (offset > 0 && k_new > k_old && k_new != E4M3_NAN_SCALE) {
-      const float f = e4m3_scale(max(127 + k_old - k_new, 0));   // (beyond 2^-127: everything is zero anyway)
-      for (int i = threadIdx.x; i < offset * a.d / 4; i += THREADS) {
-        uint32_t* const word = reinterpret_cast<uint32_t*>(k_rows) + i;
-        const uint32_t w = *word;
-        const float2 lo = e4m3_unpack((uint16_t)w), hi = e4m3_unpack((uint16_t)(w >> 16));
-        *word = (uint32_t)e4m3_pack(lo.x * f, lo.y * f) | (uint32_t)e4m3_pack(hi.x * f, hi.y * f) << 16;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < PER_WARP; ++i) {
-      const int r = warp + i * WARPS;
-      if (r >= n) break;
-      uint8_t* const key = k_rows + (offset + r) * a.d;
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        const int p = pair_index<PAIRS, FAST>(lane, j);
-        if (p >= half) continue;
-        int ia, ib;
-        pair_elements<FAST>(p, a, ia, ib);
-        const uint16_t vv = e4m3_pack(vx[i][j] * v_times, vy[i][j] * v_times);
-        v_rows[ia * V_PITCH + offset + r] = (uint8_t)vv;
-        v_rows[ib * V_PITCH + offset + r] = (uint8_t)(vv >> 8);
-        if (FAST && PAIRS > 1) {
-          if (j & 1) continue;
-          *reinterpret_cast<uint16_t*>(key + p) = e4m3_pack(kx[i][j] * k_times, kx[i][(j + 1) % PAIRS] * k_times);
-          *reinterpret_cast<uint16_t*>(key + p + half) = e4m3_pack(ky[i][j] * k_times, ky[i][(j + 1) % PAIRS] * k_times);
-          continue;
-        }
-        const uint16_t kk = e4m3_pack(kx[i][j] * k_times, ky[i][j] * k_times);
-        key[ia] = (uint8_t)kk;
-        key[ib] = (uint8_t)(kk >> 8);
-      }
-    }
-    __syncthreads();
-    // values: a thread takes a feature's 16 tokens, a word of four at a time
-    const bool regrow = offset > 0 && v_new > v_old && v_new != E4M3_NAN_SCALE;
-    const float f = regrow ? e4m3_scale(max(127 + v_old - v_new, 0)) : 1.f;
-    for (int i = threadIdx.x; i < a.d * 4; i += THREADS) {
-      const int feature = i >> 2, w0 = (i & 3) * 4;              // tokens w0 .. w0 + 3 of the block
-      if (w0 >= offset + n || (w0 + 4 <= offset && !regrow)) continue;
-      uint32_t* const word = reinterpret_cast<uint32_t*>(v_block + feature * E4M3_BLOCK) + (i & 3);
-      const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
-      uint32_t w = *reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH + w0) & new_bytes;
-      if (new_bytes != 0xffffffffu) {
-        uint32_t there = *word;
-        if (regrow) {
-          const float2 lo = e4m3_unpack((uint16_t)there), hi = e4m3_unpack((uint16_t)(there >> 16));
-          const uint32_t again = (uint32_t)e4m3_pack(lo.x * f, lo.y * f) | (uint32_t)e4m3_pack(hi.x * f, hi.y * f) << 16;
-          there = (there & ~old_bytes) | (again & old_bytes);
-        }
-        w |= there & ~new_bytes;
-      }
-      *word = w;
-    }
-    if (threadIdx.x == 0) {
-      a.k_scale[block] = (uint8_t)k_new;
-      a.v_scale[block] = (uint8_t)v_new;
-    }
-    __syncthreads();                                             // the next run takes the shared memory
-  }
+  for (; long_runs != 0; long_runs &= long_runs - 1)             // (the same in all warps)
+    store_run<T, L, true>(a, t_begin + __ffs(long_runs) - 1, g, rows_of_values, &shared, wx, wy);
+  for (int i = 0; short_runs != 0; short_runs &= short_runs - 1, ++i)
+    if (i % WARPS == warp) store_run<T, L, false>(a, t_begin + __ffs(short_runs) - 1, g, rows_of_values + warp * a.d * V_PITCH, nullptr, wx, wy);
 }
 
-template <typename T, int PAIRS, bool FAST>
+template <typename T, typename L>
 cudaError_t launch_post(const PostArgs& a, cudaStream_t stream) {
-  const int64_t q_steps = a.tokens <= FEW ? a.tokens : (a.tokens + Q_TOKENS - 1) / Q_TOKENS;
-  const dim3 grid((unsigned)((int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv + q_steps * ((a.nq + E4M3_BLOCK - 1) / E4M3_BLOCK)));
-  return vosti_launch(qkv_post_e4m3_kernel<T, PAIRS, FAST>, grid, dim3(THREADS), (size_t)a.d * V_PITCH, stream, a);
+  constexpr int CHUNK = L::HEADS * Q_ITEMS;
+  const int64_t q_blocks = ((int64_t)a.tokens * ((a.nq + CHUNK - 1) / CHUNK) + WARPS - 1) / WARPS;
+  const int64_t blocks = (int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv + q_blocks;
+  return vosti_launch(qkv_post_e4m3_kernel<T, L>, dim3((unsigned)blocks), dim3(THREADS), (size_t)WARPS * a.d * V_PITCH, stream, a);
 }
 template <typename T>
 cudaError_t launch_post_as(const PostArgs& a, cudaStream_t stream) {
-  // whole words: two elements of every operand
-  const uintptr_t words = (uintptr_t)a.partial | (uintptr_t)a.cos_table | (uintptr_t)a.sin_table, rows = (uintptr_t)a.qkv | (uintptr_t)a.q_out;
-  const bool whole = (a.cos_table == nullptr || (a.rotary_dim == a.d && !a.interleaved)) && (a.d == 64 || a.d == 128 || a.d == 256) &&
-                     words % 8 == 0 && rows % (2 * sizeof(T)) == 0;
-  if (whole) return a.d == 64 ? launch_post<T, 1, true>(a, stream) : a.d == 128 ? launch_post<T, 2, true>(a, stream) : launch_post<T, 4, true>(a, stream);
-  return a.d <= 64 ? launch_post<T, 1, false>(a, stream) : a.d <= 128 ? launch_post<T, 2, false>(a, stream) : launch_post<T, 4, false>(a, stream);
+  // whole words: four elements of every operand
+  const uintptr_t words = (uintptr_t)a.partial | (uintptr_t)a.cos_table | (uintptr_t)a.sin_table | (uintptr_t)a.q_norm_w | (uintptr_t)a.k_norm_w, rows = (uintptr_t)a.qkv | (uintptr_t)a.q_out;
+  if ((a.cos_table == nullptr || (a.rotary_dim == a.d && !a.interleaved)) && words % 16 == 0 && rows % (4 * sizeof(T)) == 0) {
+    if (a.d == 64) return launch_post<T, Lay<8, 4, true>>(a, stream);
+    if (a.d == 128) return launch_post<T, Lay<16, 4, true>>(a, stream);
+    if (a.d == 256) return launch_post<T, Lay<32, 4, true>>(a, stream);
+  }
+  if (a.d <= 64) return launch_post<T, Lay<32, 1, false>>(a, stream);
+  return a.d <= 128 ? launch_post<T, Lay<32, 2, false>>(a, stream) : launch_post<T, Lay<32, 4, false>>(a, stream);
 }
 
 }  // namespace
@@ -449,11 +483,12 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
   VOSTI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qkv_post_e4m3: the cache must start on 16 bytes");
   VOSTI_REQUIRE(slot_mapping != nullptr && k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr, "qkv_post_e4m3: the cache is missing");
   if (tokens == 0) return VOSTI_OK;
-  VOSTI_REQUIRE((int64_t)tokens * (nkv + (nq + E4M3_BLOCK - 1) / E4M3_BLOCK) <= 0x7fffffff, "qkv_post_e4m3: too many tokens and heads for one launch");
-  // few tokens: a CTA for each, so that none waits for another's run; many (prompts): a CTA for 16, one or two runs
-  const int tile = tokens <= FEW ? 1 : E4M3_BLOCK;
+  VOSTI_REQUIRE((int64_t)tokens * (nq + nkv) <= 0x7fffffff - 4096, "qkv_post_e4m3: too many tokens and heads for one launch");
+  // Few tokens: a CTA for each, so that none waits for another's run. Many: a CTA for eight, of which a prompt's hold a run or two and a batch of
+  // single tokens' two a warp. us, so and with a CTA for sixteen whose runs the CTA takes in turn: 128 single tokens 9.7 and 56, a prompt of 2,048 21.6 and 22.4.
+  const int tile = tokens <= FEW ? 1 : TILE;
   const PostArgs a = {qkv, partial, splits, (int64_t)tokens * (nq + 2 * nkv) * d, q_out, (uint8_t*)k, (uint8_t*)v, (uint8_t*)k_scale,
-                      (uint8_t*)v_scale, q_norm_w, k_norm_w, norm_w_is_f32, eps, cos_table, sin_table, max_positions, positions, slot_mapping,
+                      (uint8_t*)v_scale, q_norm_w, k_norm_w, norm_w_is_f32, eps, 1.f / (float)d, cos_table, sin_table, max_positions, positions, slot_mapping,
                       num_slots, page_size, tokens, nq, nkv, d, cos_table != nullptr ? rotary_dim : d, interleaved, tile, status};
   const cudaError_t e = is_f32 ? launch_post_as<float>(a, stream) : launch_post_as<bf16>(a, stream);
   if (e != cudaSuccess) {
