@@ -19,12 +19,21 @@ namespace {
 constexpr int KB = 128;                    // k of a block of codes: 64 bytes a row
 constexpr int TILE_BYTES = 16 * KB / 2;    // codes of 16 rows
 
-// Codes of k offsets 2 P and 2 P + 1 of a word, in bfloat16.
+// Codes of k offsets 2 P and 2 P + 1 of a word, in bfloat16. The constants are handed over in registers: mask and or are then one
+// instruction (with constants in place they were two, and the integer pipe, at half the issue rate, bounded the product).
+struct Int4Masks { uint32_t low, base, minus; };
+__device__ __forceinline__ Int4Masks int4_masks() {
+  Int4Masks m;
+  asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(m.low));
+  asm volatile("mov.b32 %0, 0x43004300;" : "=r"(m.base));
+  asm volatile("mov.b32 %0, 0xc308c308;" : "=r"(m.minus));
+  return m;
+}
 template <int P>
-__device__ __forceinline__ uint32_t int4_codes(uint32_t w) {
-  const uint32_t t = ((w >> (4 * P)) & 0x000f000fu) | 0x43004300u;
-  uint32_t r;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0xc308c308u));
+__device__ __forceinline__ uint32_t int4_codes(uint32_t w, const Int4Masks& m) {
+  uint32_t t, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(t) : "r"(w >> (4 * P)), "r"(m.low), "r"(m.base));
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(m.minus));
   return r;
 }
 __device__ __forceinline__ uint32_t int4_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -55,11 +64,15 @@ __device__ __forceinline__ void load_scales(const bf16* p, int left, uint32_t (&
 __device__ __forceinline__ float scale_of(uint32_t word, int i) { return __uint_as_float((i & 1) ? word & 0xffff0000u : word << 16); }
 
 // ---------------------------------------------------------------------------------------------- up to 16 tokens
-// A CTA takes FT tiles of 16 features over all of k, its eight warps every eighth block of 128 k, straight from memory into registers
-// one block ahead. The order of k inside an instruction is free: lane j of a row takes offsets 8 j .. 8 j + 7 of every 32 k, so that four of
-// them are a word's half and the tokens' 8 are one 16-byte load. An instruction never mixes groups: a group's codes are summed exactly, then
-// multiplied by its scale in float32. The warps' sums meet in shared memory, in warp order.
+// A CTA takes FT tiles of 16 features over all of k, each of its eight warps a run of the blocks of 128 k, which comes by bulk copies (a
+// tile's codes of neighbouring blocks are contiguous, and so are its scales) into two buffers of 4 KB of the warp's own: with three CTAs an
+// SM some 190 KB are on their way from the start. The order of k inside an instruction is free: lane j of a row takes offsets 8 j .. 8 j + 7
+// of every 32 k, so that four of them are a word's half and the tokens' 8 are one 16-byte load. An instruction never mixes groups: a group's codes
+// are summed exactly, then multiplied by its scale in float32. The warps' sums meet in shared memory, in warp order.
+// What bounds it: the weights' bytes, then the tokens, which every CTA reads again from L2 (as much as its weights, with FT = 2 and 8 tokens).
 constexpr int FEW_WARPS = 8, FEW_THREADS = FEW_WARPS * 32;
+constexpr int STAGE_CODES = 4096, FEW_STAGES = 2;
+template <int GROUPS> __host__ __device__ constexpr int stage_bytes() { return STAGE_CODES + 4 * 32 * GROUPS; }
 
 // 16 bytes of a token's row from element kk on; rows that do not start on whole words are read element by element, zeros beyond k.
 template <bool WORDS>
@@ -79,55 +92,81 @@ __device__ __forceinline__ uint4 load_tokens(const bf16* row, int kk, int k) {
 }
 
 template <int FT, int NT, int GROUPS, bool WORDS>
-__global__ void __launch_bounds__(FEW_THREADS)
+__global__ void __launch_bounds__(FEW_THREADS, NT == 1 ? 3 : 2)
 int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y, int y_is_f32,
-                int rows, int n, int k, int tiles, int deep) {
-  constexpr int SW = (GROUPS + 1) / 2;
-  __shared__ float sums[FEW_WARPS][NT * 8][FT * 16 + 4];
+                int rows, int n, int k, int tiles, int deep, unsigned* status) {
+  constexpr int SW = (GROUPS + 1) / 2, DEEP = 4 / FT, SCALES = 32 * GROUPS;       // blocks of k a buffer, bytes of a tile's scales a block
+  constexpr int STAGE = stage_bytes<GROUPS>();
+  extern __shared__ __align__(128) uint8_t ring[];             // [warp][buffer]: codes [FT][DEEP][1,024], then scales [FT][DEEP][SCALES]
+  __shared__ __align__(8) uint64_t full[FEW_WARPS][FEW_STAGES];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r8 = lane >> 2, j = lane & 3;
   const int tile0 = blockIdx.x * FT;
-  uint4 c[FT][2];
-  uint32_t s[FT][2][SW];
-  auto load = [&](int kb) {
-#pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const int64_t at = ((int64_t)min(tile0 + f, tiles - 1) * deep + kb) * 16;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        c[f][h] = load_codes(codes + (at + r8 + 8 * h) * (KB / 2) + 16 * j);
-        load_scales<GROUPS>(scales + (at + r8 + 8 * h) * GROUPS, k - kb * KB, s[f][h]);
-      }
+  const Int4Masks masks = int4_masks();
+  const int kb_begin = deep * warp / FEW_WARPS, blocks = deep * (warp + 1) / FEW_WARPS - kb_begin, stages = (blocks + DEEP - 1) / DEEP;
+  uint8_t* const mine = ring + warp * (FEW_STAGES * STAGE);
+  if (lane == 0) {
+    for (int i = 0; i < FEW_STAGES; ++i) mb_init(smem_addr(&full[warp][i]), 1);
+    mb_fence_init();
+  }
+  __syncwarp();
+  auto request = [&](int st) {                                   // lanes 0 .. FT - 1: a tile's codes and scales
+    const int count = min(DEEP, blocks - st * DEEP);
+    const uint32_t bar = smem_addr(&full[warp][st % FEW_STAGES]);
+    if (lane == 0) mb_expect_tx(bar, (uint32_t)(FT * count * (TILE_BYTES + SCALES)));
+    __syncwarp();
+    if (lane < FT) {
+      uint8_t* const to = mine + st % FEW_STAGES * STAGE;
+      const int64_t from = (int64_t)min(tile0 + lane, tiles - 1) * deep + kb_begin + st * DEEP;
+      bulk_copy_g2s(smem_addr(to + lane * DEEP * TILE_BYTES), codes + from * TILE_BYTES, (uint32_t)(count * TILE_BYTES), bar);
+      bulk_copy_g2s(smem_addr(to + STAGE_CODES + lane * DEEP * SCALES), reinterpret_cast<const uint8_t*>(scales) + from * SCALES, (uint32_t)(count * SCALES), bar);
     }
   };
-  // the first weights do not depend on the kernel before this one
-  if (warp < deep) load(warp);
+  // the weights do not depend on the kernel before this one
+  for (int st = 0; st < min(stages, FEW_STAGES); ++st) request(st);
   pdl_wait();
   pdl_launch_dependents();
-  float acc[FT][NT][4];
-#pragma unroll
-  for (int f = 0; f < FT; ++f)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[f][t][0] = acc[f][t][1] = acc[f][t][2] = acc[f][t][3] = 0.f;
-  for (int kb = warp; kb < deep; kb += FEW_WARPS) {
-    uint4 b[NT][4];                                              // [8 tokens][32 k]
+  uint4 b[NT][4];                                                // [8 tokens][32 k] of a block
+  auto load_block = [&](int kb) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         b[t][i] = t * 8 + r8 < rows ? load_tokens<WORDS>(x + (int64_t)(t * 8 + r8) * k, kb * KB + 32 * i + 8 * j, k) : make_uint4(0, 0, 0, 0);
-    uint4 now[FT][2];
-    uint32_t s_now[FT][2][SW];
+  };
+  if (blocks > 0) load_block(kb_begin);
+  float acc[FT][NT][4];
 #pragma unroll
-    for (int f = 0; f < FT; ++f)
+  for (int f = 0; f < FT; ++f)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        now[f][h] = c[f][h];
-#pragma unroll
-        for (int w = 0; w < SW; ++w) s_now[f][h][w] = s[f][h][w];
+    for (int t = 0; t < NT; ++t) acc[f][t][0] = acc[f][t][1] = acc[f][t][2] = acc[f][t][3] = 0.f;
+  for (int at = 0; at < blocks; ++at) {
+    const int st = at / DEEP, inside = at % DEEP;
+    if (inside == 0) {
+      const uint32_t bar = smem_addr(&full[warp][st % FEW_STAGES]);
+      if (!__all_sync(0xffffffffu, mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status))) {
+        // reported; once more, so that none of the warp's copies is in flight when it ends
+        (void)mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status);
+        if (st + 1 < stages) (void)mb_wait(smem_addr(&full[warp][(st + 1) % FEW_STAGES]), (uint32_t)((st + 1) / FEW_STAGES) & 1, status);
+        break;
       }
-    if (kb + FEW_WARPS < deep) load(kb + FEW_WARPS);
+    }
+    uint4 now[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) now[t][i] = b[t][i];
+    if (at + 1 < blocks) load_block(kb_begin + at + 1);
+    const uint8_t* const stage = mine + st % FEW_STAGES * STAGE + inside * TILE_BYTES;
+    const bf16* const stage_scales = reinterpret_cast<const bf16*>(mine + st % FEW_STAGES * STAGE + STAGE_CODES + inside * SCALES);
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
+      uint4 c[2];
+      uint32_t s[2][SW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[h] = *reinterpret_cast<const uint4*>(stage + f * DEEP * TILE_BYTES + (r8 + 8 * h) * (KB / 2) + 16 * j);
+        load_scales<GROUPS>(stage_scales + f * DEEP * (SCALES / 2) + (r8 + 8 * h) * GROUPS, k - (kb_begin + at) * KB, s[h]);
+      }
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         float part[NT][4];
@@ -135,16 +174,16 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
         for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
 #pragma unroll
         for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
-          const uint32_t lo = int4_word(now[f][0], i), hi = int4_word(now[f][1], i);
-          const uint32_t first[4] = {int4_codes<0>(lo), int4_codes<0>(hi), int4_codes<1>(lo), int4_codes<1>(hi)};
-          const uint32_t second[4] = {int4_codes<2>(lo), int4_codes<2>(hi), int4_codes<3>(lo), int4_codes<3>(hi)};
+          const uint32_t lo = int4_word(c[0], i), hi = int4_word(c[1], i);
+          const uint32_t first[4] = {int4_codes<0>(lo, masks), int4_codes<0>(hi, masks), int4_codes<1>(lo, masks), int4_codes<1>(hi, masks)};
+          const uint32_t second[4] = {int4_codes<2>(lo, masks), int4_codes<2>(hi, masks), int4_codes<3>(lo, masks), int4_codes<3>(hi, masks)};
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_bf16(part[t], first, b[t][i].x, b[t][i].y);
-            mma_bf16(part[t], second, b[t][i].z, b[t][i].w);
+            mma_bf16(part[t], first, now[t][i].x, now[t][i].y);
+            mma_bf16(part[t], second, now[t][i].z, now[t][i].w);
           }
         }
-        const float s0 = scale_of(s_now[f][0][g / 2], g), s1 = scale_of(s_now[f][1][g / 2], g);
+        const float s0 = scale_of(s[0][g / 2], g), s1 = scale_of(s[1][g / 2], g);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           acc[f][t][0] = fmaf(part[t][0], s0, acc[f][t][0]);
@@ -154,20 +193,27 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
         }
       }
     }
+    if (inside == DEEP - 1 && st + FEW_STAGES < stages) {
+      __syncwarp();                                              // every lane has read the buffer
+      request(st + FEW_STAGES);
+    }
   }
+  __syncthreads();                                               // the buffers' place takes the sums
+  constexpr int PITCH = FT * 16 + 4;
+  float* const sums = reinterpret_cast<float*>(ring);            // [warp][token][feature]
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[warp][t * 8 + 2 * j + (e & 1)][f * 16 + r8 + 8 * (e >> 1)] = acc[f][t][e];
+      for (int e = 0; e < 4; ++e) sums[(warp * NT * 8 + t * 8 + 2 * j + (e & 1)) * PITCH + f * 16 + r8 + 8 * (e >> 1)] = acc[f][t][e];
   __syncthreads();
   for (int i = threadIdx.x; i < rows * FT * 16; i += FEW_THREADS) {
     const int t = i / (FT * 16), f = i % (FT * 16);
     if (tile0 * 16 + f >= n) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < FEW_WARPS; ++w) v += sums[w][t][f];
+    for (int w = 0; w < FEW_WARPS; ++w) v += sums[(w * NT * 8 + t) * PITCH + f];
     const int64_t at = (int64_t)t * n + tile0 * 16 + f;
     if (y_is_f32) reinterpret_cast<float*>(y)[at] = v;
     else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
@@ -302,6 +348,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   const uint8_t* const my_codes = codes + row * (KB / 2) + 32 * half;
   const bf16* const my_scales = scales + row * GROUPS;
   const uint32_t my_a = tmem_a + ((uint32_t)(quarter * 32) << 16) + 8 * half;
+  const Int4Masks masks = int4_masks();
   uint4 c[DEPTH][2];
   uint32_t sc[DEPTH][SW];
   auto load = [&](int b, int d) {
@@ -329,9 +376,9 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
         const int g = i * GROUPS / 4;
         const uint32_t two = __byte_perm(sc[d][g / 2], 0, (g & 1) ? 0x3232 : 0x1010);
         const uint32_t lo = int4_word(c[d][0], i), hi = int4_word(c[d][1], i);
-        const uint32_t r[8] = {int4_times(int4_codes<0>(lo), two), int4_times(int4_codes<1>(lo), two), int4_times(int4_codes<2>(lo), two),
-                               int4_times(int4_codes<3>(lo), two), int4_times(int4_codes<0>(hi), two), int4_times(int4_codes<1>(hi), two),
-                               int4_times(int4_codes<2>(hi), two), int4_times(int4_codes<3>(hi), two)};
+        const uint32_t r[8] = {int4_times(int4_codes<0>(lo, masks), two), int4_times(int4_codes<1>(lo, masks), two), int4_times(int4_codes<2>(lo, masks), two),
+                               int4_times(int4_codes<3>(lo, masks), two), int4_times(int4_codes<0>(hi, masks), two), int4_times(int4_codes<1>(hi, masks), two),
+                               int4_times(int4_codes<2>(hi, masks), two), int4_times(int4_codes<3>(hi, masks), two)};
         int4_tmem_store8(my_a + s * A_COLS + 16 * i, r);
       }
       if (b + DEPTH < blocks) load(b + DEPTH, d);
@@ -426,20 +473,26 @@ struct Int4Args {
   cudaStream_t stream;
 };
 
-template <int FT, int NT, int GROUPS>
-cudaError_t launch_few(const Int4Args& a, bool words) {
-  const dim3 grid((a.tiles + FT - 1) / FT);
-  if (words)
-    return vosti_launch(int4_few_kernel<FT, NT, GROUPS, true>, grid, dim3(FEW_THREADS), 0, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n,
-                        a.k, a.tiles, a.deep);
-  return vosti_launch(int4_few_kernel<FT, NT, GROUPS, false>, grid, dim3(FEW_THREADS), 0, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n,
-                      a.k, a.tiles, a.deep);
+template <int FT, int NT, int GROUPS, bool WORDS>
+cudaError_t launch_few(const Int4Args& a) {
+  auto kernel = int4_few_kernel<FT, NT, GROUPS, WORDS>;
+  constexpr int SMEM = FEW_WARPS * FEW_STAGES * stage_bytes<GROUPS>();
+  static_assert(FEW_WARPS * NT * 8 * (FT * 16 + 4) * 4 <= SMEM, "the sums take the buffers' place");
+  const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (raised != cudaSuccess) return raised;
+  return vosti_launch(kernel, dim3((a.tiles + FT - 1) / FT), dim3(FEW_THREADS), SMEM, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n, a.k,
+                      a.tiles, a.deep, a.status);
+}
+// Tiles of 16 features a CTA: as many as leave two CTAs an SM.
+template <int GROUPS, int NT>
+cudaError_t launch_few_as(const Int4Args& a, bool words) {
+  if (!words) return launch_few<1, NT, GROUPS, false>(a);
+  if (a.tiles >= 4 * 296) return launch_few<4, NT, GROUPS, true>(a);
+  return a.tiles >= 2 * 296 ? launch_few<2, NT, GROUPS, true>(a) : launch_few<1, NT, GROUPS, true>(a);
 }
 template <int GROUPS>
-cudaError_t launch_few_as(const Int4Args& a, bool words) {
-  const bool wide = a.tiles > 2 * 148;
-  if (a.rows <= 8) return wide ? launch_few<2, 1, GROUPS>(a, words) : launch_few<1, 1, GROUPS>(a, words);
-  return wide ? launch_few<2, 2, GROUPS>(a, words) : launch_few<1, 2, GROUPS>(a, words);
+cudaError_t launch_few_groups(const Int4Args& a, bool words) {
+  return a.rows <= 8 ? launch_few_as<GROUPS, 1>(a, words) : launch_few_as<GROUPS, 2>(a, words);
 }
 
 template <int TOK, int GROUPS>
@@ -487,7 +540,7 @@ VOSTI_API int vosti_gemm_int4(const void* x, const void* codes, const void* scal
                               unsigned* status, cudaStream_t stream) {
   VOSTI_REQUIRE(rows >= 0 && n > 0 && k > 0, "gemm_int4: bad sizes rows=%d n=%d k=%d", rows, n, k);
   VOSTI_REQUIRE(group == 32 || group == 64 || group == 128, "gemm_int4: the group is 32, 64 or 128, not %d", group);
-  VOSTI_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 7) == 0, "gemm_int4: the weights must start on whole words");
+  VOSTI_REQUIRE((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "gemm_int4: the weights must start on 16 bytes");
   if (rows == 0) return VOSTI_OK;
   Int4Args a = {(const bf16*)x, (const uint8_t*)codes, (const bf16*)scales, y, y_is_f32, rows, n, k, (n + 15) / 16, (k + KB - 1) / KB, status, stream};
   // whole words of eight tokens' elements: every row starts on 16 bytes
@@ -501,7 +554,7 @@ VOSTI_API int vosti_gemm_int4(const void* x, const void* codes, const void* scal
     a.x = (const bf16*)x + (int64_t)t * k;
     a.y = (uint8_t*)y + (int64_t)t * n * (y_is_f32 ? 4 : 2);
     a.rows = rows - t < 16 ? rows - t : 16;
-    const cudaError_t e = group == 32 ? launch_few_as<4>(a, words) : group == 64 ? launch_few_as<2>(a, words) : launch_few_as<1>(a, words);
+    const cudaError_t e = group == 32 ? launch_few_groups<4>(a, words) : group == 64 ? launch_few_groups<2>(a, words) : launch_few_groups<1>(a, words);
     if (e != cudaSuccess) {
       vosti_set_error("gemm_int4: %s", cudaGetErrorString(e));
       return (int)e;

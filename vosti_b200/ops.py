@@ -2475,8 +2475,8 @@ class Int4Weight:
             raise KernelError(f"Int4Weight: scales are bfloat16 {(tiles, deep, 16)} x (128 / group), the group 32, 64 or 128, got {scales.dtype} {tuple(scales.shape)}")
         if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
             raise KernelError("Int4Weight: codes and scales are contiguous, on one device")
-        if codes.data_ptr() % 16 or scales.data_ptr() % 8:
-            raise KernelError("Int4Weight: codes start on 16 bytes, scales on 8")
+        if (codes.data_ptr() | scales.data_ptr()) % 16:
+            raise KernelError("Int4Weight: codes and scales start on 16 bytes")
         self.codes, self.scales, self.shape, self.group, self.device = codes, scales, (features, k), 128 // scales.shape[3], codes.device
 
     @property
