@@ -225,13 +225,16 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
 // memory. Eight warps read the codes into registers DEPTH blocks ahead (a thread: half a feature's block, one 32-byte sector), make them
 // bfloat16 times their scale (rounded once: codes of 1, 2, 4 and 8 are exact) and store them to one of two stages in tensor memory; a
 // ninth warp issues the MMAs, a tenth brings the tokens by TMA.
-constexpr int WORKERS = 256, TILE_THREADS = WORKERS + 64;
 constexpr int FEATURES = 128;
-constexpr int A_STAGES = 2, A_COLS = KB / 2;
-constexpr int DEPTH = 4;
+constexpr int A_COLS = KB / 2;
+
+constexpr int MAX_SEGMENTS = 8;
 
 template <int TOK>
 struct Int4Tile {
+  // A tile of 256 tokens fills its SM: two groups of eight warps fill its four stages of weights in turn. (Smaller ones: two CTAs an SM.)
+  static constexpr int GROUPS = TOK > 128 ? 2 : 1, A_STAGES = 2 * GROUPS, DEPTH = 4 / GROUPS;
+  static constexpr int WORKERS = 256 * GROUPS, THREADS = WORKERS + 64;
   static constexpr int X_STAGE = TOK * KB * 2;
   static constexpr int X_STAGES = TOK >= 128 ? 3 : 4;
   static constexpr int COLS = TOK + A_STAGES * A_COLS <= 256 ? 256 : 512;
@@ -267,17 +270,19 @@ __device__ __forceinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatil
   __syncwarp();
   return ok;
 }
+template <int WORKERS>
 __device__ __forceinline__ void int4_workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
 
 template <int TOK, int GROUPS>
-__global__ void __launch_bounds__(TILE_THREADS, Int4Tile<TOK>::CTAS)
+__global__ void __launch_bounds__(Int4Tile<TOK>::THREADS, Int4Tile<TOK>::CTAS)
 int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y,
                   int y_is_f32, int rows, int n, int k, int tiles, int deep, int token_tiles, int segments, unsigned* status) {
   using Tile = Int4Tile<TOK>;
-  constexpr int SW = (GROUPS + 1) / 2, COLS = TOK / 2;
+  constexpr int SW = (GROUPS + 1) / 2, WORKERS = Tile::WORKERS, A_STAGES = Tile::A_STAGES, DEPTH = Tile::DEPTH, TURNS = Tile::GROUPS;
+  constexpr int COLS = TOK / (WORKERS / 128);                    // token columns of a warp at the end
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t x_full[Tile::X_STAGES], x_empty[Tile::X_STAGES], a_full[A_STAGES], a_empty[A_STAGES];
+  __shared__ __align__(8) uint64_t x_full[Tile::X_STAGES], x_empty[Tile::X_STAGES], a_full[A_STAGES], a_empty[A_STAGES], done;
   __shared__ uint32_t tmem_base_holder;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -292,9 +297,10 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       mbar_init(smem_u32(&x_empty[s]), 1);
     }
     for (int s = 0; s < A_STAGES; ++s) {
-      mbar_init(smem_u32(&a_full[s]), WORKERS / 32);
+      mbar_init(smem_u32(&a_full[s]), 8);
       mbar_init(smem_u32(&a_empty[s]), 1);
     }
+    mbar_init(smem_u32(&done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(smem_u32(&tmem_base_holder), Tile::COLS);
@@ -335,6 +341,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
           umma_bf16_ts(tmem_sum, tmem_a + s * A_COLS + 8 * q, desc + (uint64_t)(((q >> 2) * (TOK * 128) + (q & 3) * 32) >> 4), idesc, b > 0 || q > 0);
         umma_commit(smem_u32(&a_empty[s]));
         umma_commit(smem_u32(&x_empty[xs]));
+        if (b + 1 == blocks) umma_commit(smem_u32(&done));
       }
       __syncwarp();
     }
@@ -342,7 +349,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   }
 
   // -------------------------------------------------------------- workers
-  const int quarter = warp & 3, half = warp >> 2, feature = quarter * 32 + lane;
+  const int quarter = warp & 3, half = (warp >> 2) & 1, turn = warp >> 3, feature = quarter * 32 + lane;
   const int tile = min(f0 / 16 + feature / 16, tiles - 1);       // (rows beyond the matrix are never stored)
   const int64_t row = ((int64_t)tile * deep + kb_begin) * 16 + feature % 16;
   const uint8_t* const my_codes = codes + row * (KB / 2) + 32 * half;
@@ -359,12 +366,12 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   };
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
-    if (d < blocks) load(d, d);
+    if (turn + d * TURNS < blocks) load(turn + d * TURNS, d);
   bool ok = true;
-  for (int b0 = 0; b0 < blocks && ok; b0 += DEPTH) {
+  for (int b0 = turn; b0 < blocks && ok; b0 += DEPTH * TURNS) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const int b = b0 + d, s = b % A_STAGES;
+      const int b = b0 + d * TURNS, s = b % A_STAGES;
       if (b >= blocks || !ok) break;
       if (b >= A_STAGES) {
         ok = int4_wait(smem_u32(&a_empty[s]), (b / A_STAGES - 1) & 1, &abort_flag, status);
@@ -381,18 +388,19 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
                                int4_times(int4_codes<2>(hi, masks), two), int4_times(int4_codes<3>(hi, masks), two)};
         int4_tmem_store8(my_a + s * A_COLS + 16 * i, r);
       }
-      if (b + DEPTH < blocks) load(b + DEPTH, d);
+      if (b + DEPTH * TURNS < blocks) load(b + DEPTH * TURNS, d);
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&a_full[s]));
     }
   }
-  if (ok && blocks > 0) ok = int4_wait(smem_u32(&a_empty[(blocks - 1) % A_STAGES]), ((blocks - 1) / A_STAGES) & 1, &abort_flag, status);
+  // (a barrier of its own: a group of warps that never waited for a stage's earlier phase could take it for the last)
+  if (ok && blocks > 0) ok = int4_wait(smem_u32(&done), 0, &abort_flag, status);
   tc_fence_after();
   pdl_wait();                                                    // (what this kernel writes may still be read before that)
 
-  const uint32_t my_sums = tmem_sum + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+  const uint32_t my_sums = tmem_sum + ((uint32_t)(quarter * 32) << 16) + (warp >> 2) * COLS;
   auto store = [&](int t, int f, float v) {
     if (t0 + t >= rows || f0 + f >= n) return;
     const int64_t at = (int64_t)(t0 + t) * n + f0 + f;
@@ -416,7 +424,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
     }
 #pragma unroll
     for (int i = 0; i < STEP; ++i) {
-      const int t = half * COLS + c0 + i;
+      const int t = (warp >> 2) * COLS + c0 + i;
       if (segments == 1) store(t, feature, __uint_as_float(r[i]));
       else part[t * FEATURES + feature] = __uint_as_float(r[i]);
     }
@@ -430,14 +438,20 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       const int t = lo + word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
       if (t0 + t >= rows) break;
       const uint32_t at = smem_u32(&part[t * FEATURES + f]);
-      float4 v = int4_load_rank(at, 0);
-      for (int r = 1; r < segments; ++r) {
-        const float4 u = int4_load_rank(at, r);
-        v.x += u.x;
-        v.y += u.y;
-        v.z += u.z;
-        v.w += u.w;
-      }
+      // (all of them on their way at once: one after the other, eight took 4 us)
+      float4 u[MAX_SEGMENTS];
+#pragma unroll
+      for (int r = 0; r < MAX_SEGMENTS; ++r)
+        if (r < segments) u[r] = int4_load_rank(at, r);
+      float4 v = u[0];
+#pragma unroll
+      for (int r = 1; r < MAX_SEGMENTS; ++r)
+        if (r < segments) {
+          v.x += u[r].x;
+          v.y += u[r].y;
+          v.z += u[r].z;
+          v.w += u[r].w;
+        }
       store(t, f, v.x);
       store(t, f + 1, v.y);
       store(t, f + 2, v.z);
@@ -445,10 +459,10 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
     }
     cluster_sync_all();                                          // nobody reads this CTA's sums after this
   }
-  int4_workers_sync();
+  int4_workers_sync<WORKERS>();
   if (abort_flag) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
-    int4_workers_sync();
+    int4_workers_sync<WORKERS>();
   }
   if (warp == 0) {
     tc_fence_after();
@@ -459,7 +473,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
 // Segments of k: as many as still find an SM, each of four blocks at least.
 int int4_segments(int64_t ctas, int deep, int at_once) {
   int s = 1;
-  while (s < 8 && ctas * s * 2 <= at_once && deep >= 8 * s) s *= 2;
+  while (s < MAX_SEGMENTS && ctas * s * 2 <= at_once && deep >= 8 * s) s *= 2;
   return s;
 }
 
@@ -507,7 +521,7 @@ int launch_tiles(const Int4Args& a) {
   const int64_t whole = (int64_t)((a.n + FEATURES - 1) / FEATURES) * token_tiles;
   const int segments = int4_segments(whole, a.deep, 140 * Int4Tile<TOK>::CTAS);
   VOSTI_REQUIRE(whole * segments <= 0x7fffffff, "gemm_int4: too many tiles for one launch");
-  const cudaError_t e = vosti_launch_clusters(kernel, dim3((unsigned)(whole * segments)), dim3(TILE_THREADS), (unsigned)segments, SMEM, a.stream, map,
+  const cudaError_t e = vosti_launch_clusters(kernel, dim3((unsigned)(whole * segments)), dim3(Int4Tile<TOK>::THREADS), (unsigned)segments, SMEM, a.stream, map,
                                               a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n, a.k, a.tiles, a.deep, token_tiles, segments, a.status);
   VOSTI_REQUIRE(e == cudaSuccess, "gemm_int4: %s", cudaGetErrorString(e));
   return VOSTI_OK;
