@@ -94,7 +94,7 @@ template <int D>
 __global__ void __launch_bounds__(THREADS, RESIDENT)
 attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const CacheArgs c, const int* __restrict__ token_list,
                       const int* __restrict__ positions, const int* __restrict__ request_of, int nq, int nkv, float scale_log2, int window,
-                      int segments, int ordered, unsigned* status) {
+                      int segments, int ordered, int beside, unsigned* status) {
   constexpr int CHUNKS = D / 64, FT = D / 16;
   constexpr int RAISED = 15;
   // a warp's buffers: four blocks of keys, and four of values whose starts lie 32 bytes apart in the banks (lanes read all four at once)
@@ -194,8 +194,11 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
     return false;
   };
 
+  // `beside`: the kernel before this one is the same step's attention of portions, which neither writes what this one reads nor reads what it
+  // writes, and waited for everything before it in all of its CTAs before it let this one start. It is waited for at the end only
+  // (the chain of completed kernels stays unbroken).
   int64_t next = block_of(begin + warp);
-  pdl_wait();
+  if (!beside) pdl_wait();
   pdl_launch_dependents();
   if (begin + warp < end) {
     request(0, next);
@@ -422,6 +425,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
       for (int w = 0; w < WARPS; ++w) v += part[w][h][f];
       out[q_at + i] = finish(v, joined(stats, WARPS, h));
     }
+    if (beside) pdl_wait();
     return;
   }
   // ---- the segments' sums into one, in their order: each CTA of the cluster is sent its share of the row by all of them
@@ -451,6 +455,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
     for (int s = 0; s < segments; ++s) v += inbox[s * share + i] * fast_exp2(inbox_stats[s][h][2] - safe_v);
     out[q_at + seg * share + i] = finish(v, r);
   }
+  if (beside) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------------- CUDA cores
@@ -618,7 +623,7 @@ struct Launch {
   CacheArgs c;
   const int *token_list, *positions, *request_of;
   int64_t items;
-  int nq, nkv, window, segments, ordered;
+  int nq, nkv, window, segments, ordered, beside;
   float scale_log2;
   unsigned* status;
   cudaStream_t stream;
@@ -635,9 +640,9 @@ cudaError_t launch_e4m3(const Launch& a) {
   const dim3 grid((unsigned)(a.items * segments));
   if (segments == 1)
     return vosti_launch(kernel, grid, dim3(THREADS), SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,
-                        a.window, 1, a.ordered, a.status);
+                        a.window, 1, a.ordered, a.beside, a.status);
   return vosti_launch_clusters(kernel, grid, dim3(THREADS), (unsigned)segments, SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of,
-                               a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.status);
+                               a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.beside, a.status);
 }
 int check_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, const int* block_table, int max_pages, int page_size,
                 int num_pages, int nq, int nkv, float scale, int window) {
@@ -652,11 +657,12 @@ int check_cache(const void* k, const void* v, const void* k_scale, const void* v
 
 }  // namespace
 
-// q, out: bfloat16 [tokens, nq * d]; the cache as in e4m3.cuh. `token_list` (or null: 0 .. count - 1) names the tokens; d is 64 or 128.
+// q, out: bfloat16 [tokens, nq * d]; the cache as in e4m3.cuh. `token_list` (or null: 0 .. count - 1) names the tokens; d is 64 or 128. `beside`: the
+// launch right before this one on the stream is vosti_attention_prefill_tc_e4m3 for other rows of the same q, out and cache.
 VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, void* out,
                                    const int* token_list, int count, const int* positions, const int* request_of, const int* block_table,
                                    int max_pages, int page_size, int num_pages, int nq, int nkv, int d, int max_kv_len, float scale, int window,
-                                   unsigned* status, cudaStream_t stream) {
+                                   int beside, unsigned* status, cudaStream_t stream) {
   if (int bad = check_cache(k, v, k_scale, v_scale, block_table, max_pages, page_size, num_pages, nq, nkv, scale, window)) return bad;
   VOSTI_REQUIRE(d == 64 || d == 128, "attention_e4m3: head_dim %d must be 64 or 128", d);
   VOSTI_REQUIRE((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "attention_e4m3: queries must start on 16 bytes");
@@ -667,7 +673,7 @@ VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, 
   // more CTAs than run at once: those of the tokens with most keys first
   const bool ordered = items > 148 * RESIDENT && count > 1 && count <= MAX_ORDERED;
   const Launch launch = {(const bf16*)q, (bf16*)out, c, token_list, positions, request_of, items, nq, nkv, window, segments_of(items, max_kv_len),
-                         ordered ? count : 0, scale * LOG2E, status, stream};
+                         ordered ? count : 0, beside, scale * LOG2E, status, stream};
   const cudaError_t e = d == 64 ? launch_e4m3<64>(launch) : launch_e4m3<128>(launch);
   if (e != cudaSuccess) {
     vosti_set_error("attention_e4m3: %s", cudaGetErrorString(e));
