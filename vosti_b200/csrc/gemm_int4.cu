@@ -232,13 +232,12 @@ constexpr int MAX_SEGMENTS = 8;
 
 template <int TOK>
 struct Int4Tile {
-  // A tile of 256 tokens fills its SM: two groups of eight warps fill its four stages of weights in turn. (Smaller ones: two CTAs an SM.)
-  static constexpr int GROUPS = TOK > 128 ? 2 : 1, A_STAGES = 2 * GROUPS, DEPTH = 4 / GROUPS;
-  static constexpr int WORKERS = 256 * GROUPS, THREADS = WORKERS + 64;
-  static constexpr int X_STAGE = TOK * KB * 2;
-  static constexpr int X_STAGES = TOK >= 128 ? 3 : 4;
-  static constexpr int COLS = TOK + A_STAGES * A_COLS <= 256 ? 256 : 512;
-  static constexpr int RING = X_STAGES * X_STAGE, SUMS = TOK * FEATURES * 4;
+  // Eight warps fill the stages' weights, DEPTH blocks asked for ahead; up to 128 tokens two CTAs share an SM, above two groups of eight
+  // warps take a CTA's stages in turn (one CTA with two groups for 24,576 x 4,096 of 128 tokens: 38 us, two with one 32).
+  static constexpr int GROUPS = TOK > 128 ? 2 : 1, DEPTH = 4, WORKERS = 256 * GROUPS, THREADS = WORKERS + 64;
+  static constexpr int X_STAGE = TOK * KB * 2, STAGES = TOK > 128 ? 3 : TOK > 64 ? 2 : 3;
+  static constexpr int COLS = TOK + STAGES * A_COLS <= 256 ? 256 : 512;
+  static constexpr int RING = STAGES * X_STAGE, SUMS = TOK * FEATURES * 4;
   // no more CTAs an SM than tensor memory has columns for: shared memory (228 KB, 1 KB of it with every CTA) is padded until that many fit
   static constexpr int FEWEST = 228 * 1024 / (512 / COLS + 1);
   static constexpr int NEEDED = (RING > SUMS ? RING : SUMS) + 1024;
@@ -263,12 +262,9 @@ __device__ __forceinline__ float4 int4_load_rank(uint32_t smem_at, uint32_t rank
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
 }
+// A wait of every lane: 50 cycles where the phase is complete already, as it should be (with the clock read first 105, one lane asking for all 290).
 __device__ __forceinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
-  bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, status);
-  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-  __syncwarp();
-  return ok;
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag, status);
 }
 template <int WORKERS>
 __device__ __forceinline__ void int4_workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
@@ -278,11 +274,12 @@ __global__ void __launch_bounds__(Int4Tile<TOK>::THREADS, Int4Tile<TOK>::CTAS)
 int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y,
                   int y_is_f32, int rows, int n, int k, int tiles, int deep, int token_tiles, int segments, unsigned* status) {
   using Tile = Int4Tile<TOK>;
-  constexpr int SW = (GROUPS + 1) / 2, WORKERS = Tile::WORKERS, A_STAGES = Tile::A_STAGES, DEPTH = Tile::DEPTH, TURNS = Tile::GROUPS;
+  constexpr int SW = (GROUPS + 1) / 2, WORKERS = Tile::WORKERS, STAGES = Tile::STAGES, DEPTH = Tile::DEPTH, TURNS = Tile::GROUPS;
   constexpr int COLS = TOK / (WORKERS / 128);                    // token columns of a warp at the end
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t x_full[Tile::X_STAGES], x_empty[Tile::X_STAGES], a_full[A_STAGES], a_empty[A_STAGES], done;
+  // a stage: the tokens have arrived and eight warps have stored the weights; its MMAs are complete; all MMAs are
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], done;
   __shared__ uint32_t tmem_base_holder;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -292,13 +289,9 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < Tile::X_STAGES; ++s) {
-      mbar_init(smem_u32(&x_full[s]), 1);
-      mbar_init(smem_u32(&x_empty[s]), 1);
-    }
-    for (int s = 0; s < A_STAGES; ++s) {
-      mbar_init(smem_u32(&a_full[s]), 8);
-      mbar_init(smem_u32(&a_empty[s]), 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 9);
+      mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(&done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -314,11 +307,11 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
     if (lane == 0) {
       pdl_wait();
       for (int b = 0; b < blocks; ++b) {
-        const int s = b % Tile::X_STAGES;
-        if (b >= Tile::X_STAGES && !mbar_wait(smem_u32(&x_empty[s]), (b / Tile::X_STAGES - 1) & 1, &abort_flag, status)) break;
-        mbar_expect_tx(smem_u32(&x_full[s]), (uint32_t)Tile::X_STAGE);
+        const int s = b % STAGES;
+        if (b >= STAGES && !int4_wait(smem_u32(&empty[s]), (b / STAGES - 1) & 1, &abort_flag, status)) break;
+        mbar_expect_tx(smem_u32(&full[s]), (uint32_t)Tile::X_STAGE);
         for (int h = 0; h < 2; ++h)
-          tma_load_2d(smem_u32(smem + s * Tile::X_STAGE + h * (TOK * 128)), &map_x, (kb_begin + b) * KB + h * 64, t0, smem_u32(&x_full[s]));
+          tma_load_2d(smem_u32(smem + s * Tile::X_STAGE + h * (TOK * 128)), &map_x, (kb_begin + b) * KB + h * 64, t0, smem_u32(&full[s]));
       }
     }
     return;
@@ -326,21 +319,17 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   if (warp == WORKERS / 32) {
     constexpr uint32_t idesc = umma_instr_desc(FEATURES, TOK, false);
     bool ok = true;
-    auto arrived = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &abort_flag, status)) != 0;
-    };
     for (int b = 0; b < blocks && ok; ++b) {
-      const int s = b % A_STAGES, xs = b % Tile::X_STAGES;
-      ok = arrived(&x_full[xs], (b / Tile::X_STAGES) & 1) && arrived(&a_full[s], (b / A_STAGES) & 1);
+      const int s = b % STAGES;
+      ok = __all_sync(0xffffffffu, int4_wait(smem_u32(&full[s]), (b / STAGES) & 1, &abort_flag, status)) != 0;
       if (!ok) break;
       tc_fence_after();
-      const uint64_t desc = smem_desc_sw128(smem_u32(smem + xs * Tile::X_STAGE));
+      const uint64_t desc = smem_desc_sw128(smem_u32(smem + s * Tile::X_STAGE));
       if (elect_one()) {
 #pragma unroll
         for (int q = 0; q < KB / 16; ++q)
           umma_bf16_ts(tmem_sum, tmem_a + s * A_COLS + 8 * q, desc + (uint64_t)(((q >> 2) * (TOK * 128) + (q & 3) * 32) >> 4), idesc, b > 0 || q > 0);
-        umma_commit(smem_u32(&a_empty[s]));
-        umma_commit(smem_u32(&x_empty[xs]));
+        umma_commit(smem_u32(&empty[s]));
         if (b + 1 == blocks) umma_commit(smem_u32(&done));
       }
       __syncwarp();
@@ -371,10 +360,14 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   for (int b0 = turn; b0 < blocks && ok; b0 += DEPTH * TURNS) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const int b = b0 + d * TURNS, s = b % A_STAGES;
+      const int b = b0 + d * TURNS, s = b % STAGES;
       if (b >= blocks || !ok) break;
-      if (b >= A_STAGES) {
-        ok = int4_wait(smem_u32(&a_empty[s]), (b / A_STAGES - 1) & 1, &abort_flag, status);
+      if (b >= STAGES) {
+        // Three stages come to the groups in turn: each waits for the other's block too, so that it has seen every phase of a stage in its
+        // order (a parity alone could stand for the phase before the last).
+        if (STAGES % TURNS != 0 && b > STAGES)
+          ok = __all_sync(0xffffffffu, int4_wait(smem_u32(&empty[(b - 1) % STAGES]), ((b - 1) / STAGES - 1) & 1, &abort_flag, status)) != 0;
+        ok = ok && __all_sync(0xffffffffu, int4_wait(smem_u32(&empty[s]), (b / STAGES - 1) & 1, &abort_flag, status)) != 0;
         if (!ok) break;
         tc_fence_after();                                        // (the MMAs that read the stage)
       }
@@ -392,23 +385,16 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&a_full[s]));
+      if (lane == 0) mbar_arrive(smem_u32(&full[s]));
     }
   }
   // (a barrier of its own: a group of warps that never waited for a stage's earlier phase could take it for the last)
-  if (ok && blocks > 0) ok = int4_wait(smem_u32(&done), 0, &abort_flag, status);
+  if (ok && blocks > 0) ok = __all_sync(0xffffffffu, int4_wait(smem_u32(&done), 0, &abort_flag, status)) != 0;
   tc_fence_after();
   pdl_wait();                                                    // (what this kernel writes may still be read before that)
 
   const uint32_t my_sums = tmem_sum + ((uint32_t)(quarter * 32) << 16) + (warp >> 2) * COLS;
-  auto store = [&](int t, int f, float v) {
-    if (t0 + t >= rows || f0 + f >= n) return;
-    const int64_t at = (int64_t)(t0 + t) * n + f0 + f;
-    if (y_is_f32) reinterpret_cast<float*>(y)[at] = v;
-    else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
-  };
-  float* const part = reinterpret_cast<float*>(smem);            // (every MMA that read the ring is complete)
-  // [TOK][128] sums; 16 columns at a time where there are fewer than 32
+  float* const part = reinterpret_cast<float*>(smem);            // [TOK][128] sums (every MMA that read the ring is complete)
   constexpr int STEP = COLS < 32 ? COLS : 32;
   for (int c0 = 0; c0 < COLS && blocks > 0; c0 += STEP) {
     uint32_t r[32];
@@ -423,20 +409,41 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       tmem_wait_loads();
     }
 #pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      const int t = (warp >> 2) * COLS + c0 + i;
-      if (segments == 1) store(t, feature, __uint_as_float(r[i]));
-      else part[t * FEATURES + feature] = __uint_as_float(r[i]);
-    }
+    for (int i = 0; i < STEP; ++i) part[((warp >> 2) * COLS + c0 + i) * FEATURES + feature] = __uint_as_float(r[i]);
   }
   tc_fence_before();
-  if (segments > 1) {
-    // The roles that bring and issue have ended: every thread of the cluster that is left takes part
+  // Four neighbouring features of a token at a time, so that a warp writes whole rows (each warp its 32 features: 64 bytes a store).
+  const bool quads = n % 4 == 0 && (uintptr_t)y % 16 == 0;
+  auto store = [&](int t, int f, const float4& v) {
+    if (f0 + f >= n) return;
+    const int64_t at = (int64_t)(t0 + t) * n + f0 + f;
+    if (quads) {
+      if (y_is_f32) store_four(reinterpret_cast<float*>(y) + at, v);
+      else store_four(reinterpret_cast<bf16*>(y) + at, v);
+      return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (f0 + f + i >= n) return;
+      if (y_is_f32) reinterpret_cast<float*>(y)[at + i] = e[i];
+      else reinterpret_cast<bf16*>(y)[at + i] = __float2bfloat16_rn(e[i]);
+    }
+  };
+  if (segments == 1) {
+    int4_workers_sync<WORKERS>();
+    const int count = min(TOK, rows - t0);
+    for (int word = threadIdx.x; word < count * (FEATURES / 4); word += WORKERS) {
+      const int t = word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
+      store(t, f, *reinterpret_cast<const float4*>(part + t * FEATURES + f));
+    }
+  } else {
+    // the segments' sums in their order, each CTA a share of the tokens (the roles that bring and issue have ended: every thread of the cluster
+    // that is left takes part)
     cluster_sync_all();
-    const int lo = TOK * segment / segments, hi = TOK * (segment + 1) / segments;
+    const int lo = TOK * segment / segments, hi = min(TOK * (segment + 1) / segments, rows - t0);
     for (int word = threadIdx.x; word < (hi - lo) * (FEATURES / 4); word += WORKERS) {
       const int t = lo + word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
-      if (t0 + t >= rows) break;
       const uint32_t at = smem_u32(&part[t * FEATURES + f]);
       // (all of them on their way at once: one after the other, eight took 4 us)
       float4 u[MAX_SEGMENTS];
@@ -452,10 +459,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
           v.z += u[r].z;
           v.w += u[r].w;
         }
-      store(t, f, v.x);
-      store(t, f + 1, v.y);
-      store(t, f + 2, v.z);
-      store(t, f + 3, v.w);
+      store(t, f, v);
     }
     cluster_sync_all();                                          // nobody reads this CTA's sums after this
   }
@@ -470,10 +474,11 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   }
 }
 
-// Segments of k: as many as still find an SM, each of four blocks at least.
+// Segments of k: as many as still find an SM at once, each of eight blocks at least, of four where few CTAs are at work. us at 1, 2, 4 and 8: 64
+// tokens, 4,096 x 4,096 16.9, 12.4, 10.2 and 11.5, 4,096 x 12,288 42, 25, 19.6 and 16.7, 24,576 x 4,096 28, 31, 37 and 61, 128 x 4,096 15.9, 11.5, 8.0 and 6.9.
 int int4_segments(int64_t ctas, int deep, int at_once) {
   int s = 1;
-  while (s < MAX_SEGMENTS && ctas * s * 2 <= at_once && deep >= 8 * s) s *= 2;
+  while (s < MAX_SEGMENTS && ctas * s * 2 <= at_once && deep >= (ctas * s * 2 <= 64 ? 8 : 16) * s) s *= 2;
   return s;
 }
 
