@@ -730,6 +730,9 @@ def main() -> int:
                         help="read every step's tokens before the next step is planned (default: the engine's async scheduling)")
     parser.add_argument("--batch-invariant", default="off", choices=["off", "decode", "full"],
                         help="measure with the engine's bitwise-invariance modes (the default run has them off)")
+    parser.add_argument("--cache-dtype", default=None, choices=["e4m3"], help="keys and values in 8 bits (the default run has them in bfloat16)")
+    parser.add_argument("--weights", default=None, choices=["int4"], help="the layers' matrices in 4 bits (the default run has them in bfloat16)")
+    parser.add_argument("--weight-group", type=int, default=128, choices=[32, 64, 128], help="inputs that share a scale")
     parser.add_argument("--design", default="", choices=["", "mugizen", "vivesun", "beralix", "nefipel", "pubulix", "difavik"],
                         help="measure this design beside the engine's closest other model at equal layer sizes instead of the headline")
     parser.add_argument("--design-sizes", default="s,m,moe", help="which of the sizes s, m, moe (comma-separated)")
@@ -778,12 +781,17 @@ def main() -> int:
     shape = {"model": name, "layers": L, "layers_full": layers_full, "hidden": H, "heads": nq, "kv_heads": nkv,
              "head_dim": d, "intermediate": I, "vocab": V}
 
+    few_bits = {k: v for k, v in dict(cache_dtype=args.cache_dtype, weights=args.weights).items() if v}
+    if args.weights:
+        few_bits["weight_group"] = args.weight_group
+    shape.update(few_bits)
+
     if args.workload == "mixed":
         num_blocks = 32 * ((3072 + 512 + PAGE) // PAGE) + 8
         engine = Engine(spec=spec, tensors=tensors, dtype="bfloat16", device="cuda:0", num_blocks=num_blocks,
                         block_size=PAGE, max_num_seqs=32, max_num_batched_tokens=4096, enable_prefix_caching=True,
                         cuda_graphs=not args.no_cuda_graphs, batch_invariant=args.batch_invariant,
-                        async_scheduling=not args.sync_scheduling, consume_tensors=True)
+                        async_scheduling=not args.sync_scheduling, consume_tensors=True, **few_bits)
         del tensors
         torch.cuda.empty_cache()
         mixed_run(engine, config, seed=4, requests=4)            # warm the kernels and the graphs' first shapes
@@ -813,11 +821,11 @@ def main() -> int:
                     block_size=PAGE, max_num_seqs=max_batch, max_num_batched_tokens=2 * CONTEXT,
                     enable_prefix_caching=False, cuda_graphs=not args.no_cuda_graphs,
                     batch_invariant=args.batch_invariant, async_scheduling=not args.sync_scheduling,
-                    consume_tensors=True)
+                    consume_tensors=True, **few_bits)
     del tensors
     torch.cuda.empty_cache()
     weight_bytes = engine.runner.model.weight_bytes()
-    assert abs(weight_bytes - closed_form_weight_bytes(config)) <= 0.002 * weight_bytes, \
+    assert args.weights or abs(weight_bytes - closed_form_weight_bytes(config)) <= 0.002 * weight_bytes, \
         (weight_bytes, closed_form_weight_bytes(config))
     kv_bytes_per_token = engine.runner.cache.bytes_per_token()
 

@@ -94,7 +94,7 @@ template <int D>
 __global__ void __launch_bounds__(THREADS, RESIDENT)
 attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const CacheArgs c, const int* __restrict__ token_list,
                       const int* __restrict__ positions, const int* __restrict__ request_of, int nq, int nkv, float scale_log2, int window,
-                      int segments, int ordered, int beside, unsigned* status) {
+                      int segments, int ordered, int beside, int appended, unsigned* status) {
   constexpr int CHUNKS = D / 64, FT = D / 16;
   constexpr int RAISED = 15;
   // a warp's buffers: four blocks of keys, and four of values whose starts lie 32 bytes apart in the banks (lanes read all four at once)
@@ -187,7 +187,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   };
   // A wait that runs out is reported, and the warp stops; before, it waits once more for what it has in flight (`other`: the other side too).
   auto arrived = [&](int side, uint32_t parity, bool other, uint32_t other_parity) {
-    const bool ok = mb_wait(bar[side], parity, status);
+    const bool ok = mb_try_wait(bar[side], parity) || mb_wait(bar[side], parity, status);    // (asked once before the clock is read)
     if (__all_sync(0xffffffffu, ok)) return true;
     (void)mb_wait(bar[side], parity, status);
     if (other) (void)mb_wait(bar[side ^ 1], other_parity, status);
@@ -198,13 +198,18 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   // writes, and waited for everything before it in all of its CTAs before it let this one start. It is waited for at the end only
   // (the chain of completed kernels stays unbroken).
   int64_t next = block_of(begin + warp);
-  if (!beside) pdl_wait();
-  pdl_launch_dependents();
-  if (begin + warp < end) {
+  auto start = [&] {
     request(0, next);
     request(1, next);
     load_scales(next);
-  }
+  };
+  // `appended` > 0: the kernel before this one writes, of what is read here, the blocks of the requests' newest `appended` tokens and nothing
+  // else; a first tile before them is asked for at once (it is aligned to blocks).
+  const bool early = appended > 0 && begin + warp < end && (begin + warp + 1) * TILE <= pos - appended + 1;
+  if (early) start();
+  if (!beside) pdl_wait();
+  pdl_launch_dependents();
+  if (!early && begin + warp < end) start();
   uint32_t qb[CHUNKS][4][2];                                   // Q^T: [chunk][k-step][features 4 w, + 2]
   float q_scale[2];                                            // what heads 2 j and 2 j + 1 were divided by, times scale_log2
   {
@@ -623,7 +628,7 @@ struct Launch {
   CacheArgs c;
   const int *token_list, *positions, *request_of;
   int64_t items;
-  int nq, nkv, window, segments, ordered, beside;
+  int nq, nkv, window, segments, ordered, beside, appended;
   float scale_log2;
   unsigned* status;
   cudaStream_t stream;
@@ -640,9 +645,9 @@ cudaError_t launch_e4m3(const Launch& a) {
   const dim3 grid((unsigned)(a.items * segments));
   if (segments == 1)
     return vosti_launch(kernel, grid, dim3(THREADS), SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,
-                        a.window, 1, a.ordered, a.beside, a.status);
+                        a.window, 1, a.ordered, a.beside, a.appended, a.status);
   return vosti_launch_clusters(kernel, grid, dim3(THREADS), (unsigned)segments, SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of,
-                               a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.beside, a.status);
+                               a.nq, a.nkv, a.scale_log2, a.window, segments, a.ordered, a.beside, a.appended, a.status);
 }
 int check_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, const int* block_table, int max_pages, int page_size,
                 int num_pages, int nq, int nkv, float scale, int window) {
@@ -658,14 +663,17 @@ int check_cache(const void* k, const void* v, const void* k_scale, const void* v
 }  // namespace
 
 // q, out: bfloat16 [tokens, nq * d]; the cache as in e4m3.cuh. `token_list` (or null: 0 .. count - 1) names the tokens; d is 64 or 128. `beside`: the
-// launch right before this one on the stream is vosti_attention_prefill_tc_e4m3 for other rows of the same q, out and cache.
+// launch right before this one on the stream is vosti_attention_prefill_tc_e4m3 for other rows of the same q, out and cache. `appended`
+// > 0: the launch before (before the one it is beside) is the step's store of keys and values, which wrote at most that many of each request's newest tokens;
+// 0: nothing is known of it.
 VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, void* out,
                                    const int* token_list, int count, const int* positions, const int* request_of, const int* block_table,
                                    int max_pages, int page_size, int num_pages, int nq, int nkv, int d, int max_kv_len, float scale, int window,
-                                   int beside, unsigned* status, cudaStream_t stream) {
+                                   int beside, int appended, unsigned* status, cudaStream_t stream) {
   if (int bad = check_cache(k, v, k_scale, v_scale, block_table, max_pages, page_size, num_pages, nq, nkv, scale, window)) return bad;
   VOSTI_REQUIRE(d == 64 || d == 128, "attention_e4m3: head_dim %d must be 64 or 128", d);
   VOSTI_REQUIRE((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "attention_e4m3: queries must start on 16 bytes");
+  VOSTI_REQUIRE(appended >= 0, "attention_e4m3: bad count of appended tokens");
   VOSTI_REQUIRE(count >= 0 && (int64_t)count * nq * MAX_SEGMENTS <= 0x7fffffff, "attention_e4m3: bad token count %d", count);
   if (count == 0) return VOSTI_OK;
   const CacheArgs c = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, max_pages, page_size, num_pages};
@@ -673,7 +681,7 @@ VOSTI_API int vosti_attention_e4m3(const void* q, const void* k, const void* v, 
   // more CTAs than run at once: those of the tokens with most keys first
   const bool ordered = items > 148 * RESIDENT && count > 1 && count <= MAX_ORDERED;
   const Launch launch = {(const bf16*)q, (bf16*)out, c, token_list, positions, request_of, items, nq, nkv, window, segments_of(items, max_kv_len),
-                         ordered ? count : 0, beside, scale * LOG2E, status, stream};
+                         ordered ? count : 0, beside, appended, scale * LOG2E, status, stream};
   const cudaError_t e = d == 64 ? launch_e4m3<64>(launch) : launch_e4m3<128>(launch);
   if (e != cudaSuccess) {
     vosti_set_error("attention_e4m3: %s", cudaGetErrorString(e));

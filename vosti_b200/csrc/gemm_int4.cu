@@ -143,7 +143,7 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
     const int st = at / DEEP, inside = at % DEEP;
     if (inside == 0) {
       const uint32_t bar = smem_addr(&full[warp][st % FEW_STAGES]);
-      if (!__all_sync(0xffffffffu, mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status))) {
+      if (!__all_sync(0xffffffffu, mb_try_wait(bar, (uint32_t)(st / FEW_STAGES) & 1) || mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status))) {
         // reported; once more, so that none of the warp's copies is in flight when it ends
         (void)mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status);
         if (st + 1 < stages) (void)mb_wait(smem_addr(&full[warp][(st + 1) % FEW_STAGES]), (uint32_t)((st + 1) / FEW_STAGES) & 1, status);

@@ -25,7 +25,7 @@ constexpr int SHORT = 4;                       // tokens of a run that one warp 
 constexpr int V_PITCH = 20;                    // bytes between a feature's rows of values in shared memory (banks apart)
 constexpr int FEW = 64;                        // up to so many tokens: one a CTA
 constexpr int TILE = 8;                        // neighbouring tokens whose runs a CTA takes, with more
-constexpr int Q_ITEMS = 4;                     // query heads that a lane holds at a time
+constexpr int Q_MANY = 4;                      // query heads that a lane holds at a time, with more (up to that, one)
 
 struct PostArgs {
   const void* qkv;               // [tokens, (nq + 2 nkv) d], or null with
@@ -71,49 +71,75 @@ __device__ __forceinline__ void load_words(const T* p, float (&x)[4]) {
   x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
 
-// A head of the projection (or of its partial sums, added in split order) that begins at element `at`.
-template <typename T, typename L>
-__device__ __forceinline__ void load_head(const PostArgs& a, int64_t at, int sub, float (&x)[L::PAIRS], float (&y)[L::PAIRS]) {
+// N heads of the projection that begin at elements at[i], or the sums of their partial sums in split order; those without `live` are zeros. The loads
+// of all of them, and of FLIGHT splits, are on their way together.
+template <typename T, typename L, int N>
+__device__ __forceinline__ void load_heads(const PostArgs& a, const int64_t (&at)[N], const bool (&live)[N], int sub, float (&x)[N][L::PAIRS],
+                                           float (&y)[N][L::PAIRS]) {
   const int half = a.d >> 1;
-  if constexpr (L::FAST) {
-    const int64_t i = at + 4 * sub;
-    if (a.partial == nullptr) {
-      load_words(reinterpret_cast<const T*>(a.qkv) + i, x);
-      load_words(reinterpret_cast<const T*>(a.qkv) + i + half, y);
-      return;
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = y[j] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
-      float u[4], v[4];
-      load_words(a.partial + s * a.plane + i, u);
-      load_words(a.partial + s * a.plane + i + half, v);
+  for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] += u[j];
-        y[j] += v[j];
+    for (int j = 0; j < L::PAIRS; ++j) x[i][j] = y[i][j] = 0.f;
+  if (a.partial == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!live[i]) continue;
+      const T* const from = reinterpret_cast<const T*>(a.qkv) + at[i];
+      if constexpr (L::FAST) {
+        load_words(from + 4 * sub, x[i]);
+        load_words(from + 4 * sub + half, y[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < L::PAIRS; ++j) {
+          const int p = L::pair(sub, j);
+          if (p >= half) continue;
+          int ia, ib;
+          L::elements(p, a, ia, ib);
+          x[i][j] = to_f32(from[ia]);
+          y[i][j] = to_f32(from[ib]);
+        }
       }
     }
-  } else {
+    return;
+  }
+  constexpr int FLIGHT = !L::FAST || N > 2 ? 1 : N == 2 ? 4 : 8;
+  for (int s0 = 0; s0 < a.splits; s0 += FLIGHT) {
+    float u[FLIGHT][N][L::PAIRS], v[FLIGHT][N][L::PAIRS];
 #pragma unroll
-    for (int j = 0; j < L::PAIRS; ++j) {
-      const int p = L::pair(sub, j);
-      x[j] = y[j] = 0.f;
-      if (p >= half) continue;
-      int ia, ib;
-      L::elements(p, a, ia, ib);
-      if (a.partial == nullptr) {
-        x[j] = to_f32(reinterpret_cast<const T*>(a.qkv)[at + ia]);
-        y[j] = to_f32(reinterpret_cast<const T*>(a.qkv)[at + ib]);
-        continue;
+    for (int f = 0; f < FLIGHT; ++f)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool here = live[i] && s0 + f < a.splits;
+        const float* const from = a.partial + (s0 + f) * a.plane + at[i];
+        if constexpr (L::FAST) {
+          if (here) {
+            load_words(from + 4 * sub, u[f][i]);
+            load_words(from + 4 * sub + half, v[f][i]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < L::PAIRS; ++j) u[f][i][j] = v[f][i][j] = 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < L::PAIRS; ++j) {
+            const int p = L::pair(sub, j);
+            int ia, ib;
+            L::elements(p, a, ia, ib);
+            u[f][i][j] = here && p < half ? from[ia] : 0.f;
+            v[f][i][j] = here && p < half ? from[ib] : 0.f;
+          }
+        }
       }
-#pragma unroll 4
-      for (int s = 0; s < a.splits; ++s) {
-        x[j] += a.partial[s * a.plane + at + ia];
-        y[j] += a.partial[s * a.plane + at + ib];
-      }
-    }
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < L::PAIRS; ++j) {
+          x[i][j] += u[f][i][j];
+          y[i][j] += v[f][i][j];
+        }
   }
 }
 
@@ -269,12 +295,13 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
     const int r = me + i * STEP;
+    const int64_t key = ((int64_t)(t0 + r) * heads + a.nq + g) * a.d;
+    const int64_t at[2] = {key, key + (int64_t)a.nkv * a.d};
+    const bool live[2] = {r < n, r < n};
+    float x[2][L::PAIRS], y[2][L::PAIRS];
+    load_heads<T, L, 2>(a, at, live, sub, x, y);
 #pragma unroll
-    for (int j = 0; j < L::PAIRS; ++j) kx[i][j] = ky[i][j] = vx[i][j] = vy[i][j] = 0.f;
-    if (r >= n) continue;
-    const int64_t at = ((int64_t)(t0 + r) * heads + a.nq + g) * a.d;
-    load_head<T, L>(a, at, sub, kx[i], ky[i]);
-    load_head<T, L>(a, at + (int64_t)a.nkv * a.d, sub, vx[i], vy[i]);
+    for (int j = 0; j < L::PAIRS; ++j) kx[i][j] = x[0][j], ky[i][j] = y[0][j], vx[i][j] = x[1][j], vy[i][j] = y[1][j];
   }
   const int k_old = offset > 0 ? a.k_scale[block] : 0, v_old = offset > 0 ? a.v_scale[block] : 0;
   float most[2] = {0.f, 0.f};
@@ -378,8 +405,8 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
 }
 
 // Blocks: `tile` neighbouring tokens' keys and values of a kv head, then query heads, WARPS * HEADS * Q_ITEMS of them.
-template <typename T, typename L>
-__global__ void __launch_bounds__(THREADS, L::LANES * L::PAIRS <= 64 ? 6 : 4) qkv_post_e4m3_kernel(const PostArgs a) {
+template <typename T, typename L, int Q_ITEMS>
+__global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <= 64 ? 6 : 4) qkv_post_e4m3_kernel(const PostArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L::LANES;
   const int kv_blocks = (a.tokens + a.tile - 1) / a.tile * a.nkv;
 
@@ -396,15 +423,20 @@ __global__ void __launch_bounds__(THREADS, L::LANES * L::PAIRS <= 64 ? 6 : 4) qk
     if (chunk >= a.tokens * of_token) return;
     float x[Q_ITEMS][L::PAIRS], y[Q_ITEMS][L::PAIRS], c[L::PAIRS], s[L::PAIRS];
     const int64_t in = (int64_t)t * (a.nq + 2 * a.nkv) * a.d, out = (int64_t)t * a.nq * a.d;
+    int64_t at[Q_ITEMS];
+    bool live[Q_ITEMS];
 #pragma unroll
-    for (int i = 0; i < Q_ITEMS; ++i)                            // (beyond the last head: the last one again, not stored)
-      load_head<T, L>(a, in + (int64_t)min(h0 + i * L::HEADS, a.nq - 1) * a.d, sub, x[i], y[i]);
+    for (int i = 0; i < Q_ITEMS; ++i) {
+      live[i] = h0 + i * L::HEADS < a.nq;
+      at[i] = in + (int64_t)(h0 + i * L::HEADS) * a.d;
+    }
+    load_heads<T, L, Q_ITEMS>(a, at, live, sub, x, y);
     load_turn<L>(a, pos, sub, c, s);                             // (behind the heads: the position has arrived by now)
 #pragma unroll
     for (int i = 0; i < Q_ITEMS; ++i) norm_and_turn<L>(a, a.q_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
 #pragma unroll
     for (int i = 0; i < Q_ITEMS; ++i)
-      if (h0 + i * L::HEADS < a.nq) store_head<T, L>(a, reinterpret_cast<T*>(a.q_out) + out + (int64_t)(h0 + i * L::HEADS) * a.d, sub, x[i], y[i]);
+      if (live[i]) store_head<T, L>(a, reinterpret_cast<T*>(a.q_out) + out + (int64_t)(h0 + i * L::HEADS) * a.d, sub, x[i], y[i]);
     return;
   }
 
@@ -438,12 +470,16 @@ __global__ void __launch_bounds__(THREADS, L::LANES * L::PAIRS <= 64 ? 6 : 4) qk
     if (i % WARPS == warp) store_run<T, L, false>(a, t_begin + __ffs(short_runs) - 1, g, rows_of_values + warp * a.d * V_PITCH, nullptr, wx, wy);
 }
 
-template <typename T, typename L>
-cudaError_t launch_post(const PostArgs& a, cudaStream_t stream) {
+template <typename T, typename L, int Q_ITEMS>
+cudaError_t launch_post_items(const PostArgs& a, cudaStream_t stream) {
   constexpr int CHUNK = L::HEADS * Q_ITEMS;
   const int64_t q_blocks = ((int64_t)a.tokens * ((a.nq + CHUNK - 1) / CHUNK) + WARPS - 1) / WARPS;
   const int64_t blocks = (int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv + q_blocks;
-  return vosti_launch(qkv_post_e4m3_kernel<T, L>, dim3((unsigned)blocks), dim3(THREADS), (size_t)WARPS * a.d * V_PITCH, stream, a);
+  return vosti_launch(qkv_post_e4m3_kernel<T, L, Q_ITEMS>, dim3((unsigned)blocks), dim3(THREADS), (size_t)WARPS * a.d * V_PITCH, stream, a);
+}
+template <typename T, typename L>
+cudaError_t launch_post(const PostArgs& a, cudaStream_t stream) {
+  return a.tokens <= FEW ? launch_post_items<T, L, 1>(a, stream) : launch_post_items<T, L, Q_MANY>(a, stream);
 }
 template <typename T>
 cudaError_t launch_post_as(const PostArgs& a, cudaStream_t stream) {

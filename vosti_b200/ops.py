@@ -2427,10 +2427,13 @@ def qkv_post_e4m3(qkv, cache: PagedE4M3, *, nq: int, nkv: int, head_dim: int, sl
     return q_out
 
 
-def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nkv: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
+def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nkv: int, head_dim: int, scale: float, window: int = 0,
+                   appended: int = 0) -> torch.Tensor:
     """`attention` over a cache of 8 bits: every query row of the step over its request's keys, causal, the last `window` of them if
     that is not 0. bfloat16 with heads of 64 or 128: single tokens on a kernel that cuts the keys into segments, portions on the tcgen05 kernel;
-    everything else on the CUDA cores in float32."""
+    everything else on the CUDA cores in float32. `appended` > 0 says that the kernel launched right before is the step's own
+    `qkv_post_e4m3`, which stored at most that many of each request's newest tokens: what lies before them is then read
+    while it still runs. 0: nothing is known of it."""
     tokens = q.shape[0]
     if q.dim() != 2 or q.shape[1] != nq * head_dim or q.dtype not in (torch.bfloat16, torch.float32):
         raise KernelError("attention_e4m3: the queries are bfloat16 or float32 [tokens, nq * d]")
@@ -2439,8 +2442,8 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
     table, status = group.block_table, ctx.status
     if table.dim() != 2 or table.dtype != torch.int32:
         raise KernelError("attention_e4m3: the block table is int32 [requests, pages]")
-    if window < 0 or not scale > 0:
-        raise KernelError("attention_e4m3: the score scale must be positive and the window not negative")
+    if window < 0 or appended < 0 or not scale > 0:
+        raise KernelError("attention_e4m3: the score scale must be positive, the window and the appended tokens not negative")
     _ints("attention_e4m3", tokens, positions=ctx.positions, request_of=ctx.request_of)
     stream = _here("attention_e4m3", q, cache.k, ctx.positions, ctx.request_of, table, status)
     out = torch.empty_like(q)
@@ -2466,9 +2469,9 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
         # (beside the portions' kernel, whose last CTAs leave SMs free)
         if short is not None:
             _here("attention_e4m3", short)
-        _check(_bound("vosti_attention_e4m3", "pppppp" "pipp" "piiiiii" "ifiipp")(
+        _check(_bound("vosti_attention_e4m3", "pppppp" "pipp" "piiiiii" "ifiiipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(short), count, ctx.positions.data_ptr(), ctx.request_of.data_ptr(), *geometry,
-            ctx.max_kv_len, scale, window, long_rows > 0, status.data_ptr(), stream), "attention_e4m3")
+            ctx.max_kv_len, scale, window, long_rows > 0, appended, status.data_ptr(), stream), "attention_e4m3")
     return out
 
 

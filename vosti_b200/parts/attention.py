@@ -107,7 +107,7 @@ class Attention(Mixer):
             if self.eight_bits:
                 common.pop("page_size")
                 q = ops.qkv_post_e4m3(qkv, cache.e4m3, nkv=self.nkv, k_norm_w=self.k_norm, slot_mapping=group.slot_mapping, **common)
-                return self._out(ctx, q, cache, group)
+                return self._out(ctx, q, cache, group, appended=ctx.max_q_len)
             if (ops.DECODE_FUSION and isinstance(qkv, ops.PartialSum) and qkv.dtype == torch.bfloat16
                     and ctx.layout["attention"]["num_short_tokens"] == ctx.num_tokens == ctx.num_requests
                     and self.nq // self.nkv <= 16 and cache.k.dtype == torch.bfloat16
@@ -132,11 +132,11 @@ class Attention(Mixer):
                              k_norm_w=self.k_norm, slot_mapping=None, **common)
         return self._out(ctx, q, cache, group)
 
-    def _out(self, ctx, q, cache, group):
-        """Attention of the rotated queries and the output projection."""
+    def _out(self, ctx, q, cache, group, appended: int = 0):
+        """Attention of the rotated queries and the output projection (`appended`: see ops.attention_e4m3)."""
         sizes = dict(nq=self.nq, nkv=self.nkv, head_dim=self.d, scale=self.scale, window=self.window)
         if self.eight_bits:
-            attn = ops.attention_e4m3(ctx, q, cache.e4m3, group, **sizes)
+            attn = ops.attention_e4m3(ctx, q, cache.e4m3, group, appended=appended, **sizes)
         else:
             attn = ops.attention(ctx, q, cache.k, cache.v, group, **sizes)
         return linear(ctx, attn, self.w_o, allow_partial=True, bias=self.b_o)   # summed by the norm that follows
