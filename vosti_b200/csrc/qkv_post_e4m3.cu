@@ -5,16 +5,17 @@
 // Norm and rotation are qkv_post.cu's (kernels/triton_kernels/qk_norm.py:40-95, rope.py:78-101); everything is float32 up to
 // the one rounding at the store.
 //
-// A scale belongs to a block, so the unit of work for keys and values is a run: the step's tokens of one block and kv head, which stand
-// next to one another in the batch and in the block. A CTA (runs of more than four tokens) or a warp (shorter ones) takes a run: it holds
-// the run's keys and values in registers, finds their largest size, takes the larger of what they need and (a block that holds earlier
+// A scale belongs to a block, so the unit of work for keys, and for values, is a run: the step's tokens of one block and kv head, which stand
+// next to one another in the batch and in the block. A CTA (runs of more than four tokens) or a warp (shorter ones) takes a run's keys, another its
+// values: it holds them in registers, finds their largest size, takes the larger of what they need and (a block that holds earlier
 // tokens) the scale that is there, rounds the earlier tokens again where the scale grew, and stores. Nothing of another run's is read.
 // A value that is not finite, or not below 2^96, makes its block's scale 255: the block is no number from then on.
 //
 // A head of 64, 128 or 256 that turns as a whole in pairs (i, i + d/2), or not at all, is d / 8 lanes with four neighbouring elements of each half;
-// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 21.6 us, a third of what its bytes need: blocks are
-// short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (blocks that walked on over query
-// heads were slower: 22.1 us with six an SM, 27 with three; a head on a whole warp 22.4 with half as many instructions again).
+// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 17 to 19 us, 40% of the rate its bytes could move at: blocks
+// are short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (20 warps with more registers, blocks that walked on over query
+// heads, and a head on a whole warp were slower). Eight tokens take 3 us, which is a launch and three loads that wait for one another; a CTA
+// that took a run's keys and values both needed 5.3.
 #include "common.cuh"
 #include "e4m3.cuh"
 
@@ -23,9 +24,8 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int SHORT = 4;                       // tokens of a run that one warp takes
 constexpr int V_PITCH = 20;                    // bytes between a feature's rows of values in shared memory (banks apart)
-constexpr int FEW = 64;                        // up to so many tokens: one a CTA
-constexpr int TILE = 8;                        // neighbouring tokens whose runs a CTA takes, with more
-constexpr int Q_MANY = 4;                      // query heads that a lane holds at a time, with more (up to that, one)
+constexpr int FEW = 32, MANY = 256;
+constexpr int Q_MANY = 4;                      // query heads that a lane holds at a time with more than FEW tokens (up to that, one)
 
 struct PostArgs {
   const void* qkv;               // [tokens, (nq + 2 nkv) d], or null with
@@ -266,13 +266,10 @@ __device__ __forceinline__ float larger(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
   return r;
 }
-struct RunStats {                 // of a CTA's warps: largest sizes of keys and values
-  float most[2][WARPS];
-};
-
-// One run: the tokens from t0 on of kv head g, by the whole CTA or by one warp (`v_rows`: [d][V_PITCH] of its own).
-template <typename T, typename L, bool WHOLE>
-__device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint8_t* v_rows, RunStats* shared, const float (&wx)[L::PAIRS], const float (&wy)[L::PAIRS]) {
+// One run's keys (or VALUES): the tokens from t0 on of kv head g, by the whole CTA or by one warp. `rows`: [d][V_PITCH] of its own,
+// `most_of`: a CTA's warps' largest sizes.
+template <typename T, typename L, bool WHOLE, bool VALUES>
+__device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint8_t* rows, float* most_of, const float (&wx)[L::PAIRS], const float (&wy)[L::PAIRS]) {
   constexpr int STEP = (WHOLE ? WARPS : 1) * L::HEADS, ROUNDS = ((WHOLE ? E4M3_BLOCK : SHORT) + STEP - 1) / STEP;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L::LANES;
   const int me = (WHOLE ? warp * L::HEADS : 0) + lane / L::LANES, thread = WHOLE ? threadIdx.x : lane, threads = WHOLE ? THREADS : 32;
@@ -283,132 +280,134 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
   const int n = __ffs(gone) - 1;
   const int64_t page = slot / a.page_size, in_page = slot % a.page_size;
   const int64_t block = (page * a.nkv + g) * (a.page_size / E4M3_BLOCK) + in_page / E4M3_BLOCK;
-  auto sync = [] {
-    if constexpr (WHOLE) __syncthreads();
-    else __syncwarp();
-  };
 
   int pos[ROUNDS];
+  if (!VALUES) {
 #pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) pos[i] = position_of(a, t0 + min(me + i * STEP, n - 1));
-  float kx[ROUNDS][L::PAIRS], ky[ROUNDS][L::PAIRS], vx[ROUNDS][L::PAIRS], vy[ROUNDS][L::PAIRS];
+    for (int i = 0; i < ROUNDS; ++i) pos[i] = position_of(a, t0 + min(me + i * STEP, n - 1));
+  }
+  float x[ROUNDS][L::PAIRS], y[ROUNDS][L::PAIRS];
+  int64_t at[ROUNDS];
+  bool live[ROUNDS];
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
     const int r = me + i * STEP;
-    const int64_t key = ((int64_t)(t0 + r) * heads + a.nq + g) * a.d;
-    const int64_t at[2] = {key, key + (int64_t)a.nkv * a.d};
-    const bool live[2] = {r < n, r < n};
-    float x[2][L::PAIRS], y[2][L::PAIRS];
-    load_heads<T, L, 2>(a, at, live, sub, x, y);
-#pragma unroll
-    for (int j = 0; j < L::PAIRS; ++j) kx[i][j] = x[0][j], ky[i][j] = y[0][j], vx[i][j] = x[1][j], vy[i][j] = y[1][j];
+    live[i] = r < n;
+    at[i] = ((int64_t)(t0 + r) * heads + a.nq + (VALUES ? a.nkv : 0) + g) * a.d;
   }
-  const int k_old = offset > 0 ? a.k_scale[block] : 0, v_old = offset > 0 ? a.v_scale[block] : 0;
-  float most[2] = {0.f, 0.f};
+  load_heads<T, L, ROUNDS>(a, at, live, sub, x, y);              // (zeros beyond the run)
+  uint8_t* const scale = (VALUES ? a.v_scale : a.k_scale) + block;
+  const int old = offset > 0 ? *scale : 0;
+  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
     if (i * STEP >= n) break;                                    // (the same in all lanes)
-    float c[L::PAIRS], s[L::PAIRS];
-    load_turn<L>(a, pos[i], sub, c, s);
-    norm_and_turn<L>(a, a.k_norm_w != nullptr, kx[i], ky[i], wx, wy, c, s);      // (zeros beyond the run stay zeros)
-#pragma unroll
-    for (int j = 0; j < L::PAIRS; ++j) {
-      most[0] = larger(larger(most[0], kx[i][j]), ky[i][j]);
-      most[1] = larger(larger(most[1], vx[i][j]), vy[i][j]);
+    if (!VALUES) {
+      float c[L::PAIRS], s[L::PAIRS];
+      load_turn<L>(a, pos[i], sub, c, s);
+      norm_and_turn<L>(a, a.k_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
     }
+#pragma unroll
+    for (int j = 0; j < L::PAIRS; ++j) most = larger(larger(most, x[i][j]), y[i][j]);
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most[i] = larger(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+  for (int o = 16; o > 0; o >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, o));
   if constexpr (WHOLE) {
-    if (lane == 0) {
-      shared->most[0][warp] = most[0];
-      shared->most[1][warp] = most[1];
-    }
+    if (lane == 0) most_of[warp] = most;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) most[i] = larger(most[i], shared->most[i][w]);
+    for (int w = 0; w < WARPS; ++w) most = larger(most, most_of[w]);
   }
-  const int k_new = !(most[0] < E4M3_LIMIT) ? E4M3_NAN_SCALE : max(e4m3_scale_for(most[0]), k_old);
-  const int v_new = !(most[1] < E4M3_LIMIT) ? E4M3_NAN_SCALE : max(e4m3_scale_for(most[1]), v_old);
+  const int now = !(most < E4M3_LIMIT) ? E4M3_NAN_SCALE : max(e4m3_scale_for(most), old);
   // 2^-(scale - 127): the bits 254 - scale as an exponent (a scale that is no number: any payload will do)
-  const float k_times = __uint_as_float((uint32_t)max(254 - k_new, 1) << 23), v_times = __uint_as_float((uint32_t)max(254 - v_new, 1) << 23);
-  uint8_t* const k_rows = a.k + block * E4M3_BLOCK * a.d;
-  uint8_t* const v_block = a.v + block * E4M3_BLOCK * a.d;
-  // earlier keys under a larger scale, in whole words (beyond 2^-127 everything is zero)
-  if (offset > 0 && k_new > k_old && k_new != E4M3_NAN_SCALE) {
-    const float f = e4m3_scale(max(127 + k_old - k_new, 0));
-    for (int i = thread; i < offset * a.d / 4; i += threads) {
-      uint32_t* const word = reinterpret_cast<uint32_t*>(k_rows) + i;
-      *word = e4m3_again(*word, f);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    const int r = me + i * STEP;
-    if (r >= n) continue;
-    uint8_t* const key = k_rows + (offset + r) * a.d;
-    uint8_t* const column = v_rows + offset + r;                 // a token's place in every feature's row
-    if constexpr (L::FAST) {
-      *reinterpret_cast<uint32_t*>(key + 4 * sub) = e4m3_pack4(kx[i][0] * k_times, kx[i][1] * k_times, kx[i][2] * k_times, kx[i][3] * k_times);
-      *reinterpret_cast<uint32_t*>(key + 4 * sub + half) = e4m3_pack4(ky[i][0] * k_times, ky[i][1] * k_times, ky[i][2] * k_times, ky[i][3] * k_times);
-    }
-#pragma unroll
-    for (int j = 0; j < L::PAIRS; ++j) {
-      const int p = L::pair(sub, j);
-      if (p >= half) continue;
-      int ia, ib;
-      L::elements(p, a, ia, ib);
-      const uint16_t vv = e4m3_pack(vx[i][j] * v_times, vy[i][j] * v_times);
-      column[ia * V_PITCH] = (uint8_t)vv;
-      column[ib * V_PITCH] = (uint8_t)(vv >> 8);
-      if constexpr (!L::FAST) {
-        const uint16_t kk = e4m3_pack(kx[i][j] * k_times, ky[i][j] * k_times);
-        key[ia] = (uint8_t)kk;
-        key[ib] = (uint8_t)(kk >> 8);
+  const float times = __uint_as_float((uint32_t)max(254 - now, 1) << 23);
+  uint8_t* const payloads = (VALUES ? a.v : a.k) + block * E4M3_BLOCK * a.d;
+  // earlier tokens under a larger scale (beyond 2^-127 everything is zero)
+  const bool regrow = offset > 0 && now > old && now != E4M3_NAN_SCALE;
+  const float f = regrow ? e4m3_scale(max(127 + old - now, 0)) : 1.f;
+
+  if constexpr (!VALUES) {
+    if (regrow)
+      for (int i = thread; i < offset * a.d / 4; i += threads) {
+        uint32_t* const word = reinterpret_cast<uint32_t*>(payloads) + i;
+        *word = e4m3_again(*word, f);
       }
-    }
-  }
-  sync();
-  // values: words of four tokens of a feature, those that hold a token of the run (or, under a larger scale, an earlier one)
-  const bool regrow = offset > 0 && v_new > v_old && v_new != E4M3_NAN_SCALE;
-  const float f = regrow ? e4m3_scale(max(127 + v_old - v_new, 0)) : 1.f;
-  const int w_first = regrow ? 0 : offset >> 2, w_count = ((offset + n - 1) >> 2) - w_first + 1;
-  if (w_count == 4 && n == E4M3_BLOCK) {
-    for (int feature = thread; feature < a.d; feature += threads) {
-      const uint32_t* const row = reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH);
-      *reinterpret_cast<uint4*>(v_block + feature * E4M3_BLOCK) = make_uint4(row[0], row[1], row[2], row[3]);
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      if (!live[i]) continue;
+      uint8_t* const key = payloads + (offset + me + i * STEP) * a.d;
+      if constexpr (L::FAST) {
+        *reinterpret_cast<uint32_t*>(key + 4 * sub) = e4m3_pack4(x[i][0] * times, x[i][1] * times, x[i][2] * times, x[i][3] * times);
+        *reinterpret_cast<uint32_t*>(key + 4 * sub + half) = e4m3_pack4(y[i][0] * times, y[i][1] * times, y[i][2] * times, y[i][3] * times);
+      } else {
+#pragma unroll
+        for (int j = 0; j < L::PAIRS; ++j) {
+          const int p = L::pair(sub, j);
+          if (p >= half) continue;
+          int ia, ib;
+          L::elements(p, a, ia, ib);
+          const uint16_t both = e4m3_pack(x[i][j] * times, y[i][j] * times);
+          key[ia] = (uint8_t)both;
+          key[ib] = (uint8_t)(both >> 8);
+        }
+      }
     }
   } else {
-#pragma unroll 4
-    for (int i = thread; i < a.d * w_count; i += threads) {
-      const int feature = i % a.d, w0 = 4 * (w_first + i / a.d);
-      uint32_t* const word = reinterpret_cast<uint32_t*>(v_block + feature * E4M3_BLOCK + w0);
-      const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
-      uint32_t w = *reinterpret_cast<const uint32_t*>(v_rows + feature * V_PITCH + w0) & new_bytes;
-      if (new_bytes != 0xffffffffu) {
-        uint32_t there = *word;
-        if (regrow) there = (there & ~old_bytes) | (e4m3_again(there, f) & old_bytes);
-        w |= there & ~new_bytes;
+    // A short run goes to its places byte by byte, without waiting for what is there; others, and runs that round earlier tokens again, through
+    // shared memory, in words of four tokens of a feature.
+    const bool direct = !WHOLE && !regrow;
+    uint8_t* const column = direct ? payloads + offset + me : rows + offset + me;
+    const int pitch = direct ? E4M3_BLOCK : V_PITCH;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      if (!live[i]) continue;
+#pragma unroll
+      for (int j = 0; j < L::PAIRS; ++j) {
+        const int p = L::pair(sub, j);
+        if (p >= half) continue;
+        int ia, ib;
+        L::elements(p, a, ia, ib);
+        const uint16_t both = e4m3_pack(x[i][j] * times, y[i][j] * times);
+        column[ia * pitch + i * STEP] = (uint8_t)both;
+        column[ib * pitch + i * STEP] = (uint8_t)(both >> 8);
       }
-      *word = w;
+    }
+    if (!direct) {
+      if constexpr (WHOLE) __syncthreads();
+      else __syncwarp();
+      const int w_first = regrow ? 0 : offset >> 2, w_count = ((offset + n - 1) >> 2) - w_first + 1;
+      if (n == E4M3_BLOCK) {
+        for (int feature = thread; feature < a.d; feature += threads) {
+          const uint32_t* const row = reinterpret_cast<const uint32_t*>(rows + feature * V_PITCH);
+          *reinterpret_cast<uint4*>(payloads + feature * E4M3_BLOCK) = make_uint4(row[0], row[1], row[2], row[3]);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = thread; i < a.d * w_count; i += threads) {
+          const int feature = i % a.d, w0 = 4 * (w_first + i / a.d);
+          uint32_t* const word = reinterpret_cast<uint32_t*>(payloads + feature * E4M3_BLOCK + w0);
+          const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
+          uint32_t w = *reinterpret_cast<const uint32_t*>(rows + feature * V_PITCH + w0) & new_bytes;
+          if (new_bytes != 0xffffffffu) {
+            uint32_t there = *word;
+            if (regrow) there = (there & ~old_bytes) | (e4m3_again(there, f) & old_bytes);
+            w |= there & ~new_bytes;
+          }
+          *word = w;
+        }
+      }
     }
   }
-  if (thread == 0) {
-    a.k_scale[block] = (uint8_t)k_new;
-    a.v_scale[block] = (uint8_t)v_new;
-  }
-  sync();                                                        // the next run takes the shared memory
+  if (thread == 0) *scale = (uint8_t)now;
+  if constexpr (WHOLE) __syncthreads();                          // the next run takes the shared memory
+  else __syncwarp();
 }
 
-// Blocks: `tile` neighbouring tokens' keys and values of a kv head, then query heads, WARPS * HEADS * Q_ITEMS of them.
+// Blocks: `tile` neighbouring tokens' keys, or values, of a kv head, then query heads, WARPS * HEADS * Q_ITEMS of them.
 template <typename T, typename L, int Q_ITEMS>
 __global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <= 64 ? 6 : 4) qkv_post_e4m3_kernel(const PostArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L::LANES;
-  const int kv_blocks = (a.tokens + a.tile - 1) / a.tile * a.nkv;
+  const int kv_blocks = (a.tokens + a.tile - 1) / a.tile * a.nkv * 2;
 
   if ((int)blockIdx.x >= kv_blocks) {
     // ------------------------------------------------------------ queries: (token, head) pairs in their order
@@ -440,41 +439,50 @@ __global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <=
     return;
   }
 
-  // -------------------------------------------------------------- keys and values of one kv head
+  // -------------------------------------------------------------- keys or values of one kv head
   extern __shared__ __align__(16) uint8_t rows_of_values[];     // [WARPS][d][V_PITCH]
-  __shared__ RunStats shared;
-  const int g = (int)blockIdx.x % a.nkv, t_begin = (int)blockIdx.x / a.nkv * a.tile, t_end = min(a.tokens, t_begin + a.tile);
+  __shared__ float most_of[WARPS];
+  const int item = (int)blockIdx.x >> 1, g = item % a.nkv, t_begin = item / a.nkv * a.tile, t_end = min(a.tokens, t_begin + a.tile);
+  const bool values = blockIdx.x & 1;
   float wx[L::PAIRS], wy[L::PAIRS];
-  load_norm<L>(a, a.k_norm_w, sub, wx, wy);
+  load_norm<L>(a, values ? nullptr : a.k_norm_w, sub, wx, wy);
   // which of the tile's tokens begin a run, and which runs are short (lane i: token t_begin + i; slots were written before the step)
   const int my_t = t_begin + lane;
   bool begins = false, is_short = false;
   if (my_t < t_end) {
     const int slot = slot_at(a, my_t), before = slot_at(a, my_t - 1);
     if (slot < -1 || slot >= a.num_slots) {
-      if (warp == 0 && g == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
+      if (warp == 0 && blockIdx.x % (2 * a.nkv) == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
     } else if (slot >= 0) {
       const bool same = before >= 0 && before / E4M3_BLOCK == slot / E4M3_BLOCK;
       begins = !same;
       // a block's tokens of a step stand next to one another in its order; others are left out
-      if (same && before != slot - 1 && warp == 0 && g == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
+      if (same && before != slot - 1 && warp == 0 && blockIdx.x % (2 * a.nkv) == 0) raise_fault(a.status, VOSTI_FAULT_SLOT_RANGE);
       is_short = begins && !(slot % E4M3_BLOCK + SHORT < E4M3_BLOCK && slot_at(a, my_t + SHORT) == slot + SHORT);
     }
   }
   unsigned long_runs = __ballot_sync(0xffffffffu, begins && !is_short), short_runs = __ballot_sync(0xffffffffu, is_short);
   pdl_wait();
   pdl_launch_dependents();
-  for (; long_runs != 0; long_runs &= long_runs - 1)             // (the same in all warps)
-    store_run<T, L, true>(a, t_begin + __ffs(long_runs) - 1, g, rows_of_values, &shared, wx, wy);
-  for (int i = 0; short_runs != 0; short_runs &= short_runs - 1, ++i)
-    if (i % WARPS == warp) store_run<T, L, false>(a, t_begin + __ffs(short_runs) - 1, g, rows_of_values + warp * a.d * V_PITCH, nullptr, wx, wy);
+  uint8_t* const mine = rows_of_values + warp * a.d * V_PITCH;
+  for (; long_runs != 0; long_runs &= long_runs - 1) {           // (the same in all warps)
+    const int t0 = t_begin + __ffs(long_runs) - 1;
+    if (values) store_run<T, L, true, true>(a, t0, g, rows_of_values, most_of, wx, wy);
+    else store_run<T, L, true, false>(a, t0, g, rows_of_values, most_of, wx, wy);
+  }
+  for (int i = 0; short_runs != 0; short_runs &= short_runs - 1, ++i) {
+    const int t0 = t_begin + __ffs(short_runs) - 1;
+    if (i % WARPS != warp) continue;
+    if (values) store_run<T, L, false, true>(a, t0, g, mine, nullptr, wx, wy);
+    else store_run<T, L, false, false>(a, t0, g, mine, nullptr, wx, wy);
+  }
 }
 
 template <typename T, typename L, int Q_ITEMS>
 cudaError_t launch_post_items(const PostArgs& a, cudaStream_t stream) {
   constexpr int CHUNK = L::HEADS * Q_ITEMS;
   const int64_t q_blocks = ((int64_t)a.tokens * ((a.nq + CHUNK - 1) / CHUNK) + WARPS - 1) / WARPS;
-  const int64_t blocks = (int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv + q_blocks;
+  const int64_t blocks = (int64_t)((a.tokens + a.tile - 1) / a.tile) * a.nkv * 2 + q_blocks;
   return vosti_launch(qkv_post_e4m3_kernel<T, L, Q_ITEMS>, dim3((unsigned)blocks), dim3(THREADS), (size_t)WARPS * a.d * V_PITCH, stream, a);
 }
 template <typename T, typename L>
@@ -519,10 +527,11 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
   VOSTI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qkv_post_e4m3: the cache must start on 16 bytes");
   VOSTI_REQUIRE(slot_mapping != nullptr && k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr, "qkv_post_e4m3: the cache is missing");
   if (tokens == 0) return VOSTI_OK;
-  VOSTI_REQUIRE((int64_t)tokens * (nq + nkv) <= 0x7fffffff - 4096, "qkv_post_e4m3: too many tokens and heads for one launch");
-  // Few tokens: a CTA for each, so that none waits for another's run. Many: a CTA for eight, of which a prompt's hold a run or two and a batch of
-  // single tokens' two a warp. us, so and with a CTA for sixteen whose runs the CTA takes in turn: 128 single tokens 9.7 and 56, a prompt of 2,048 21.6 and 22.4.
-  const int tile = tokens <= FEW ? 1 : TILE;
+  VOSTI_REQUIRE((int64_t)tokens * (nq + 2 * nkv) <= 0x7fffffff - 4096, "qkv_post_e4m3: too many tokens and heads for one launch");
+  // Neighbouring tokens whose runs a CTA takes: few tokens one, so that none waits for another's run; more of them four, a run a warp in a batch of
+  // single tokens; many, as prompts bring them, eight or sixteen, which hold a run or two. us with tiles of 1, 4, 8, 16 (8B sizes): 8 single tokens 3.3, 3.5, 5.2,
+  // 5.2; 64 6.1, 4.3, 5.6, 8.6; 256 12.2, 8.8, 9.3, 12.6; a prompt of 512 14, 7.3, 6.5, 6.1; of 2,048 50, 24, 19.5, 17.1.
+  const int tile = tokens <= FEW ? 1 : tokens <= MANY ? 4 : tokens <= 4 * MANY ? 8 : 16;
   const PostArgs a = {qkv, partial, splits, (int64_t)tokens * (nq + 2 * nkv) * d, q_out, (uint8_t*)k, (uint8_t*)v, (uint8_t*)k_scale,
                       (uint8_t*)v_scale, q_norm_w, k_norm_w, norm_w_is_f32, eps, 1.f / (float)d, cos_table, sin_table, max_positions, positions, slot_mapping,
                       num_slots, page_size, tokens, nq, nkv, d, cos_table != nullptr ? rotary_dim : d, interleaved, tile, status};
