@@ -12,10 +12,11 @@
 // A value that is not finite, or not below 2^96, makes its block's scale 255: the block is no number from then on.
 //
 // A head of 64, 128 or 256 that turns as a whole in pairs (i, i + d/2), or not at all, is d / 8 lanes with four neighbouring elements of each half;
-// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 17 to 19 us, 40% of the rate its bytes could move at: blocks
-// are short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (20 warps with more registers, blocks that walked on over query
-// heads, and a head on a whole warp were slower). Eight tokens take 3 us, which is a launch and three loads that wait for one another; a CTA
-// that took a run's keys and values both needed 5.3.
+// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 17 to 19 us, 40% of the rate its bytes could move
+// at: blocks are short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (20 warps with more
+// registers, blocks that walked on over query heads, and a head on a whole warp were slower). Eight tokens take 3 us; a CTA that took a run's keys and
+// values both needed 5.3. Between a model's other kernels, which leave neither the cache nor the turns in L2, they take 4.5 us behind the projection;
+// without the turns' loads and the blocks' prefetch before its end 6.3, with a grown block's words read one after another 7.4.
 #include "common.cuh"
 #include "e4m3.cuh"
 
@@ -23,6 +24,7 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int SHORT = 4;                       // tokens of a run that one warp takes
+constexpr int ROWS = 4;                        // words of 16 bytes of a block that a lane asks for at a time
 constexpr int V_PITCH = 20;                    // bytes between a feature's rows of values in shared memory (banks apart)
 constexpr int FEW = 32, MANY = 256;
 constexpr int Q_MANY = 4;                      // query heads that a lane holds at a time with more than FEW tokens (up to that, one)
@@ -266,6 +268,16 @@ __device__ __forceinline__ float larger(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
   return r;
 }
+// Masks of the first n bytes of 16.
+__device__ __forceinline__ uint4 first_bytes(int n) {
+  return make_uint4(e4m3_first_bytes(n), e4m3_first_bytes(n - 4), e4m3_first_bytes(n - 8), e4m3_first_bytes(n - 12));
+}
+// Four values' payloads: earlier ones again under the larger scale, new ones, and what else there is.
+__device__ __forceinline__ uint32_t merged(uint32_t there, uint32_t given, uint32_t old_bytes, uint32_t new_bytes, float f) {
+  if (old_bytes != 0) there = (there & ~old_bytes) | (e4m3_again(there, f) & old_bytes);
+  return (there & ~new_bytes) | (given & new_bytes);
+}
+
 // One run's keys (or VALUES): the tokens from t0 on of kv head g, by the whole CTA or by one warp. `rows`: [d][V_PITCH] of its own,
 // `most_of`: a CTA's warps' largest sizes.
 template <typename T, typename L, bool WHOLE, bool VALUES>
@@ -281,10 +293,10 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
   const int64_t page = slot / a.page_size, in_page = slot % a.page_size;
   const int64_t block = (page * a.nkv + g) * (a.page_size / E4M3_BLOCK) + in_page / E4M3_BLOCK;
 
-  int pos[ROUNDS];
-  if (!VALUES) {
+  float c[VALUES ? 1 : ROUNDS][L::PAIRS], s[VALUES ? 1 : ROUNDS][L::PAIRS];
+  if constexpr (!VALUES) {
 #pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) pos[i] = position_of(a, t0 + min(me + i * STEP, n - 1));
+    for (int i = 0; i < ROUNDS; ++i) load_turn<L>(a, position_of(a, t0 + min(me + i * STEP, n - 1)), sub, c[i], s[i]);
   }
   float x[ROUNDS][L::PAIRS], y[ROUNDS][L::PAIRS];
   int64_t at[ROUNDS];
@@ -295,17 +307,17 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
     live[i] = r < n;
     at[i] = ((int64_t)(t0 + r) * heads + a.nq + (VALUES ? a.nkv : 0) + g) * a.d;
   }
-  load_heads<T, L, ROUNDS>(a, at, live, sub, x, y);              // (zeros beyond the run)
   uint8_t* const scale = (VALUES ? a.v_scale : a.k_scale) + block;
+  pdl_wait();                                                    // (nothing before this is of an earlier kernel's making)
+  pdl_launch_dependents();
   const int old = offset > 0 ? *scale : 0;
+  load_heads<T, L, ROUNDS>(a, at, live, sub, x, y);              // (zeros beyond the run)
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
     if (i * STEP >= n) break;                                    // (the same in all lanes)
     if (!VALUES) {
-      float c[L::PAIRS], s[L::PAIRS];
-      load_turn<L>(a, pos[i], sub, c, s);
-      norm_and_turn<L>(a, a.k_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
+      norm_and_turn<L>(a, a.k_norm_w != nullptr, x[i], y[i], wx, wy, c[i], s[i]);
     }
 #pragma unroll
     for (int j = 0; j < L::PAIRS; ++j) most = larger(larger(most, x[i][j]), y[i][j]);
@@ -327,11 +339,18 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
   const float f = regrow ? e4m3_scale(max(127 + old - now, 0)) : 1.f;
 
   if constexpr (!VALUES) {
-    if (regrow)
-      for (int i = thread; i < offset * a.d / 4; i += threads) {
-        uint32_t* const word = reinterpret_cast<uint32_t*>(payloads) + i;
-        *word = e4m3_again(*word, f);
+    if (regrow) {
+      uint4* const words = reinterpret_cast<uint4*>(payloads);
+      for (int i0 = thread; i0 < offset * a.d / 16; i0 += ROWS * threads) {
+        uint4 there[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) there[r] = i0 + r * threads < offset * a.d / 16 ? words[i0 + r * threads] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+          if (i0 + r * threads < offset * a.d / 16)
+            words[i0 + r * threads] = make_uint4(e4m3_again(there[r].x, f), e4m3_again(there[r].y, f), e4m3_again(there[r].z, f), e4m3_again(there[r].w, f));
       }
+    }
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
       if (!live[i]) continue;
@@ -354,7 +373,7 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
     }
   } else {
     // A short run goes to its places byte by byte, without waiting for what is there; others, and runs that round earlier tokens again, through
-    // shared memory, in words of four tokens of a feature.
+    // shared memory, a feature's 16 tokens at a time.
     const bool direct = !WHOLE && !regrow;
     uint8_t* const column = direct ? payloads + offset + me : rows + offset + me;
     const int pitch = direct ? E4M3_BLOCK : V_PITCH;
@@ -375,25 +394,23 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
     if (!direct) {
       if constexpr (WHOLE) __syncthreads();
       else __syncwarp();
-      const int w_first = regrow ? 0 : offset >> 2, w_count = ((offset + n - 1) >> 2) - w_first + 1;
-      if (n == E4M3_BLOCK) {
-        for (int feature = thread; feature < a.d; feature += threads) {
-          const uint32_t* const row = reinterpret_cast<const uint32_t*>(rows + feature * V_PITCH);
-          *reinterpret_cast<uint4*>(payloads + feature * E4M3_BLOCK) = make_uint4(row[0], row[1], row[2], row[3]);
+      const uint4 old_bytes = first_bytes(regrow ? offset : 0);
+      const uint4 mine = first_bytes(offset + n), before = first_bytes(offset);
+      for (int f0 = thread; f0 < a.d; f0 += ROWS * threads) {
+        uint4 there[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const bool read = n < E4M3_BLOCK && f0 + r * threads < a.d;
+          there[r] = read ? reinterpret_cast<const uint4*>(payloads)[f0 + r * threads] : make_uint4(0, 0, 0, 0);
         }
-      } else {
-#pragma unroll 4
-        for (int i = thread; i < a.d * w_count; i += threads) {
-          const int feature = i % a.d, w0 = 4 * (w_first + i / a.d);
-          uint32_t* const word = reinterpret_cast<uint32_t*>(payloads + feature * E4M3_BLOCK + w0);
-          const uint32_t old_bytes = e4m3_first_bytes(offset - w0), new_bytes = e4m3_first_bytes(offset + n - w0) & ~old_bytes;
-          uint32_t w = *reinterpret_cast<const uint32_t*>(rows + feature * V_PITCH + w0) & new_bytes;
-          if (new_bytes != 0xffffffffu) {
-            uint32_t there = *word;
-            if (regrow) there = (there & ~old_bytes) | (e4m3_again(there, f) & old_bytes);
-            w |= there & ~new_bytes;
-          }
-          *word = w;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const int feature = f0 + r * threads;
+          if (feature >= a.d) break;
+          const uint32_t* const row = reinterpret_cast<const uint32_t*>(rows + feature * V_PITCH);
+          reinterpret_cast<uint4*>(payloads)[feature] =
+              make_uint4(merged(there[r].x, row[0], old_bytes.x, mine.x & ~before.x, f), merged(there[r].y, row[1], old_bytes.y, mine.y & ~before.y, f),
+                         merged(there[r].z, row[2], old_bytes.z, mine.z & ~before.z, f), merged(there[r].w, row[3], old_bytes.w, mine.w & ~before.w, f));
         }
       }
     }
@@ -462,8 +479,14 @@ __global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <=
     }
   }
   unsigned long_runs = __ballot_sync(0xffffffffu, begins && !is_short), short_runs = __ballot_sync(0xffffffffu, is_short);
-  pdl_wait();
-  pdl_launch_dependents();
+  // Blocks that hold earlier tokens: on their way to L2 before the projection ends.
+  for (unsigned todo = long_runs | short_runs; todo != 0; todo &= todo - 1) {
+    const int slot = slot_at(a, t_begin + __ffs(todo) - 1), line = (int)threadIdx.x * 128;
+    if (slot % E4M3_BLOCK == 0 || line >= E4M3_BLOCK * a.d + 128) continue;
+    const int64_t block = ((int64_t)(slot / a.page_size) * a.nkv + g) * (a.page_size / E4M3_BLOCK) + slot % a.page_size / E4M3_BLOCK;
+    const uint8_t* const from = threadIdx.x == 0 ? (values ? a.v_scale : a.k_scale) + block : (values ? a.v : a.k) + block * E4M3_BLOCK * a.d + line - 128;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(from));
+  }
   uint8_t* const mine = rows_of_values + warp * a.d * V_PITCH;
   for (; long_runs != 0; long_runs &= long_runs - 1) {           // (the same in all warps)
     const int t0 = t_begin + __ffs(long_runs) - 1;
@@ -476,6 +499,7 @@ __global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <=
     if (values) store_run<T, L, false, true>(a, t0, g, mine, nullptr, wx, wy);
     else store_run<T, L, false, false>(a, t0, g, mine, nullptr, wx, wy);
   }
+  pdl_wait();                                                    // (warps that stored nothing)
 }
 
 template <typename T, typename L, int Q_ITEMS>
