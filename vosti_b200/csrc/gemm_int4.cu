@@ -69,7 +69,9 @@ __device__ __forceinline__ float scale_of(uint32_t word, int i) { return __uint_
 // SM some 190 KB are on their way from the start. The order of k inside an instruction is free: lane j of a row takes offsets 8 j .. 8 j + 7
 // of every 32 k, so that four of them are a word's half and the tokens' 8 are one 16-byte load. An instruction never mixes groups: a group's codes
 // are summed exactly, then multiplied by its scale in float32. The warps' sums meet in shared memory, in warp order.
-// What bounds it: the weights' bytes, then the tokens, which every CTA reads again from L2 (as much as its weights, with FT = 2 and 8 tokens).
+// What bounds it: with many tiles the integer pipe (seven operations at half rate for a word of eight codes: 8 tokens, 151,936 x 4,096 in 80 us, 62% of
+// its bytes' rate); with few the chain from launch to the last sum (4,096 x 4,096 5.2, 4,096 x 12,288 11.5 us; 13.3 when a block's addresses and the
+// tokens' bounds were worked out block by block).
 constexpr int FEW_WARPS = 8, FEW_THREADS = FEW_WARPS * 32;
 constexpr int STAGE_CODES = 4096, FEW_STAGES = 2;
 template <int GROUPS> __host__ __device__ constexpr int stage_bytes() { return STAGE_CODES + 4 * 32 * GROUPS; }
@@ -125,13 +127,23 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
   for (int st = 0; st < min(stages, FEW_STAGES); ++st) request(st);
   pdl_wait();
   pdl_launch_dependents();
-  uint4 b[NT][4];                                                // [8 tokens][32 k] of a block
+  uint4 b[NT][4];                                                // [8 tokens][32 k] of a block; beyond the last token it again (its column is not stored)
+  const bf16* row[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) row[t] = x + (int64_t)min(t * 8 + r8, rows - 1) * k;
+  const bool whole = WORDS && k % KB == 0;
   auto load_block = [&](int kb) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      if (whole) {
+        const uint4* const from = reinterpret_cast<const uint4*>(row[t] + kb * KB + 8 * j);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        b[t][i] = t * 8 + r8 < rows ? load_tokens<WORDS>(x + (int64_t)(t * 8 + r8) * k, kb * KB + 32 * i + 8 * j, k) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) b[t][i] = from[4 * i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[t][i] = load_tokens<WORDS>(row[t], kb * KB + 32 * i + 8 * j, k);
+      }
+    }
   };
   if (blocks > 0) load_block(kb_begin);
   float acc[FT][NT][4];
@@ -139,61 +151,63 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[f][t][0] = acc[f][t][1] = acc[f][t][2] = acc[f][t][3] = 0.f;
-  for (int at = 0; at < blocks; ++at) {
-    const int st = at / DEEP, inside = at % DEEP;
-    if (inside == 0) {
-      const uint32_t bar = smem_addr(&full[warp][st % FEW_STAGES]);
-      if (!__all_sync(0xffffffffu, mb_try_wait(bar, (uint32_t)(st / FEW_STAGES) & 1) || mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status))) {
-        // reported; once more, so that none of the warp's copies is in flight when it ends
-        (void)mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status);
-        if (st + 1 < stages) (void)mb_wait(smem_addr(&full[warp][(st + 1) % FEW_STAGES]), (uint32_t)((st + 1) / FEW_STAGES) & 1, status);
-        break;
-      }
+  for (int st = 0; st < stages; ++st) {
+    const uint32_t bar = smem_addr(&full[warp][st % FEW_STAGES]);
+    if (!__all_sync(0xffffffffu, mb_try_wait(bar, (uint32_t)(st / FEW_STAGES) & 1) || mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status))) {
+      // reported; once more, so that none of the warp's copies is in flight when it ends
+      (void)mb_wait(bar, (uint32_t)(st / FEW_STAGES) & 1, status);
+      if (st + 1 < stages) (void)mb_wait(smem_addr(&full[warp][(st + 1) % FEW_STAGES]), (uint32_t)((st + 1) / FEW_STAGES) & 1, status);
+      break;
     }
-    uint4 now[NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int inside = 0; inside < DEEP; ++inside) {
+      const int at = st * DEEP + inside;
+      if (inside > 0 && at >= blocks) break;
+      uint4 now[NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) now[t][i] = b[t][i];
-    if (at + 1 < blocks) load_block(kb_begin + at + 1);
-    const uint8_t* const stage = mine + st % FEW_STAGES * STAGE + inside * TILE_BYTES;
-    const bf16* const stage_scales = reinterpret_cast<const bf16*>(mine + st % FEW_STAGES * STAGE + STAGE_CODES + inside * SCALES);
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      uint4 c[2];
-      uint32_t s[2][SW];
+        for (int i = 0; i < 4; ++i) now[t][i] = b[t][i];
+      if (at + 1 < blocks) load_block(kb_begin + at + 1);
+      const uint8_t* const stage = mine + st % FEW_STAGES * STAGE + inside * TILE_BYTES;
+      const bf16* const stage_scales = reinterpret_cast<const bf16*>(mine + st % FEW_STAGES * STAGE + STAGE_CODES + inside * SCALES);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        c[h] = *reinterpret_cast<const uint4*>(stage + f * DEEP * TILE_BYTES + (r8 + 8 * h) * (KB / 2) + 16 * j);
-        load_scales<GROUPS>(stage_scales + f * DEEP * (SCALES / 2) + (r8 + 8 * h) * GROUPS, k - (kb_begin + at) * KB, s[h]);
-      }
+      for (int f = 0; f < FT; ++f) {
+        uint4 c[2];
+        uint32_t s[2][SW];
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        float part[NT][4];
+        for (int h = 0; h < 2; ++h) {
+          c[h] = *reinterpret_cast<const uint4*>(stage + f * DEEP * TILE_BYTES + (r8 + 8 * h) * (KB / 2) + 16 * j);
+          load_scales<GROUPS>(stage_scales + f * DEEP * (SCALES / 2) + (r8 + 8 * h) * GROUPS, k - (kb_begin + at) * KB, s[h]);
+        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
+        for (int g = 0; g < GROUPS; ++g) {
+          float part[NT][4];
 #pragma unroll
-        for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
-          const uint32_t lo = int4_word(c[0], i), hi = int4_word(c[1], i);
-          const uint32_t first[4] = {int4_codes<0>(lo, masks), int4_codes<0>(hi, masks), int4_codes<1>(lo, masks), int4_codes<1>(hi, masks)};
-          const uint32_t second[4] = {int4_codes<2>(lo, masks), int4_codes<2>(hi, masks), int4_codes<3>(lo, masks), int4_codes<3>(hi, masks)};
+          for (int t = 0; t < NT; ++t) part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
+#pragma unroll
+          for (int i = g * 4 / GROUPS; i < (g + 1) * 4 / GROUPS; ++i) {
+            const uint32_t lo = int4_word(c[0], i), hi = int4_word(c[1], i);
+            const uint32_t first[4] = {int4_codes<0>(lo, masks), int4_codes<0>(hi, masks), int4_codes<1>(lo, masks), int4_codes<1>(hi, masks)};
+            const uint32_t second[4] = {int4_codes<2>(lo, masks), int4_codes<2>(hi, masks), int4_codes<3>(lo, masks), int4_codes<3>(hi, masks)};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma_bf16(part[t], first, now[t][i].x, now[t][i].y);
+              mma_bf16(part[t], second, now[t][i].z, now[t][i].w);
+            }
+          }
+          const float s0 = scale_of(s[0][g / 2], g), s1 = scale_of(s[1][g / 2], g);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_bf16(part[t], first, now[t][i].x, now[t][i].y);
-            mma_bf16(part[t], second, now[t][i].z, now[t][i].w);
+            acc[f][t][0] = fmaf(part[t][0], s0, acc[f][t][0]);
+            acc[f][t][1] = fmaf(part[t][1], s0, acc[f][t][1]);
+            acc[f][t][2] = fmaf(part[t][2], s1, acc[f][t][2]);
+            acc[f][t][3] = fmaf(part[t][3], s1, acc[f][t][3]);
           }
-        }
-        const float s0 = scale_of(s[0][g / 2], g), s1 = scale_of(s[1][g / 2], g);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          acc[f][t][0] = fmaf(part[t][0], s0, acc[f][t][0]);
-          acc[f][t][1] = fmaf(part[t][1], s0, acc[f][t][1]);
-          acc[f][t][2] = fmaf(part[t][2], s1, acc[f][t][2]);
-          acc[f][t][3] = fmaf(part[t][3], s1, acc[f][t][3]);
         }
       }
     }
-    if (inside == DEEP - 1 && st + FEW_STAGES < stages) {
+    if (st + FEW_STAGES < stages) {
       __syncwarp();                                              // every lane has read the buffer
       request(st + FEW_STAGES);
     }
@@ -502,7 +516,7 @@ cudaError_t launch_few(const Int4Args& a) {
   return vosti_launch(kernel, dim3((a.tiles + FT - 1) / FT), dim3(FEW_THREADS), SMEM, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n, a.k,
                       a.tiles, a.deep, a.status);
 }
-// Tiles of 16 features a CTA: as many as leave two CTAs an SM.
+// Tiles of 16 features a CTA: as many as leave two CTAs an SM. us, 8 tokens, two and four of them: 24,576 x 4,096 18.7 and 15.9, 151,936 x 4,096 89 and 80.
 template <int GROUPS, int NT>
 cudaError_t launch_few_as(const Int4Args& a, bool words) {
   if (!words) return launch_few<1, NT, GROUPS, false>(a);
