@@ -51,9 +51,10 @@ def heads_after(x, w, eps, cos, sin, pos, rotary, neighbours):
     return y
 
 
-def attend(q, keys, values, *, pos, nq, nkv, scale, window):
+def attend(q, keys, values, *, pos, nq, nkv, scale, window, value_scales=None):
     """(out, spread, reach) of one request's query rows q [n, nq, d] at positions `pos` over keys and values [nkv, kv, d]: the
-    output, sum_j p_j |v_j|, and the largest scale * sum |q||k| (what the error bounds are made of)."""
+    output, sum_j p_j |v_j|, and the largest scale * sum |q||k| (what the error bounds are made of). With the values' scales [nkv, kv] also the
+    largest p_j scale_j times sum_j |v_j| / scale_j."""
     n, _, d = q.shape
     group = nq // nkv
     q = q.double().view(n, nkv, group, d)
@@ -73,7 +74,13 @@ def attend(q, keys, values, *, pos, nq, nkv, scale, window):
     p = torch.where(seen.any(-1).view(n, 1, 1, 1), p, 0.0)
     v = torch.nan_to_num(v, nan=0.0)
     out, spread = torch.einsum("nhgk,hkd->nhgd", p, v), torch.einsum("nhgk,hkd->nhgd", p, v.abs())
-    return out.reshape(n, nq, d), spread.reshape(n, nq, d), reach.reshape(n, nq, 1)
+    three = out.reshape(n, nq, d), spread.reshape(n, nq, d), reach.reshape(n, nq, 1)
+    if value_scales is None:
+        return three
+    s = torch.nan_to_num(value_scales, nan=0.0)
+    payload = torch.where(s.unsqueeze(-1) > 0, v.abs() / s.unsqueeze(-1), 0.0)
+    beside = torch.nan_to_num(p * s.view(1, nkv, 1, -1), nan=0.0).amax(-1, keepdim=True) * torch.einsum("nhgk,hkd->nhgd", seen.view(n, 1, 1, -1).expand(p.shape).double(), payload)
+    return (*three, beside.reshape(n, nq, d))
 
 
 def step(new, past, page_size, device="cuda:0", *, seed=0, spare=2, shuffled=True):

@@ -3,7 +3,9 @@
 Bounds. A rounding to bfloat16 is off by 2^-8 of the value at most, one to e4m3 by 2^-4 (2^-10 scales below its normal range).
 Attention rounds the weights (2^-8 of sum p |v|) and the output (2^-8); payloads, scales and their products in bfloat16 are exact; scores are float32
 sums of d products: off by d 2^-23 of sum |q||k| scale, which moves a weight, and the sum of the weights, by as much; the special-function unit's
-exponential adds 2^-21."""
+exponential adds 2^-21. Where weights are taken together with their values' scales, in float16 with 2^15 for the largest, those below 2^-14 are multiples
+of 2^-24, so off by 2^-25, which is 2^-40 of the largest p_j scale_j, for every |v_j| / scale_j: what counts where the heaviest key's value is near zero and
+others' scales are far from its own."""
 import math
 
 import pytest
@@ -196,14 +198,17 @@ def test_a_value_that_is_not_finite_marks_its_block(bad):
 # ---------------------------------------------------------------- attention
 def check_attention(q, cache, ctx, group, out, *, nq, nkv, d, window, scale):
     keys, values = plain.dequantized(cache)
+    v_scales = plain.scales(cache.v_scale).repeat_interleave(16, dim=2)
     at = 0
     for r, (n, total) in enumerate(zip(ctx.host_q_lens, ctx.host_kv_lens)):
         page, place = plain.rows_of(group.block_table[r], total, group.page_size)
         k, v = keys[page, :, place].transpose(0, 1), values[page, :, place].transpose(0, 1)
-        want, spread, reach = plain.attend(q[at:at + n].cpu().view(n, nq, d), k, v, pos=torch.arange(total - n, total), nq=nq, nkv=nkv, scale=scale, window=window)
+        s = v_scales[page, :, place].transpose(0, 1)
+        want, spread, reach, beside = plain.attend(q[at:at + n].cpu().view(n, nq, d), k, v, pos=torch.arange(total - n, total), nq=nq, nkv=nkv, scale=scale, window=window,
+                                                   value_scales=s)
         got = out[at:at + n].cpu().double().view(n, nq, d)
         half = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -22
-        bound = half * (spread + want.abs()) + 2 * (d * 2.0 ** -23 * reach + 2.0 ** -21) * spread + total * 2.0 ** -24 * spread
+        bound = half * (spread + want.abs()) + 2 * (d * 2.0 ** -23 * reach + 2.0 ** -21) * spread + total * 2.0 ** -24 * spread + 2.0 ** -40 * beside
         assert torch.equal(got.isnan(), want.isnan())
         worst = ((got - want).abs() - bound).nan_to_num(0.0).max()
         assert float(worst) <= 0, (r, float(worst))
@@ -367,3 +372,95 @@ def test_another_stream_and_a_graph():
         kept.zero_()
         graph.replay()
         assert torch.equal(kept, want)
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.parametrize("new,past", [([1], [0]), ([1] * 3, [15, 16, 700]), ([1] * 9, [0, 63, 64, 65, 127, 128, 1000, 2047, 31]), ([4, 1, 3], [60, 61, 190]), ([70, 1, 4, 1], [30, 500, 126, 64]),
+                                      ([1] * 70, [(i * 131) % 900 for i in range(70)])])
+@pytest.mark.parametrize("nq,nkv,d,window", [(32, 8, 128, 0), (4, 2, 64, 0), (8, 1, 128, 40), (24, 1, 64, 0)])
+def test_attention_right_behind_the_store(new, past, nq, nkv, d, window):
+    """What is read while the store still runs is what stands there after it: with blocks whose scale grows, so that their earlier tokens
+    are rounded again, the same bits as from a call that waits."""
+    gen = torch.Generator().manual_seed(len(new) + nq)
+    ctx, group, pages = plain.step(new, past, 16, seed=7)
+    first = [plain.random_cache(pages, nkv, 16, d, gen, low=100, high=120) for _ in range(4)]
+    qkv = [(torch.randn(sum(new), (nq + 2 * nkv) * d, generator=gen) * 3).bfloat16().to(DEVICE) for _ in first]
+    copies = lambda: [ops.PagedE4M3(*(getattr(c, n).view(torch.uint8).clone().view(getattr(c, n).dtype) for n in ("k", "v", "k_scale", "v_scale"))) for c in first]
+    sizes = dict(nq=nq, nkv=nkv, head_dim=d)
+
+    def run(caches, outs, **more):
+        for cache, x in zip(caches, qkv):
+            q = ops.qkv_post_e4m3(x, cache, slot_mapping=group.slot_mapping, status=ctx.status, **sizes)
+            outs.append(ops.attention_e4m3(ctx, q, cache, group, scale=d ** -0.5, window=window, **sizes, **more))
+            if not more:
+                torch.cuda.synchronize()
+    slow, fast = copies(), copies()
+    want, got = [], []
+    run(slow, want)
+    run(fast, got, appended=ctx.max_q_len)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(fast, slow):
+        assert all(torch.equal(getattr(a, n).view(torch.uint8), getattr(b, n).view(torch.uint8)) for n in ("k", "v", "k_scale", "v_scale"))
+    check_attention(ops.qkv_post_e4m3(qkv[0], copies()[0], slot_mapping=group.slot_mapping, status=ctx.status, **sizes), fast[0], ctx, group, got[0], nq=nq, nkv=nkv, d=d,
+                    window=window, scale=d ** -0.5)
+    again, kept = copies(), []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(again, kept, appended=ctx.max_q_len)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(kept, want)) and int(ctx.status) == 0
+
+
+@pytest.mark.parametrize("d,count", [(128, 1), (128, 40), (64, 3), (96, 2)])
+def test_tokens_of_a_block_one_after_another(d, count):
+    """Stores that follow one another without a pause, each with larger values than the last: every one of them rounds what the block holds again."""
+    gen = torch.Generator().manual_seed(5)
+    steps = [plain.step([1] * count, [p] * count, 16, seed=2, spare=2 if p > 15 else 2 + count) for p in range(12, 24)]
+    ctx, group, pages = steps[-1]
+    rows = [(torch.randn(count, 4 * d, generator=gen) * 1.7 ** i).bfloat16().to(DEVICE) for i in range(len(steps))]
+    table = group.block_table.cpu()
+    slots = [torch.tensor([int(table[r, p // 16]) * 16 + p % 16 for r in range(count)], dtype=torch.int32, device=DEVICE) for p in range(12, 24)]
+    kept = []
+    for wait in (True, False):
+        cache = plain.random_cache(pages, 1, 16, d, torch.Generator().manual_seed(9), low=90, high=100)
+        torch.cuda.synchronize()
+        for x, slot in zip(rows, slots):
+            ops.qkv_post_e4m3(x, cache, nq=2, nkv=1, head_dim=d, slot_mapping=slot, status=ctx.status)
+            if wait:
+                torch.cuda.synchronize()
+        kept.append([getattr(cache, n).view(torch.uint8).clone() for n in ("k", "v", "k_scale", "v_scale")])
+    assert all(torch.equal(a, b) for a, b in zip(*kept)) and int(ctx.status) == 0
+
+
+def test_calls_that_are_refused():
+    ctx, group, pages = plain.step([2, 40], [5, 0], 16)
+    cache = ops.PagedE4M3.zeros(pages, 2, 16, 64)
+    x = torch.zeros(42, 8 * 64, dtype=torch.bfloat16, device=DEVICE)
+    cos = torch.ones(64, 32, device=DEVICE)
+    good = dict(nq=4, nkv=2, head_dim=64, slot_mapping=group.slot_mapping, status=ctx.status)
+    ops.qkv_post_e4m3(x, cache, **good)
+    w64, w32 = torch.ones(64, dtype=torch.bfloat16, device=DEVICE), torch.ones(32, dtype=torch.bfloat16, device=DEVICE)
+    for bad, more in ((x[0], {}), (x.half(), {}), (x.cpu(), {}), (x[:, :-64], {}), (x.t().contiguous().t(), {}), (x, dict(nkv=4)), (x, dict(nq=0, nkv=4)), (x, dict(head_dim=128)),
+                      (x, dict(slot_mapping=group.slot_mapping[:5])), (x, dict(slot_mapping=group.slot_mapping.long())), (x, dict(slot_mapping=group.slot_mapping.cpu())),
+                      (x, dict(status=ctx.status.float())), (x, dict(cos=cos, sin=cos)), (x, dict(cos=cos, positions=ctx.positions)),
+                      (x, dict(cos=cos, sin=cos[:, :16], positions=ctx.positions)), (x, dict(cos=cos.double(), sin=cos, positions=ctx.positions)),
+                      (x, dict(cos=cos, sin=cos, positions=ctx.positions[:3])), (x, dict(cos=cos, sin=cos, positions=ctx.positions, rotary_dim=128)),
+                      (x, dict(q_norm_w=w32)), (x, dict(k_norm_w=w64.float(), q_norm_w=w64))):
+        with pytest.raises(ops.KernelError):
+            ops.qkv_post_e4m3(bad, cache, **{**good, **more})
+    q = torch.zeros(42, 4 * 64, dtype=torch.bfloat16, device=DEVICE)
+    good = dict(nq=4, nkv=2, head_dim=64, scale=0.1)
+    ops.attention_e4m3(ctx, q, cache, group, **good)
+    for bad, more in ((q[0], {}), (q.half(), {}), (q.cpu(), {}), (q[:, :-64], {}), (q.t().contiguous().t(), {}), (q, dict(nkv=4)), (q, dict(nq=5)), (q, dict(nkv=0)),
+                      (q, dict(head_dim=32)), (q, dict(scale=0.0)), (q, dict(scale=math.nan)), (q, dict(window=-1)), (q, dict(appended=-1))):
+        with pytest.raises(ops.KernelError):
+            ops.attention_e4m3(ctx, bad, cache, group, **{**good, **more})
+    for owner, name, bad in ((ctx, "positions", ctx.positions[:7]), (ctx, "request_of", ctx.request_of.long()), (ctx, "cu_q", ctx.cu_q.long()), (ctx, "kv_len", ctx.kv_len.cpu()),
+                             (ctx, "status", ctx.status.long()), (group, "block_table", group.block_table.long()), (group, "block_table", group.block_table[0]),
+                             (group, "page_size", 32)):
+        kept = getattr(owner, name)
+        setattr(owner, name, bad)
+        with pytest.raises(ops.KernelError):
+            ops.attention_e4m3(ctx, q, cache, group, **good)
+        setattr(owner, name, kept)
+    assert int(ctx.status) == 0

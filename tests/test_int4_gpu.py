@@ -117,3 +117,20 @@ def test_tiles_ask_for_no_more_tensor_memory_than_an_sm_has():
     for tile in range(4):
         assert 0 < ops.library().vosti_gemm_int4_columns_an_sm(tile) <= 512
     assert ops.library().vosti_gemm_int4_columns_an_sm(4) == -1
+
+
+def test_calls_that_are_refused():
+    w, _, gen = weight(64, 256, 64)
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    x = torch.randn(5, 256, generator=gen).bfloat16().to(DEVICE)
+    ops.gemm_int4(x, w, status)
+    for bad in (x[0], x.float(), x.cpu(), x[:, :128].contiguous(), x[:, ::2], x.t().contiguous().t()):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int4(bad, w, status)
+    for more in (dict(out_dtype=torch.float16), dict(out_dtype=torch.uint8)):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int4(x, w, status, **more)
+    for bad in (status.cpu(), status.float(), status[:0]):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int4(x, w, bad)
+    assert int(status) == 0

@@ -2434,7 +2434,6 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
     everything else on the CUDA cores in float32. `appended` > 0 says that the kernel launched right before is the step's own
     `qkv_post_e4m3`, which stored at most that many of each request's newest tokens: what lies before them is then read
     while it still runs. 0: nothing is known of it."""
-    tokens = q.shape[0]
     if q.dim() != 2 or q.shape[1] != nq * head_dim or q.dtype not in (torch.bfloat16, torch.float32):
         raise KernelError("attention_e4m3: the queries are bfloat16 or float32 [tokens, nq * d]")
     if nq <= 0 or nkv <= 0 or nq % nkv or cache.heads != nkv or cache.head_dim != head_dim or group.page_size != cache.page_size:
@@ -2444,7 +2443,9 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
         raise KernelError("attention_e4m3: the block table is int32 [requests, pages]")
     if window < 0 or appended < 0 or not scale > 0:
         raise KernelError("attention_e4m3: the score scale must be positive, the window and the appended tokens not negative")
+    tokens = q.shape[0]
     _ints("attention_e4m3", tokens, positions=ctx.positions, request_of=ctx.request_of)
+    _ints("attention_e4m3", 1, status=status)
     stream = _here("attention_e4m3", q, cache.k, ctx.positions, ctx.request_of, table, status)
     out = torch.empty_like(q)
     geometry = (table.data_ptr(), table.shape[1], cache.page_size, cache.pages, nq, nkv, head_dim)
@@ -2461,6 +2462,7 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
         short = ctx.extras.get("attention.short_tokens")
     if long_rows:
         rows = ctx.extras.get("attention.long_rows")
+        _ints("attention_e4m3", long_rows, cu_q=ctx.cu_q, kv_len=ctx.kv_len, **({} if rows is None else {"long_rows": rows}))
         _here("attention_e4m3", rows, ctx.cu_q, ctx.kv_len)
         _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iifipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
@@ -2468,6 +2470,7 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
     if count:
         # (beside the portions' kernel, whose last CTAs leave SMs free)
         if short is not None:
+            _ints("attention_e4m3", count, short_tokens=short)
             _here("attention_e4m3", short)
         _check(_bound("vosti_attention_e4m3", "pppppp" "pipp" "piiiiii" "ifiiipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(short), count, ctx.positions.data_ptr(), ctx.request_of.data_ptr(), *geometry,
@@ -2556,10 +2559,11 @@ class Int4Weight:
 def gemm_int4(x: torch.Tensor, w: Int4Weight, status: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y = x @ w.T for bfloat16 rows and a weight in 4 bits, rounded once to `out_dtype` (bfloat16 or float32). Up to 16 rows a group's codes
     are summed exactly and scaled in float32; more rows multiply codes times scales rounded to bfloat16."""
-    rows, k = x.shape
-    features = w.shape[0]
-    if x.dtype != torch.bfloat16 or k != w.shape[1]:
-        raise KernelError(f"gemm_int4: x is bfloat16 [rows, {w.shape[1]}], got {x.dtype} {tuple(x.shape)}")
+    features, k = w.shape
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != k:
+        raise KernelError(f"gemm_int4: x is bfloat16 [rows, {k}], got {x.dtype} {tuple(x.shape)}")
+    rows = x.shape[0]
+    _ints("gemm_int4", 1, status=status)
     out_dtype = out_dtype or torch.bfloat16
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"gemm_int4: the result is bfloat16 or float32, not {out_dtype}")
