@@ -263,6 +263,34 @@ def test_portions(new, past, nq, nkv, d, page):
     attention(new, past, nq=nq, nkv=nkv, d=d, page=page, seed=3)
 
 
+@pytest.mark.parametrize("new,past", [([300], [1200]), ([20], [1500]), ([5], [3000]), ([130, 7, 1], [900, 2000, 50]), ([64], [700]), ([512], [600])])
+@pytest.mark.parametrize("nq,nkv,d,page,window", [(32, 8, 128, 16, 0), (6, 2, 64, 32, 0), (16, 1, 128, 16, 0), (8, 8, 64, 64, 900), (5, 1, 128, 48, 600)])
+def test_portions_behind_long_caches(new, past, nq, nkv, d, page, window):
+    """Few rows, many keys: the keys are cut over CTAs."""
+    attention(new, past, nq=nq, nkv=nkv, d=d, page=page, window=window, seed=4)
+
+
+def test_segments_of_both_head_sizes():
+    """One token of few heads behind many keys, for each head size first or after the other."""
+    for d in (64, 128, 64):
+        attention([1], [9000], nq=2, nkv=1, d=d, page=64)
+
+
+@pytest.mark.parametrize("side", ["k_scale", "v_scale"])
+def test_segments_that_are_no_number(side):
+    gen = torch.Generator().manual_seed(4)
+    ctx, group, pages = plain.step([40, 1], [1000, 600], 16)
+    cache = plain.random_cache(pages, 1, 16, 128, gen)
+    first, middle = (int(group.block_table[0, i]) for i in (0, 40))
+    for blocks in ([middle], [first, middle], [int(p) for p in group.block_table[0, :16]]):
+        for b in blocks:
+            getattr(cache, side).view(torch.uint8)[b, 0, 0] = 255
+        for window in (0, 100):
+            q = torch.randn(41, 2 * 128, generator=gen).bfloat16().to(DEVICE)
+            out = ops.attention_e4m3(ctx, q, cache, group, nq=2, nkv=1, head_dim=128, scale=0.09, window=window)
+            check_attention(q, cache, ctx, group, out, nq=2, nkv=1, d=128, window=window, scale=0.09)
+
+
 @pytest.mark.parametrize("new,past", [([1], [0]), ([1, 1], [40, 300]), ([70, 1, 5], [30, 64, 0])])
 @pytest.mark.parametrize("dtype,nq,nkv,d,window", [(torch.float32, 4, 2, 128, 0), (torch.float32, 3, 3, 80, 33), (torch.bfloat16, 4, 1, 96, 0), (torch.bfloat16, 2, 2, 256, 40),
                                                    (torch.float32, 2, 1, 16, 0)])

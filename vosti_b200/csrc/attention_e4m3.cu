@@ -195,8 +195,8 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
   };
 
   // `beside`: the kernel before this one is the same step's attention of portions, which neither writes what this one reads nor reads what it
-  // writes, and waited for everything before it in all of its CTAs before it let this one start. It is waited for at the end only
-  // (the chain of completed kernels stays unbroken).
+  // writes, and waited for everything before it in all of its CTAs before it let this one start. The last CTA alone waits for it, at its end:
+  // this kernel then ends after it (the chain of completed kernels stays unbroken), while CTAs that are done leave their place to others.
   int64_t next = block_of(begin + warp);
   auto start = [&] {
     request(0, next);
@@ -430,7 +430,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
       for (int w = 0; w < WARPS; ++w) v += part[w][h][f];
       out[q_at + i] = finish(v, joined(stats, WARPS, h));
     }
-    if (beside) pdl_wait();
+    if (beside && blockIdx.x == gridDim.x - 1) pdl_wait();
     return;
   }
   // ---- the segments' sums into one, in their order: each CTA of the cluster is sent its share of the row by all of them
@@ -460,7 +460,7 @@ attention_e4m3_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const 
     for (int s = 0; s < segments; ++s) v += inbox[s * share + i] * fast_exp2(inbox_stats[s][h][2] - safe_v);
     out[q_at + seg * share + i] = finish(v, r);
   }
-  if (beside) pdl_wait();
+  if (beside && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------------- CUDA cores
@@ -591,9 +591,10 @@ int segments_of(int64_t items, int max_kv_len) {
   return most < 1 ? 1 : (int)most;
 }
 
-// Whether clusters of `size` CTAs can run at all; asked once per device, kernel and size.
-template <typename Kernel>
-bool cluster_runs(Kernel kernel, int threads, int smem, int size) {
+// Whether clusters of `size` CTAs can run at all; asked once per device, kernel (by its head size) and size.
+template <int D>
+bool cluster_runs(int smem, int size) {
+  auto kernel = attention_e4m3_kernel<D>;
   static std::unordered_map<uint64_t, bool> known;
   static std::mutex mutex;
   std::lock_guard<std::mutex> lock(mutex);
@@ -605,7 +606,7 @@ bool cluster_runs(Kernel kernel, int threads, int smem, int size) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)size);
-  config.blockDim = dim3((unsigned)threads);
+  config.blockDim = dim3((unsigned)THREADS);
   config.dynamicSmemBytes = (size_t)smem;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -641,7 +642,7 @@ cudaError_t launch_e4m3(const Launch& a) {
   const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (raised != cudaSuccess) return raised;
   int segments = a.segments;
-  while (segments > 1 && !cluster_runs(kernel, THREADS, SMEM, segments)) --segments;
+  while (segments > 1 && !cluster_runs<D>(SMEM, segments)) --segments;
   const dim3 grid((unsigned)(a.items * segments));
   if (segments == 1)
     return vosti_launch(kernel, grid, dim3(THREADS), SMEM, a.stream, a.q, a.out, a.c, a.token_list, a.positions, a.request_of, a.nq, a.nkv, a.scale_log2,

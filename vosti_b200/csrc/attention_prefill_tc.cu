@@ -37,6 +37,8 @@
 // A cache of 8 bits (e4m3.cuh) differs in the loaders alone: a loader warp's 16 keys are a block with one scale. It reads
 // the block's payloads into registers while the stage is still in use, makes them bfloat16 (exactly: the scale is a power
 // of two) and stores them swizzled. Values lie feature-major in the cache, so the second MMA reads them K-major.
+// Its keys may also be cut into segments, one CTA of a cluster each: every CTA sends its rows' running products and statistics to the
+// CTA that joins them (each of them a share of the rows), through shared memory that the tiles no longer need.
 #include <type_traits>
 
 #include "common.cuh"
@@ -69,10 +71,21 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 
 // score; keys before `bias_last` are visible whatever the window (tiles of them come first, in ascending key
 // order like all tiles); and every head's row is multiplied by the sigmoid of head_gate[token, head] (or null).
 // Without BIASED the arithmetic is what it was before the flag existed, bit for bit.
-// Side: how keys, or values, are held: a tensor map of a bfloat16 cache, or an E4m3Side.
+// Side: how keys, or values, are held: a tensor map of a bfloat16 cache, or an E4m3Side (CUT: the keys are cut into segments).
+template <bool CUT>
 struct E4m3Side {
   const uint8_t *payload, *scale;
+  int segments;                           // CTAs that a pair of row tiles' keys are cut over: 1, 2, 4 or 8
 };
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t address_at_rank(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
 template <int D, bool BIASED, bool CAPPED, bool SLOPED, typename Side = CUtensorMap>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Side map_k,
@@ -83,7 +96,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                             int window, const float* __restrict__ bias, int bias_last,
                             const float* __restrict__ sink, float softcap, const float* __restrict__ head_gate, unsigned* status) {
   const float scale_log2 = BIASED ? 1.f : scale_log2_in;      // BIASED: scores are scaled where the bias is added
-  constexpr bool EIGHT = std::is_same<Side, E4m3Side>::value;
+  constexpr bool CUT = std::is_same<Side, E4m3Side<true>>::value, EIGHT = CUT || std::is_same<Side, E4m3Side<false>>::value;
   constexpr int NB = D / 64;                          // 64-element blocks of the head size
   constexpr int STAGES = kv_stages<D>();
   constexpr int Q_BYTES = NB * ROWS * 128;            // one row tile of Q
@@ -105,7 +118,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = row_list ? row_list[blockIdx.y] : blockIdx.y;
-  const int g = blockIdx.x % nkv, pair = blockIdx.x / nkv, pairs = gridDim.x / nkv;
+  int segments = 1;
+  if constexpr (CUT) segments = map_k.segments;
+  const int seg = blockIdx.x % segments, place = blockIdx.x / segments;
+  const int g = place % nkv, pair = place / nkv, pairs = gridDim.x / segments / nkv;
   const int group = nq / nkv;
   const int tokens_per_tile = ROWS / group, rows_used = tokens_per_tile * group;
   pdl_wait();
@@ -117,7 +133,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   // the tiles from the first tile's first key to the last tile's last key, a row tile stops at
   // its own end
   const int first_key = first_visible_key(shift + token0, window);
-  const int tile_begin = (first_key / KT) * KT;
+  int tile_begin = (first_key / KT) * KT;
   const int keep = SLOPED ? bias_last : 0;
   const int head_tiles = SLOPED ? min((keep + KT - 1) / KT, tile_begin / KT) : 0;        // tiles of kept keys before the window
   auto tile_key = [&](int t) { return SLOPED && t < head_tiles ? t * KT : tile_begin + (t - head_tiles) * KT; };
@@ -129,7 +145,14 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     tiles_of[w] = end > tile_begin ? head_tiles + (end - tile_begin + KT - 1) / KT : 0;
     key_end = max(key_end, end);
   }
-  const int tiles = max(tiles_of[0], tiles_of[1]);
+  int tiles = max(tiles_of[0], tiles_of[1]);
+  if constexpr (CUT) {                                // this CTA's run of the tiles
+    const int from = tiles * seg / segments, to = tiles * (seg + 1) / segments;
+#pragma unroll
+    for (int w = 0; w < ROW_TILES; ++w) tiles_of[w] = max(min(tiles_of[w], to) - from, 0);
+    tile_begin += from * KT;
+    tiles = to - from;
+  }
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -307,7 +330,59 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     if (ok && my_tiles > 0)
       ok = mbar_wait(smem_u32(&p_empty[wg][(my_tiles - 1) & 1]), ((my_tiles - 1) >> 1) & 1, &abort_flag, status);
     tc_fence_after();
-    if (my_tiles > 0) {
+    if constexpr (CUT) {
+      // ---- the segments' sums into one, in their order: rows share * rank .. of the pair of row tiles at each rank. [segment][row][D] float32 where queries and keys were
+      // (16-byte pieces swizzled: a warp's rows lie a whole number of 128 bytes apart), then [segment][row] the maximum and the sum.
+      constexpr int JOINED_BYTES = ROW_TILES * ROWS * D * 4;
+      static_assert(JOINED_BYTES + ROW_TILES * ROWS * 8 <= ROW_TILES * Q_BYTES + STAGES * STAGE_BYTES, "the segments' sums take the tiles' place");
+      const int share = ROW_TILES * ROWS / segments, row = wg * ROWS + r, local = row % share;
+      const uint32_t base = smem_u32(q_s), at_rank = address_at_rank(base, row / share);
+      cluster_barrier();                                         // every CTA's tiles have been read
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at_rank + JOINED_BYTES + (seg * share + local) * 8), "f"(m_run), "f"(l_run) : "memory");
+      if (my_tiles > 0) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t v[32];
+          tmem_load32(o_tmem + c0, v);                           // (all lanes of the warp take part)
+          if (valid) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at_rank + (seg * share + local) * (D * 4) + (((c0 >> 2) + c) ^ (local & 7)) * 16),
+                           "r"(v[4 * c]), "r"(v[4 * c + 1]), "r"(v[4 * c + 2]), "r"(v[4 * c + 3])
+                           : "memory");
+          }
+        }
+      }
+      cluster_barrier();
+      const uint8_t* const sums = q_s;
+      const float2* const stats = reinterpret_cast<const float2*>(q_s + JOINED_BYTES);
+      for (int u = threadIdx.x; u < share * (D / 8) && !abort_flag; u += ROW_TILES * ROWS) {
+        const int mine = u / (D / 8), c8 = u % (D / 8), joined = seg * share + mine, of_tile = joined % ROWS;
+        const int t = token0 + joined / ROWS * tokens_per_tile + of_tile / group;
+        if (of_tile >= rows_used || t >= q_len) continue;
+        float top = -INFINITY;
+        for (int s = 0; s < segments; ++s) top = fmaxf(top, stats[s * share + mine].x);
+        float sum = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < segments; ++s) {
+          const float2 st = stats[s * share + mine];
+          if (st.x == -INFINITY && st.y == 0.f) continue;        // saw nothing (a sum that is no number stays one)
+          const float weight = st.x == -INFINITY ? 1.f : fast_exp2(st.x - top);
+          sum += st.y * weight;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 v = *reinterpret_cast<const float4*>(sums + (s * share + mine) * (D * 4) + ((2 * c8 + h) ^ (mine & 7)) * 16);
+            y[4 * h] += v.x * weight;
+            y[4 * h + 1] += v.y * weight;
+            y[4 * h + 2] += v.z * weight;
+            y[4 * h + 3] += v.w * weight;
+          }
+        }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        bf16* const dst = out + ((int64_t)(q_start + t) * nq + g * group + of_tile % group) * D + 8 * c8;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv), pack_bf16(y[4] * inv, y[5] * inv),
+                                                    pack_bf16(y[6] * inv, y[7] * inv));
+      }
+    } else if (my_tiles > 0) {
       if (BIASED && sink != nullptr && valid && m_run > -INFINITY) l_run += fast_exp2(sink[head] * LOG2E - m_run);
       float inv = l_run > 0.f ? 1.f / l_run : 0.f;
       if (SLOPED && valid && head_gate != nullptr) inv *= 1.f / (1.f + expf(-head_gate[(int64_t)(q_start + token) * nq + head]));
@@ -405,6 +480,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&kv_full[stage]));
+      }
+      if constexpr (CUT) {
+        cluster_barrier();
+        cluster_barrier();
       }
     } else
     for (int j = 0; j < tiles && ok; ++j) {
@@ -517,6 +596,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         }
         __syncwarp();
       }
+    }
+    if constexpr (CUT) {
+      cluster_barrier();
+      cluster_barrier();
     }
   }
   tc_fence_before();
@@ -651,11 +734,21 @@ VOSTI_API int vosti_attention_prefill_tc_sloped(const void* q, const void* k_cac
                            stream, true, head_gate);
 }
 
-// The same over a cache of 8 bits (e4m3.cuh); q and out as above.
+// Segments of the keys: as many as still find an SM at once (a CTA fills one), of a tile or more each, two from 16 tiles on. us at 1, 2, 4 and 8
+// (32 query heads, 8 kv heads of 128; `ctas` in brackets): 16 tokens behind 2,048 [8] 54, 35, 25, 20; 64 behind 4,096 [16] 112, 67, 42, 31; 128
+// behind 2,048 [24] 62, 42, 30, 46; 512 behind 2,048 [72] 73, 49, 64, 117; 512 behind 8,192 [72] 223, 124, 139; a prompt of 512 [72] 22, 23, 36, 78; of
+// 256 [40] 15, 19, 17, 46; of 2,048 [264] 65, 109, 179.
+static int prefill_segments(int64_t ctas, int tiles) {
+  for (int s = 8; s > 1; s /= 2)
+    if (ctas * s <= 148 && tiles >= (s == 2 ? 16 : 8)) return s;
+  return 1;
+}
+
+// The same over a cache of 8 bits (e4m3.cuh); q and out as above. `max_kv_len`: no request has more keys.
 VOSTI_API int vosti_attention_prefill_tc_e4m3(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, void* out,
                                               const int* row_list, int count, const int* cu_q, const int* kv_len, const int* block_table,
                                               int max_pages, int page_size, int num_pages, int nq, int nkv, int d, int max_q_len,
-                                              int tokens_total, float scale, int window, unsigned* status, cudaStream_t stream) {
+                                              int tokens_total, int max_kv_len, float scale, int window, unsigned* status, cudaStream_t stream) {
   VOSTI_REQUIRE(count >= 0 && count <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0 && nq / nkv <= 16,
                 "attention_prefill_tc_e4m3: bad request or head counts (%d requests, nq=%d nkv=%d)", count, nq, nkv);
   VOSTI_REQUIRE(vosti_attention_prefill_tc_supported(d, page_size),
@@ -670,23 +763,38 @@ VOSTI_API int vosti_attention_prefill_tc_e4m3(const void* q, const void* k, cons
   const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)nq * d * 2, 128};
   const cuuint32_t box[4] = {64, (cuuint32_t)group, (cuuint32_t)tokens_per_tile, 1};
   VOSTI_REQUIRE(encode_tensor_map_nd(&map_q, q, 4, dims, strides, box), "attention_prefill_tc_e4m3: cuTensorMapEncodeTiled failed (q)");
-  const E4m3Side keys = {(const uint8_t*)k, (const uint8_t*)k_scale}, values = {(const uint8_t*)v, (const uint8_t*)v_scale};
-  const dim3 grid((unsigned)((max_q_len + tokens_per_cta - 1) / tokens_per_cta) * nkv, count);
+  const int64_t ctas = ((int64_t)tokens_total / tokens_per_cta + count) * nkv;            // (at most; the grid's others end at once)
+  const int tiles = ((window > 0 && window + tokens_per_cta < max_kv_len ? window + tokens_per_cta : max_kv_len) + KT - 1) / KT;
+  const int segments = prefill_segments(ctas, tiles);
+  const dim3 grid((unsigned)((max_q_len + tokens_per_cta - 1) / tokens_per_cta) * nkv * segments, count);
   int page_shift = -1;
   if ((page_size & (page_size - 1)) == 0)
     for (page_shift = 0; (1 << page_shift) < page_size; ++page_shift) {}
-#define LAUNCH_PREFILL_TC_E4M3(D)                                                                                     \
+#define LAUNCH_PREFILL_TC_E4M3(D, CUT)                                                                                \
   do {                                                                                                                \
-    auto kernel = attention_prefill_tc_kernel<D, false, false, false, E4m3Side>;                                      \
-    const cudaError_t raised =                                                                                        \
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prefill_tc_smem_bytes<D>());   \
+    auto kernel = attention_prefill_tc_kernel<D, false, false, false, E4m3Side<CUT>>;                                 \
+    const E4m3Side<CUT> keys = {(const uint8_t*)k, (const uint8_t*)k_scale, segments};                                \
+    const E4m3Side<CUT> values = {(const uint8_t*)v, (const uint8_t*)v_scale, segments};                              \
+    const size_t smem = prefill_tc_smem_bytes<D>();                                                                   \
+    const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  \
     VOSTI_REQUIRE(raised == cudaSuccess, "attention_prefill_tc_e4m3: %s", cudaGetErrorString(raised));                \
-    vosti_launch(kernel, grid, dim3(THREADS), prefill_tc_smem_bytes<D>(), stream, map_q, keys, values, (bf16*)out,    \
-                 row_list, cu_q, kv_len, block_table, max_pages, page_size, page_shift, num_pages, nq, nkv,           \
-                 scale * LOG2E, window, nullptr, 0, nullptr, 0.f, nullptr, status);                                   \
+    auto launch = [&](auto... args) {                                                                                 \
+      return CUT ? vosti_launch_clusters(kernel, grid, dim3(THREADS), (unsigned)segments, smem, stream, args...)      \
+                 : vosti_launch(kernel, grid, dim3(THREADS), smem, stream, args...);                                  \
+    };                                                                                                                \
+    const cudaError_t e =                                                                                             \
+        launch(map_q, keys, values, (bf16*)out, row_list, cu_q, kv_len, block_table, max_pages, page_size, page_shift, \
+               num_pages, nq, nkv, scale * LOG2E, window, (const float*)nullptr, 0, (const float*)nullptr, 0.f,       \
+               (const float*)nullptr, status);                                                                        \
+    VOSTI_REQUIRE(e == cudaSuccess, "attention_prefill_tc_e4m3: %s", cudaGetErrorString(e));                          \
   } while (0)
-  if (d == 64) LAUNCH_PREFILL_TC_E4M3(64);
-  else LAUNCH_PREFILL_TC_E4M3(128);
+  if (segments > 1) {
+    if (d == 64) LAUNCH_PREFILL_TC_E4M3(64, true);
+    else LAUNCH_PREFILL_TC_E4M3(128, true);
+  } else {
+    if (d == 64) LAUNCH_PREFILL_TC_E4M3(64, false);
+    else LAUNCH_PREFILL_TC_E4M3(128, false);
+  }
 #undef LAUNCH_PREFILL_TC_E4M3
   VOSTI_LAUNCH_CHECK();
 }

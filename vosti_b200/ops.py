@@ -2430,7 +2430,7 @@ def qkv_post_e4m3(qkv, cache: PagedE4M3, *, nq: int, nkv: int, head_dim: int, sl
 def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nkv: int, head_dim: int, scale: float, window: int = 0,
                    appended: int = 0) -> torch.Tensor:
     """`attention` over a cache of 8 bits: every query row of the step over its request's keys, causal, the last `window` of them if
-    that is not 0. bfloat16 with heads of 64 or 128: single tokens on a kernel that cuts the keys into segments, portions on the tcgen05 kernel;
+    that is not 0. bfloat16 with heads of 64 or 128: single tokens on a kernel that cuts the keys into segments, portions on the tcgen05 kernel, their keys in segments too where rows are few;
     everything else on the CUDA cores in float32. `appended` > 0 says that the kernel launched right before is the step's own
     `qkv_post_e4m3`, which stored at most that many of each request's newest tokens: what lies before them is then read
     while it still runs. 0: nothing is known of it."""
@@ -2464,9 +2464,9 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
         rows = ctx.extras.get("attention.long_rows")
         _ints("attention_e4m3", long_rows, cu_q=ctx.cu_q, kv_len=ctx.kv_len, **({} if rows is None else {"long_rows": rows}))
         _here("attention_e4m3", rows, ctx.cu_q, ctx.kv_len)
-        _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iifipp")(
+        _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iiifipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
-            lists["max_long_q_len"], tokens, scale, window, status.data_ptr(), stream), "attention_prefill_tc_e4m3")
+            lists["max_long_q_len"], tokens, ctx.max_kv_len, scale, window, status.data_ptr(), stream), "attention_prefill_tc_e4m3")
     if count:
         # (beside the portions' kernel, whose last CTAs leave SMs free)
         if short is not None:
