@@ -134,3 +134,36 @@ def test_calls_that_are_refused():
         with pytest.raises(ops.KernelError):
             ops.gemm_int4(x, w, bad)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 64, 130, 300])
+@pytest.mark.parametrize("inter,k,group", [(16, 128, 128), (48, 200, 32), (1040, 512, 64), (12288, 1024, 128), (320, 4096, 32)])
+def test_gated_products(rows, inter, k, group):
+    """silu(gate) * up of blocks of 16 rows each. silu(g) moves by 1.1 times what g is off by at most, exp by (2 + 1.16 |g|) 2^-23 of itself and the
+    division and products by 2^-23."""
+    w, numbers, gen = weight(2 * inter, k, group)
+    x = torch.randn(rows, k, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    sums = x.double() @ numbers.T
+    off = (k + 8) * 2.0 ** -24 * (x.double().abs() @ numbers.abs().T) + (2.0 ** -8 * (x.double().abs() @ numbers.abs().T) if rows > 16 else 0)
+    (g, u), (dg, du) = (m.view(rows, inter // 16, 2, 16).permute(2, 0, 1, 3).reshape(2, rows, inter) for m in (sums, off))
+    want = g * torch.sigmoid(g) * u
+    for kind in (torch.bfloat16, torch.float32):
+        y = ops.gemm_int4(x.to(DEVICE), w, status, out_dtype=kind, swiglu=True)
+        assert int(status) == 0 and y.dtype == kind and tuple(y.shape) == (rows, inter)
+        exact = (5 + 1.16 * g.abs()) * 2.0 ** -23 * want.abs() + 1.1 * dg * (u.abs() + du) + (g * torch.sigmoid(g)).abs() * du
+        bound = exact + (2.0 ** -8 if kind == torch.bfloat16 else 2.0 ** -24) * (want.abs() + exact) + 1e-37
+        assert bool(((y.cpu().double() - want).abs() <= bound).all())
+
+
+def test_gated_products_that_are_refused():
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    for features, k in ((48, 128), (64, 100)):
+        w, _, _ = weight(features, k, 32)
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int4(torch.zeros(3, k, dtype=torch.bfloat16, device=DEVICE), w, status, swiglu=True)
+    w, _, _ = weight(64, 128, 32)
+    odd = torch.zeros(3 * 128 + 1, dtype=torch.bfloat16, device=DEVICE)[1:].view(3, 128)
+    with pytest.raises(ops.KernelError):
+        ops.gemm_int4(odd, w, status, swiglu=True)
+    assert tuple(ops.gemm_int4(odd[:0], w, status).shape) == (0, 64) and int(status) == 0

@@ -7,6 +7,9 @@
 // A word shifted by 4 p and masked holds the codes of neighbouring k in its halves; with the exponent of 128 or'ed in they are 128 + c + 8 in
 // bfloat16, exactly, and minus 136 the codes.
 //
+// Gated: tiles of 16 features are taken in pairs, a gate and what it is for, and Y[t, 16 p + i] = silu(gate) * up of pair p, in float32 (24,576 x 4,096,
+// us without and with it, and with a kernel of its own behind: 8 tokens 14.5, 14.5, 19.3, 64 25.6, 26.1, 33.7, 2,048 309, 350, 380 to 440).
+//
 // Up to 16 tokens: mma.sync, weights as the 16 rows (int4_few_kernel). What bounds it is the weights' bytes. More tokens: tcgen05
 // (int4_tiles_kernel), weights made bfloat16 in tensor memory.
 #include "common.cuh"
@@ -61,6 +64,8 @@ __device__ __forceinline__ void load_scales(const bf16* p, int left, uint32_t (&
       if (i * (KB / N) >= left) s[i / 2] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
   }
 }
+// (the quick division: a divisor beyond 2^126 gives 0, where silu is below 1e-36)
+__device__ __forceinline__ float int4_gated(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
 __device__ __forceinline__ float scale_of(uint32_t word, int i) { return __uint_as_float((i & 1) ? word & 0xffff0000u : word << 16); }
 
 // ---------------------------------------------------------------------------------------------- up to 16 tokens
@@ -69,7 +74,7 @@ __device__ __forceinline__ float scale_of(uint32_t word, int i) { return __uint_
 // SM some 190 KB are on their way from the start. The order of k inside an instruction is free: lane j of a row takes offsets 8 j .. 8 j + 7
 // of every 32 k, so that four of them are a word's half and the tokens' 8 are one 16-byte load. An instruction never mixes groups: a group's codes
 // are summed exactly, then multiplied by its scale in float32. The warps' sums meet in shared memory, in warp order.
-// What bounds it: with many tiles the integer pipe (seven operations at half rate for a word of eight codes: 8 tokens, 151,936 x 4,096 in 80 us, 62% of
+// What bounds it: with many tiles the integer pipe (seven operations at half rate for a word of eight codes: 8 tokens, 151,936 x 4,096 in 74 us, 66% of
 // its bytes' rate); with few the chain from launch to the last sum (4,096 x 4,096 5.2, 4,096 x 12,288 11.5 us; 13.3 when a block's addresses and the
 // tokens' bounds were worked out block by block).
 constexpr int FEW_WARPS = 8, FEW_THREADS = FEW_WARPS * 32;
@@ -93,7 +98,7 @@ __device__ __forceinline__ uint4 load_tokens(const bf16* row, int kk, int k) {
   }
 }
 
-template <int FT, int NT, int GROUPS, bool WORDS>
+template <int FT, int NT, int GROUPS, bool WORDS, bool GATED>
 __global__ void __launch_bounds__(FEW_THREADS, NT == 1 ? 3 : 2)
 int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y, int y_is_f32,
                 int rows, int n, int k, int tiles, int deep, unsigned* status) {
@@ -222,15 +227,28 @@ int4_few_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes, c
 #pragma unroll
       for (int e = 0; e < 4; ++e) sums[(warp * NT * 8 + t * 8 + 2 * j + (e & 1)) * PITCH + f * 16 + r8 + 8 * (e >> 1)] = acc[f][t][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * FT * 16; i += FEW_THREADS) {
-    const int t = i / (FT * 16), f = i % (FT * 16);
-    if (tile0 * 16 + f >= n) continue;
+  auto total = [&](int t, int f) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < FEW_WARPS; ++w) v += sums[(w * NT * 8 + t) * PITCH + f];
-    const int64_t at = (int64_t)t * n + tile0 * 16 + f;
+    return v;
+  };
+  auto store = [&](int64_t at, float v) {
     if (y_is_f32) reinterpret_cast<float*>(y)[at] = v;
     else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
+  };
+  int mine_at;                                                   // (read again here: worked out ahead, places spill registers in the main loop)
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(mine_at));
+  if constexpr (GATED) {
+    for (int i = mine_at; i < rows * FT * 8; i += FEW_THREADS) {
+      const int t = i / (FT * 8), f = i % (FT * 8), gate = f / 16 * 32 + f % 16;
+      if (tile0 * 8 + f < n / 2) store((int64_t)t * (n / 2) + tile0 * 8 + f, int4_gated(total(t, gate), total(t, gate + 16)));
+    }
+  } else {
+    for (int i = mine_at; i < rows * FT * 16; i += FEW_THREADS) {
+      const int t = i / (FT * 16), f = i % (FT * 16);
+      if (tile0 * 16 + f < n) store((int64_t)t * n + tile0 * 16 + f, total(t, f));
+    }
   }
 }
 
@@ -283,7 +301,7 @@ __device__ __forceinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatil
 template <int WORKERS>
 __device__ __forceinline__ void int4_workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
 
-template <int TOK, int GROUPS>
+template <int TOK, int GROUPS, bool GATED>
 __global__ void __launch_bounds__(Int4Tile<TOK>::THREADS, Int4Tile<TOK>::CTAS)
 int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ codes, const bf16* __restrict__ scales, void* __restrict__ y,
                   int y_is_f32, int rows, int n, int k, int tiles, int deep, int token_tiles, int segments, unsigned* status) {
@@ -427,10 +445,12 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   }
   tc_fence_before();
   // Four neighbouring features of a token at a time, so that a warp writes whole rows (each warp its 32 features: 64 bytes a store).
-  const bool quads = n % 4 == 0 && (uintptr_t)y % 16 == 0;
+  constexpr int WORDS = GATED ? FEATURES / 8 : FEATURES / 4;
+  const int wide = GATED ? n / 2 : n, first = GATED ? f0 / 2 : f0;
+  const bool quads = wide % 4 == 0 && (uintptr_t)y % 16 == 0;
   auto store = [&](int t, int f, const float4& v) {
-    if (f0 + f >= n) return;
-    const int64_t at = (int64_t)(t0 + t) * n + f0 + f;
+    if (first + f >= wide) return;
+    const int64_t at = (int64_t)(t0 + t) * wide + first + f;
     if (quads) {
       if (y_is_f32) store_four(reinterpret_cast<float*>(y) + at, v);
       else store_four(reinterpret_cast<bf16*>(y) + at, v);
@@ -439,42 +459,55 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
     const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (f0 + f + i >= n) return;
+      if (first + f + i >= wide) return;
       if (y_is_f32) reinterpret_cast<float*>(y)[at + i] = e[i];
       else reinterpret_cast<bf16*>(y)[at + i] = __float2bfloat16_rn(e[i]);
+    }
+  };
+  // (`total` sums four features of a token)
+  auto finish = [&](int t, int word, auto total) {
+    const int f = word * 4;
+    if constexpr (GATED) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f), gate = v;
+#pragma unroll 1                                                 // (both at once do not fit the registers)
+      for (int side = 0; side < 2; ++side) {
+        gate = v;
+        v = total(t, f / 16 * 32 + f % 16 + 16 * side);
+      }
+      store(t, f, make_float4(int4_gated(gate.x, v.x), int4_gated(gate.y, v.y), int4_gated(gate.z, v.z), int4_gated(gate.w, v.w)));
+    } else {
+      store(t, f, total(t, f));
     }
   };
   if (segments == 1) {
     int4_workers_sync<WORKERS>();
     const int count = min(TOK, rows - t0);
-    for (int word = threadIdx.x; word < count * (FEATURES / 4); word += WORKERS) {
-      const int t = word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
-      store(t, f, *reinterpret_cast<const float4*>(part + t * FEATURES + f));
-    }
+    for (int word = threadIdx.x; word < count * WORDS; word += WORKERS)
+      finish(word / WORDS, word % WORDS, [&](int t, int f) { return *reinterpret_cast<const float4*>(part + t * FEATURES + f); });
   } else {
     // the segments' sums in their order, each CTA a share of the tokens (the roles that bring and issue have ended: every thread of the cluster
     // that is left takes part)
     cluster_sync_all();
     const int lo = TOK * segment / segments, hi = min(TOK * (segment + 1) / segments, rows - t0);
-    for (int word = threadIdx.x; word < (hi - lo) * (FEATURES / 4); word += WORKERS) {
-      const int t = lo + word / (FEATURES / 4), f = word % (FEATURES / 4) * 4;
-      const uint32_t at = smem_u32(&part[t * FEATURES + f]);
-      // (all of them on their way at once: one after the other, eight took 4 us)
-      float4 u[MAX_SEGMENTS];
+    for (int word = threadIdx.x; word < (hi - lo) * WORDS; word += WORKERS)
+      finish(lo + word / WORDS, word % WORDS, [&](int t, int f) {
+        const uint32_t at = smem_u32(&part[t * FEATURES + f]);
+        // (all of them on their way at once: one after the other, eight took 4 us)
+        float4 u[MAX_SEGMENTS];
 #pragma unroll
-      for (int r = 0; r < MAX_SEGMENTS; ++r)
-        if (r < segments) u[r] = int4_load_rank(at, r);
-      float4 v = u[0];
+        for (int r = 0; r < MAX_SEGMENTS; ++r)
+          if (r < segments) u[r] = int4_load_rank(at, r);
+        float4 v = u[0];
 #pragma unroll
-      for (int r = 1; r < MAX_SEGMENTS; ++r)
-        if (r < segments) {
-          v.x += u[r].x;
-          v.y += u[r].y;
-          v.z += u[r].z;
-          v.w += u[r].w;
-        }
-      store(t, f, v);
-    }
+        for (int r = 1; r < MAX_SEGMENTS; ++r)
+          if (r < segments) {
+            v.x += u[r].x;
+            v.y += u[r].y;
+            v.z += u[r].z;
+            v.w += u[r].w;
+          }
+        return v;
+      });
     cluster_sync_all();                                          // nobody reads this CTA's sums after this
   }
   int4_workers_sync<WORKERS>();
@@ -501,14 +534,14 @@ struct Int4Args {
   const uint8_t* codes;
   const bf16* scales;
   void* y;
-  int y_is_f32, rows, n, k, tiles, deep;
+  int y_is_f32, gated, rows, n, k, tiles, deep;
   unsigned* status;
   cudaStream_t stream;
 };
 
-template <int FT, int NT, int GROUPS, bool WORDS>
+template <int FT, int NT, int GROUPS, bool WORDS, bool GATED = false>
 cudaError_t launch_few(const Int4Args& a) {
-  auto kernel = int4_few_kernel<FT, NT, GROUPS, WORDS>;
+  auto kernel = int4_few_kernel<FT, NT, GROUPS, WORDS, GATED>;
   constexpr int SMEM = FEW_WARPS * FEW_STAGES * stage_bytes<GROUPS>();
   static_assert(FEW_WARPS * NT * 8 * (FT * 16 + 4) * 4 <= SMEM, "the sums take the buffers' place");
   const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
@@ -516,9 +549,10 @@ cudaError_t launch_few(const Int4Args& a) {
   return vosti_launch(kernel, dim3((a.tiles + FT - 1) / FT), dim3(FEW_THREADS), SMEM, a.stream, a.x, a.codes, a.scales, a.y, a.y_is_f32, a.rows, a.n, a.k,
                       a.tiles, a.deep, a.status);
 }
-// Tiles of 16 features a CTA: as many as leave two CTAs an SM. us, 8 tokens, two and four of them: 24,576 x 4,096 18.7 and 15.9, 151,936 x 4,096 89 and 80.
+// Tiles of 16 features a CTA: as many as leave two CTAs an SM. us, 8 tokens, two and four of them: 24,576 x 4,096 18.7 and 14.8, 151,936 x 4,096 89 and 74.
 template <int GROUPS, int NT>
 cudaError_t launch_few_as(const Int4Args& a, bool words) {
+  if (a.gated) return a.tiles >= 4 * 296 ? launch_few<4, NT, GROUPS, true, true>(a) : launch_few<2, NT, GROUPS, true, true>(a);      // (tiles in pairs)
   if (!words) return launch_few<1, NT, GROUPS, false>(a);
   if (a.tiles >= 4 * 296) return launch_few<4, NT, GROUPS, true>(a);
   return a.tiles >= 2 * 296 ? launch_few<2, NT, GROUPS, true>(a) : launch_few<1, NT, GROUPS, true>(a);
@@ -530,7 +564,7 @@ cudaError_t launch_few_groups(const Int4Args& a, bool words) {
 
 template <int TOK, int GROUPS>
 int launch_tiles(const Int4Args& a) {
-  auto kernel = int4_tiles_kernel<TOK, GROUPS>;
+  auto kernel = a.gated ? int4_tiles_kernel<TOK, GROUPS, true> : int4_tiles_kernel<TOK, GROUPS, false>;
   constexpr int SMEM = Int4Tile<TOK>::SMEM;
   const cudaError_t raised = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   VOSTI_REQUIRE(raised == cudaSuccess, "gemm_int4: %s", cudaGetErrorString(raised));
@@ -568,16 +602,17 @@ VOSTI_API int vosti_gemm_int4_columns_an_sm(int tile) {
 }
 
 // x: bfloat16 [rows, k]; codes, scales: as at the top of this file, for n features and k, group 32, 64 or 128; y: [rows, n] bfloat16, or
-// float32 with y_is_f32.
-VOSTI_API int vosti_gemm_int4(const void* x, const void* codes, const void* scales, void* y, int y_is_f32, int rows, int n, int k, int group,
+// float32 with y_is_f32. `gated`: y [rows, n / 2], n a multiple of 32, k one of 8 and x on 16 bytes.
+VOSTI_API int vosti_gemm_int4(const void* x, const void* codes, const void* scales, void* y, int y_is_f32, int gated, int rows, int n, int k, int group,
                               unsigned* status, cudaStream_t stream) {
   VOSTI_REQUIRE(rows >= 0 && n > 0 && k > 0, "gemm_int4: bad sizes rows=%d n=%d k=%d", rows, n, k);
   VOSTI_REQUIRE(group == 32 || group == 64 || group == 128, "gemm_int4: the group is 32, 64 or 128, not %d", group);
   VOSTI_REQUIRE((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "gemm_int4: the weights must start on 16 bytes");
   if (rows == 0) return VOSTI_OK;
-  Int4Args a = {(const bf16*)x, (const uint8_t*)codes, (const bf16*)scales, y, y_is_f32, rows, n, k, (n + 15) / 16, (k + KB - 1) / KB, status, stream};
+  Int4Args a = {(const bf16*)x, (const uint8_t*)codes, (const bf16*)scales, y, y_is_f32, gated != 0, rows, n, k, (n + 15) / 16, (k + KB - 1) / KB, status, stream};
   // whole words of eight tokens' elements: every row starts on 16 bytes
   const bool words = k % 8 == 0 && ((uintptr_t)x & 15) == 0;
+  VOSTI_REQUIRE(!gated || (n % 32 == 0 && words), "gemm_int4: a gated product takes 32 features at a time and rows that start on 16 bytes");
   if (rows > 16 && words) {
     const int code = group == 32 ? launch_tiles_as<4>(a) : group == 64 ? launch_tiles_as<2>(a) : launch_tiles_as<1>(a);
     if (code != VOSTI_OK) return code;

@@ -2556,9 +2556,10 @@ class Int4Weight:
         return (codes * scales).reshape(tiles * 16, deep * 128)[:self.shape[0], :self.shape[1]].contiguous()
 
 
-def gemm_int4(x: torch.Tensor, w: Int4Weight, status: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+def gemm_int4(x: torch.Tensor, w: Int4Weight, status: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None, swiglu: bool = False) -> torch.Tensor:
     """y = x @ w.T for bfloat16 rows and a weight in 4 bits, rounded once to `out_dtype` (bfloat16 or float32). Up to 16 rows a group's codes
-    are summed exactly and scaled in float32; more rows multiply codes times scales rounded to bfloat16."""
+    are summed exactly and scaled in float32; more rows multiply codes times scales rounded to bfloat16. `swiglu`: w holds blocks of 16 gate rows
+    followed by their 16 up rows (features a multiple of 32, k of 8), and y [rows, features / 2] is silu(gate) * up, in float32 up to the one rounding."""
     features, k = w.shape
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != k:
         raise KernelError(f"gemm_int4: x is bfloat16 [rows, {k}], got {x.dtype} {tuple(x.shape)}")
@@ -2568,7 +2569,7 @@ def gemm_int4(x: torch.Tensor, w: Int4Weight, status: torch.Tensor, *, out_dtype
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"gemm_int4: the result is bfloat16 or float32, not {out_dtype}")
     stream = _here("gemm_int4", x, w.codes, status)
-    out = x.new_empty((rows, features), dtype=out_dtype)
-    _check(_bound("vosti_gemm_int4", "pppp" "iiiii" "pp")(x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), out_dtype == torch.float32,
-                                                          rows, features, k, w.group, status.data_ptr(), stream), "gemm_int4")
+    out = x.new_empty((rows, features // 2 if swiglu else features), dtype=out_dtype)
+    _check(_bound("vosti_gemm_int4", "pppp" "iiiiii" "pp")(x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), out_dtype == torch.float32,
+                                                           swiglu, rows, features, k, w.group, status.data_ptr(), stream), "gemm_int4")
     return out

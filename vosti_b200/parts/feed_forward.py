@@ -57,6 +57,8 @@ def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 def gated_activation(ctx, x, w_gate_up, fused: bool, activation: str = "silu", glu=(0.0, 0.0)):
+    if fused and isinstance(w_gate_up, ops.Int4Weight):
+        return ops.gemm_int4(ops.materialize(x), w_gate_up, ctx.status, swiglu=True)
     if fused:
         return ops.gemm_tc(ops.materialize(x), w_gate_up, ctx.status, swiglu=True, activation=activation)
     return ops.glu_mul(ops.materialize(linear(ctx, x, w_gate_up)), activation, *glu)
@@ -101,7 +103,10 @@ class SwiGLU(FeedForward):
         self.w_down = prepare_weight(tensors[down], dtype, self.weight_group)
         if self.weight_group:
             common = torch.float32 if torch.float32 in (tensors[gate].dtype, tensors[up].dtype) else tensors[gate].dtype
-            self.w_gate_up = prepare_weight(torch.cat([tensors[gate].to(common), tensors[up].to(common)]), dtype, self.weight_group)
+            pair = tensors[gate].to(common), tensors[up].to(common)
+            # as for 16 bits, in blocks of 16 rows where the product may apply the activation itself
+            self.fused = self.activation == "silu" and self.inter % 16 == 0 and self.hidden_size % 8 == 0
+            self.w_gate_up = prepare_weight(interleave_gate_up(*pair) if self.fused else torch.cat(pair), dtype, self.weight_group)
             return
         if self.has_bias:
             pair, biases = (tensors[gate], tensors[up]), (tensors[gate + ".b"].float(), tensors[up + ".b"].float())
