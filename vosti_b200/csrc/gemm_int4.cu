@@ -268,6 +268,13 @@ struct Int4Tile {
   // warps take a CTA's stages in turn (one CTA with two groups for 24,576 x 4,096 of 128 tokens: 38 us, two with one 32).
   static constexpr int GROUPS = TOK > 128 ? 2 : 1, DEPTH = 4, WORKERS = 256 * GROUPS, THREADS = WORKERS + 64;
   static constexpr int X_STAGE = TOK * KB * 2, STAGES = TOK > 128 ? 3 : TOK > 64 ? 2 : 3;
+  // A stage's MMAs are reported on a barrier that goes by the block, and whoever refills a stage waits for the block that held it. With as many
+  // barriers as stages and groups have a common multiple of, (1) a waiter's blocks meet a barrier's phases one after another, so that a parity
+  // never stands for an earlier phase, and (2) the phase after the awaited one takes the MMAs of a block behind the one that the waiter is about to
+  // fill, so that it never stands for a later one, however late the waiter looks.
+  static constexpr int REPORTS = STAGES % GROUPS == 0 ? STAGES : STAGES * GROUPS;
+  static __host__ __device__ constexpr int report(int block) { return block % REPORTS; }
+  static __host__ __device__ constexpr uint32_t report_parity(int block) { return (uint32_t)(block / REPORTS) & 1; }
   static constexpr int COLS = TOK + STAGES * A_COLS <= 256 ? 256 : 512;
   static constexpr int RING = STAGES * X_STAGE, SUMS = TOK * FEATURES * 4;
   // no more CTAs an SM than tensor memory has columns for: shared memory (228 KB, 1 KB of it with every CTA) is padded until that many fit
@@ -310,8 +317,8 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
   constexpr int COLS = TOK / (WORKERS / 128);                    // token columns of a warp at the end
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  // a stage: the tokens have arrived and eight warps have stored the weights; its MMAs are complete; all MMAs are
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], done;
+  // a stage: the tokens have arrived and eight warps have stored the weights; a block's MMAs are complete; all MMAs are
+  __shared__ __align__(8) uint64_t full[STAGES], empty[Tile::REPORTS], done;
   __shared__ uint32_t tmem_base_holder;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -321,10 +328,8 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full[s]), 9);
-      mbar_init(smem_u32(&empty[s]), 1);
-    }
+    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&full[s]), 9);
+    for (int r = 0; r < Tile::REPORTS; ++r) mbar_init(smem_u32(&empty[r]), 1);
     mbar_init(smem_u32(&done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -340,7 +345,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       pdl_wait();
       for (int b = 0; b < blocks; ++b) {
         const int s = b % STAGES;
-        if (b >= STAGES && !int4_wait(smem_u32(&empty[s]), (b / STAGES - 1) & 1, &abort_flag, status)) break;
+        if (b >= STAGES && !int4_wait(smem_u32(&empty[Tile::report(b - STAGES)]), Tile::report_parity(b - STAGES), &abort_flag, status)) break;
         mbar_expect_tx(smem_u32(&full[s]), (uint32_t)Tile::X_STAGE);
         for (int h = 0; h < 2; ++h)
           tma_load_2d(smem_u32(smem + s * Tile::X_STAGE + h * (TOK * 128)), &map_x, (kb_begin + b) * KB + h * 64, t0, smem_u32(&full[s]));
@@ -361,7 +366,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
 #pragma unroll
         for (int q = 0; q < KB / 16; ++q)
           umma_bf16_ts(tmem_sum, tmem_a + s * A_COLS + 8 * q, desc + (uint64_t)(((q >> 2) * (TOK * 128) + (q & 3) * 32) >> 4), idesc, b > 0 || q > 0);
-        umma_commit(smem_u32(&empty[s]));
+        umma_commit(smem_u32(&empty[Tile::report(b)]));
         if (b + 1 == blocks) umma_commit(smem_u32(&done));
       }
       __syncwarp();
@@ -395,11 +400,7 @@ int4_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __re
       const int b = b0 + d * TURNS, s = b % STAGES;
       if (b >= blocks || !ok) break;
       if (b >= STAGES) {
-        // Three stages come to the groups in turn: each waits for the other's block too, so that it has seen every phase of a stage in its
-        // order (a parity alone could stand for the phase before the last).
-        if (STAGES % TURNS != 0 && b > STAGES)
-          ok = __all_sync(0xffffffffu, int4_wait(smem_u32(&empty[(b - 1) % STAGES]), ((b - 1) / STAGES - 1) & 1, &abort_flag, status)) != 0;
-        ok = ok && __all_sync(0xffffffffu, int4_wait(smem_u32(&empty[s]), (b / STAGES - 1) & 1, &abort_flag, status)) != 0;
+        ok = __all_sync(0xffffffffu, int4_wait(smem_u32(&empty[Tile::report(b - STAGES)]), Tile::report_parity(b - STAGES), &abort_flag, status)) != 0;
         if (!ok) break;
         tc_fence_after();                                        // (the MMAs that read the stage)
       }
@@ -599,6 +600,23 @@ VOSTI_API int vosti_gemm_int4_columns_an_sm(int tile) {
     case 3: return of(Int4Tile<256>::SMEM, Int4Tile<256>::COLS);
   }
   return -1;
+}
+
+// What the roles of a token tile (0 .. 3) do about block `block`: out = {stages, groups of warps, barrier that reports its MMAs, barrier and parity
+// waited for before its stage is filled (barrier -1: none)}.
+VOSTI_API int vosti_gemm_int4_schedule(int tile, int block, int* out) {
+  auto of = [&](auto kind) {
+    using Tile = decltype(kind);
+    const int held = block - Tile::STAGES;
+    out[0] = Tile::STAGES;
+    out[1] = Tile::GROUPS;
+    out[2] = Tile::report(block);
+    out[3] = held >= 0 ? Tile::report(held) : -1;
+    out[4] = held >= 0 ? (int)Tile::report_parity(held) : 0;
+    return VOSTI_OK;
+  };
+  VOSTI_REQUIRE(block >= 0 && out != nullptr && tile >= 0 && tile <= 3, "gemm_int4: no such tile or block");
+  return tile == 0 ? of(Int4Tile<32>()) : tile == 1 ? of(Int4Tile<64>()) : tile == 2 ? of(Int4Tile<128>()) : of(Int4Tile<256>());
 }
 
 // x: bfloat16 [rows, k]; codes, scales: as at the top of this file, for n features and k, group 32, 64 or 128; y: [rows, n] bfloat16, or
