@@ -106,6 +106,26 @@ def test_store_rotations(rotary, neighbours, norm, dtype):
     store(cache, ctx, group, torch.randn(63, 8 * 64, generator=gen).to(dtype), nq=4, nkv=2, d=64, gen=gen, rotary=rotary, neighbours=neighbours, norm=norm)
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 15, 16])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64), (torch.bfloat16, 256), (torch.bfloat16, 80), (torch.float32, 16)])
+def test_store_of_a_norm_without_an_eps(n, dtype, d):
+    """A run's lanes without a token hold zeros, whose norm is no number at eps 0: they do not count. A token of zeros does."""
+    gen = torch.Generator().manual_seed(n + d)
+    ctx, group, pages = plain.step([n], [0], 16)
+    qkv = torch.randn(n, 4 * d, generator=gen).to(dtype)
+    caches = [plain.random_cache(pages, 1, 16, d, torch.Generator().manual_seed(3)) for _ in range(2)]
+    common = dict(nq=2, nkv=1, head_dim=d, k_norm_w=torch.ones(d, device=DEVICE), slot_mapping=group.slot_mapping, status=ctx.status)
+    for cache, eps in zip(caches, (0.0, 1e-12)):                          # (1e-12 beside a mean square near 1 is nothing in float32)
+        ops.qkv_post_e4m3(qkv.to(DEVICE), cache, eps=eps, **common)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(caches[0], name).view(torch.uint8), getattr(caches[1], name).view(torch.uint8)), name
+    at = int(group.block_table[0, 0])
+    assert int(caches[0].k_scale.view(torch.uint8)[at, 0, 0]) != 255
+    qkv[-1, 2 * d:3 * d] = 0
+    ops.qkv_post_e4m3(qkv.to(DEVICE), caches[0], eps=0.0, **common)
+    assert int(caches[0].k_scale.view(torch.uint8)[at, 0, 0]) == 255 and int(ctx.status) == 0
+
+
 @pytest.mark.parametrize("splits", [1, 3, 7])
 @pytest.mark.parametrize("d", [64, 96, 128])
 def test_store_of_unsummed_products(splits, d):

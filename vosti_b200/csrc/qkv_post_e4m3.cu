@@ -206,9 +206,10 @@ __device__ __forceinline__ void load_turn(const PostArgs& a, int pos, int sub, f
   }
 }
 
-// All lanes of the warp take part: a head's sum of squares runs over its lanes.
+// All lanes of the warp take part: a head's sum of squares runs over its lanes. Lanes without `live` hold zeros and keep them (a norm without an
+// eps would make them no numbers, and with them the largest size of the run).
 template <typename L>
-__device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, float (&x)[L::PAIRS], float (&y)[L::PAIRS], const float (&wx)[L::PAIRS],
+__device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, bool live, float (&x)[L::PAIRS], float (&y)[L::PAIRS], const float (&wx)[L::PAIRS],
                                               const float (&wy)[L::PAIRS], const float (&c)[L::PAIRS], const float (&s)[L::PAIRS]) {
   if (normed) {
     float ss = 0.f;
@@ -216,7 +217,7 @@ __device__ __forceinline__ void norm_and_turn(const PostArgs& a, bool normed, fl
     for (int j = 0; j < L::PAIRS; ++j) ss = fmaf(x[j], x[j], fmaf(y[j], y[j], ss));
 #pragma unroll
     for (int o = 1; o < L::LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(fmaf(ss, a.inverse_d, a.eps));
+    const float r = live ? rsqrtf(fmaf(ss, a.inverse_d, a.eps)) : 0.f;
 #pragma unroll
     for (int j = 0; j < L::PAIRS; ++j) {
       x[j] *= r * wx[j];
@@ -317,7 +318,7 @@ __device__ __forceinline__ void store_run(const PostArgs& a, int t0, int g, uint
   for (int i = 0; i < ROUNDS; ++i) {
     if (i * STEP >= n) break;                                    // (the same in all lanes)
     if (!VALUES) {
-      norm_and_turn<L>(a, a.k_norm_w != nullptr, x[i], y[i], wx, wy, c[i], s[i]);
+      norm_and_turn<L>(a, a.k_norm_w != nullptr, live[i], x[i], y[i], wx, wy, c[i], s[i]);
     }
 #pragma unroll
     for (int j = 0; j < L::PAIRS; ++j) most = larger(larger(most, x[i][j]), y[i][j]);
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, Q_ITEMS > 1 && L::LANES * L::PAIRS <=
     load_heads<T, L, Q_ITEMS>(a, at, live, sub, x, y);
     load_turn<L>(a, pos, sub, c, s);                             // (behind the heads: the position has arrived by now)
 #pragma unroll
-    for (int i = 0; i < Q_ITEMS; ++i) norm_and_turn<L>(a, a.q_norm_w != nullptr, x[i], y[i], wx, wy, c, s);
+    for (int i = 0; i < Q_ITEMS; ++i) norm_and_turn<L>(a, a.q_norm_w != nullptr, true, x[i], y[i], wx, wy, c, s);
 #pragma unroll
     for (int i = 0; i < Q_ITEMS; ++i)
       if (live[i]) store_head<T, L>(a, reinterpret_cast<T*>(a.q_out) + out + (int64_t)(h0 + i * L::HEADS) * a.d, sub, x[i], y[i]);
