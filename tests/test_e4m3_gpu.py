@@ -357,6 +357,30 @@ def test_a_block_that_is_no_number_reaches_only_who_sees_it(new, past, side, d, 
         check_attention(q, cache, ctx, group, out, nq=2, nkv=1, d=d, window=window, scale=d ** -0.5)
 
 
+@pytest.mark.parametrize("new,past", [([1] * 4, [10, 33, 40, 200]), ([60], [0]), ([50, 1], [20, 40]), ([70], [1400])])
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("byte", [0x7f, 0xff])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32)])
+def test_a_payload_that_is_no_number_reaches_only_who_sees_it(new, past, side, byte, d, dtype):
+    """One of a key makes the rows that see it no numbers, one of a value their feature at least; the same for single tokens, portions and the CUDA cores."""
+    gen = torch.Generator().manual_seed(5)
+    ctx, group, pages = plain.step(new, past, 16)
+    cache = plain.random_cache(pages, 1, 16, d, gen)
+    for r, total in enumerate(ctx.host_kv_lens):
+        for token, feature in ((33, 7), (45, d - 1)):
+            if total > token:
+                page, place = int(group.block_table[r, token // 16]), token % 16
+                at = (page, 0, place, feature) if side == "k" else (page, 0, 0, feature, place)
+                getattr(cache, side).view(torch.uint8)[at] = byte
+    for window in (0, 5, 8):
+        q = torch.randn(sum(new), 2 * d, generator=gen).to(dtype).to(DEVICE)
+        out = ops.attention_e4m3(ctx, q, cache, group, nq=2, nkv=1, head_dim=d, scale=d ** -0.5, window=window)
+        heads = out.view(-1, 2, d)
+        if side == "v":                                   # the rest of such a row is a number or none
+            heads = torch.where(heads[..., [7, d - 1]].isnan().any(-1, keepdim=True), torch.nan, heads)
+        check_attention(q, cache, ctx, group, heads.reshape(out.shape), nq=2, nkv=1, d=d, window=window, scale=d ** -0.5)
+
+
 def test_pages_beyond_the_pool_are_reported():
     gen = torch.Generator().manual_seed(6)
     for new, past, dtype in (([1], [100], torch.bfloat16), ([40], [60], torch.bfloat16), ([1], [100], torch.float32)):

@@ -423,18 +423,21 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     uint32_t edges = 0;
     if constexpr (EIGHT) {
       constexpr int UNITS = D / 32;                      // 16-byte pieces of a block's keys, or values, that a lane moves
+      auto block_of = [&](int key) {                     // the cache's block that begins with the key, -1 where no page holds it
+        const int index = page_shift >= 0 ? key >> page_shift : key / page_size;
+        const int page = index < max_pages ? table[index] : -1;
+        return page < 0 || page >= num_pages ? (int64_t)-1 : ((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (key - index * page_size) / GROUP_KEYS;
+      };
       for (int j = 0; j < tiles && ok; ++j) {
         const int stage = j % STAGES;
         const int lo = tile_key(j) + w * GROUP_KEYS;
         uint4 piece[2][UNITS];
         int k_scale = 0, v_scale = 0, seen = 0;          // tokens of the block before the last visible one's end
         if (lo + GROUP_KEYS - 1 >= first_key && lo < key_end) {
-          const int index = page_shift >= 0 ? lo >> page_shift : lo / page_size;
-          const int page = index < max_pages ? table[index] : -1;
-          if (page < 0 || page >= num_pages) {
+          const int64_t block = block_of(lo);
+          if (block < 0) {
             raise_fault(status, VOSTI_FAULT_PAGE_RANGE);
           } else {
-            const int64_t block = ((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (lo - index * page_size) / GROUP_KEYS;
             seen = min(GROUP_KEYS, key_end - lo);
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
@@ -451,6 +454,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         // value would meet weights of zero in rows that do not see it.
         const bool none = k_scale == E4M3_NAN_SCALE || v_scale == E4M3_NAN_SCALE;
         uint8_t* const kd = kv_s + stage * STAGE_BYTES;
+        uint32_t wrong = 0;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
           const E4m3Factor f = e4m3_factor(side == 0 ? (none ? E4M3_NAN_SCALE : k_scale) : none ? 0 : v_scale);
@@ -465,6 +469,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
               v.z &= e4m3_first_bytes(seen - 8);
               v.w &= e4m3_first_bytes(seen - 12);
             }
+            wrong |= e4m3_no_numbers(v.x);
+            wrong |= e4m3_no_numbers(v.y);
+            wrong |= e4m3_no_numbers(v.z);
+            wrong |= e4m3_no_numbers(v.w);
             uint4 lower = make_uint4(e4m3_widen<0>(v.x, f), e4m3_widen<1>(v.x, f), e4m3_widen<0>(v.y, f), e4m3_widen<1>(v.y, f));
             uint4 upper = make_uint4(e4m3_widen<0>(v.z, f), e4m3_widen<1>(v.z, f), e4m3_widen<0>(v.w, f), e4m3_widen<1>(v.w, f));
             if (f.second != E4M3_ONE) {
@@ -476,6 +484,28 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             *reinterpret_cast<uint4*>(dst + swizzled(row, (at & 3) * 2)) = lower;
             *reinterpret_cast<uint4*>(dst + swizzled(row, (at & 3) * 2 + 1)) = upper;
           }
+        }
+        if (__any_sync(0xffffffffu, (wrong & E4M3_NO_NUMBERS) != 0)) {
+          // Payloads that are no numbers, read again (few caches hold any). A key's makes its score none, as its block's scale does; a value's becomes
+          // zero, and its token's key is none. (Places are worked out again too: kept for this, they spill registers of the loop.)
+          int key, me;
+          asm volatile("mov.u32 %0, %2;\n\tmov.u32 %1, %%laneid;" : "=r"(key), "=r"(me) : "r"(lo));
+          const int64_t at = block_of(key) * (GROUP_KEYS * D);
+          uint32_t tokens = 0;                           // of the block that are no numbers, bit by bit
+          __syncwarp();                                  // (every lane's pieces are in their places)
+#pragma unroll 1
+          for (int u = 4 * me; u < GROUP_KEYS * D && at >= 0; u += 128) {
+            const uint32_t of_key = *reinterpret_cast<const uint32_t*>(map_k.payload + at + u), of_values = *reinterpret_cast<const uint32_t*>(map_v.payload + at + u);
+            if ((e4m3_no_numbers(of_key) & E4M3_NO_NUMBERS) != 0) tokens |= 1u << (u / D);
+#pragma unroll 1
+            for (int token = u % GROUP_KEYS, bytes = e4m3_no_numbers(of_values) & E4M3_NO_NUMBERS; bytes != 0; ++token, bytes = (unsigned)bytes >> 8)
+              if ((bytes & 0x80) != 0) {
+                tokens |= 1u << token;
+                *reinterpret_cast<uint16_t*>(kd + K_BYTES + swizzled(u / GROUP_KEYS, w * 2 + (token >> 3)) + token % 8 * 2) = 0;
+              }
+          }
+          tokens = __reduce_or_sync(0xffffffffu, tokens);
+          if (me < GROUP_KEYS && (tokens >> me & 1u) != 0) *reinterpret_cast<uint32_t*>(kd + swizzled(w * GROUP_KEYS + me, 0)) = 0x7fff7fffu;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();

@@ -5,7 +5,7 @@
 //   scales    [pages, kv heads, page / 16]             one byte each, keys and values
 // Feature-major values are what a matrix instruction wants of the weights' product (its k index, the token, runs along a
 // lane's word); the writer turns a block once, readers would have to turn it at every step.
-// (One is also where a size of 2^96 or more was to be held.)
+// (One is also where a size of 2^96 or more was to be held.) The payloads 0x7f and 0xff are no numbers either; a store leaves them in such blocks only.
 // A power of two as the scale costs e4m3 nothing (its own exponent moves), makes what is held exact in bfloat16, and lets a
 // block take a larger scale by moving exponents: only values that fall below e4m3's 2^-6 are rounded a second time.
 #pragma once
@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t bf16x2_times(uint32_t a, uint32_t b) {
   return r;
 }
 // A payload's bits moved into bfloat16's places stand for its value times 2^-120 (the formats' exponents are biased by 7 and 127), its
-// subnormals included. The block's factor is 2^120 * 2^(scale - 127); what of it is above bfloat16's range is a second one.
+// subnormals included (0x7f and 0xff come out as 480 and have to be looked for). The block's factor is 2^120 * 2^(scale - 127); what of it is above bfloat16's range is a second one.
 struct E4m3Factor { uint32_t first, second; };
 constexpr uint32_t E4M3_ONE = 0x3f803f80u;
 __device__ __forceinline__ E4m3Factor e4m3_factor(int scale) {
@@ -59,11 +59,15 @@ __device__ __forceinline__ E4m3Factor e4m3_factor(int scale) {
   const int e = scale - 7, lo = e < 127 ? e : 127;             // e: -7 .. 247
   return {(uint32_t)((lo + 127) << 7) * 0x10001u, (uint32_t)((e - lo + 127) << 7) * 0x10001u};
 }
-// Payload bytes 2 I and 2 I + 1 of a word, times the first factor.
+// Payload bytes 2 I and 2 I + 1 of a word, times the first factor (each byte with copies of its sign above it, moved up: sign, zeros, exponent, mantissa).
 template <int I>
 __device__ __forceinline__ uint32_t e4m3_widen(uint32_t w, const E4m3Factor& f) {
-  const uint32_t x = __byte_perm(w, 0, I == 0 ? 0x1404 : 0x3424);
-  return bf16x2_times((x & 0x80008000u) | ((x >> 4) & 0x07f007f0u), f.first);
+  uint32_t x;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(x) : "r"(w), "n"(I == 0 ? 0x9180 : 0xb3a2));
+  return bf16x2_times((x << 4) & 0x87f087f0u, f.first);
 }
+// Bit 7 of every byte of a word that is no number's payload, and other bits of no meaning.
+constexpr uint32_t E4M3_NO_NUMBERS = 0x80808080u;
+__device__ __forceinline__ uint32_t e4m3_no_numbers(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
 // A mask of the first n bytes of a word (n <= 0: none, n >= 4: all).
 __device__ __forceinline__ uint32_t e4m3_first_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u; }
