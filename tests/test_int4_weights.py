@@ -55,3 +55,31 @@ def test_refusals():
                 (good.codes, good.scales.expand(1, 1, 16, 3).contiguous(), good.shape)):
         with pytest.raises(ops.KernelError):
             ops.Int4Weight(*bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_codes_of_other_quantizers(dtype):
+    """Codes beyond -8 .. 7 would stand for others and reach into their neighbours' nibbles: refused, whatever their type."""
+    scales = torch.ones(16, 1)
+    for bad in (8, 15, 255, -9, -248, 2 ** 32):
+        info = torch.iinfo(dtype)
+        if info.min <= bad <= info.max:
+            codes = torch.zeros(16, 128, dtype=dtype)
+            codes[3, 77] = bad
+            with pytest.raises(ops.KernelError, match="-8 .. 7"):
+                ops.Int4Weight.from_codes(codes, scales, 128)
+    codes = (torch.arange(16 * 128).view(16, 128) % 16).to(dtype) % 8
+    assert torch.equal(ops.Int4Weight.from_codes(codes, scales, 128).dequantized(), codes.float())
+
+
+def test_scales_and_types_that_are_refused():
+    codes = torch.zeros(16, 128, dtype=torch.int8)
+    for bad in (float("nan"), float("inf"), 3.4e38):               # (the last is infinite in bfloat16)
+        scales = torch.ones(16, 1)
+        scales[5] = bad
+        with pytest.raises(ops.KernelError, match="finite"):
+            ops.Int4Weight.from_codes(codes, scales, 128)
+    for args in ((codes.bool(), torch.ones(16, 1)), (codes, torch.ones(16, 1, dtype=torch.int32)), (codes[:0], torch.ones(0, 1)), (codes[:, :0], torch.ones(16, 0)),
+                 (codes.to(torch.complex64), torch.ones(16, 1))):
+        with pytest.raises(ops.KernelError):
+            ops.Int4Weight.from_codes(*args, 128)

@@ -2517,10 +2517,18 @@ class Int4Weight:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, group: int) -> "Int4Weight":
-        """From integer codes [features, k] in -8 .. 7 and scales [features, k / group] (rounded up), which become bfloat16."""
+        """From integer codes [features, k] in -8 .. 7 and finite scales [features, k / group] (rounded up), which become bfloat16. Both are looked
+        over, so on a GPU the call waits for it."""
         cls.check_group(group)
-        if codes.dim() != 2 or codes.dtype.is_floating_point or tuple(scales.shape) != (codes.shape[0], -(-codes.shape[1] // group)):
-            raise KernelError(f"Int4Weight: integer codes [features, k] and scales [features, k / {group}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.dim() != 2 or codes.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64) or codes.numel() == 0 \
+                or not scales.dtype.is_floating_point or tuple(scales.shape) != (codes.shape[0], -(-codes.shape[1] // group)):
+            raise KernelError(f"Int4Weight: integer codes [features, k] and scales [features, k / {group}], got {codes.dtype} {tuple(codes.shape)} and "
+                              f"{scales.dtype} {tuple(scales.shape)}")
+        if codes.device != scales.device:
+            raise KernelError("Int4Weight: codes and scales are on one device")
+        low, high = (int(v) for v in codes.aminmax())
+        if low < -8 or high > 7:
+            raise KernelError(f"Int4Weight: codes are -8 .. 7, got {low} .. {high} (codes 0 .. 15 about a zero of 8 become these by subtracting it)")
         features, k = codes.shape
         tiles, deep = -(-features // 16), -(-k // 128)
         padded = torch.full((tiles * 16, deep * 128), 8, dtype=torch.uint8, device=codes.device)
@@ -2532,6 +2540,8 @@ class Int4Weight:
         groups = 128 // group
         wide = torch.zeros((tiles * 16, deep * groups), dtype=torch.bfloat16, device=codes.device)
         wide[:features, :scales.shape[1]] = scales.to(torch.bfloat16)
+        if not bool(torch.isfinite(wide).all()):
+            raise KernelError("Int4Weight: scales that are not finite in bfloat16")
         return cls(packed, wide.view(tiles, 16, deep, groups).transpose(1, 2).contiguous(), (features, k))
 
     @classmethod
