@@ -504,6 +504,25 @@ def test_tokens_of_a_block_one_after_another(d, count):
     assert all(torch.equal(a, b) for a, b in zip(*kept)) and int(ctx.status) == 0
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64), (torch.bfloat16, 96)])
+def test_a_step_without_tokens(dtype, d):
+    ctx, group, pages = plain.step([3], [20], 16)
+    cache = plain.random_cache(pages, 2, 16, d, torch.Generator().manual_seed(1))
+    before = [getattr(cache, n).view(torch.uint8).clone() for n in ("k", "v", "k_scale", "v_scale")]
+    sizes = dict(nq=4, nkv=2, head_dim=d)
+    none = torch.zeros(0, dtype=torch.int32, device=DEVICE)
+    cos, sin = (t.to(DEVICE) for t in tables(8, d))
+    q = ops.qkv_post_e4m3(torch.zeros(0, 8 * d, dtype=dtype, device=DEVICE), cache, slot_mapping=none, positions=none, cos=cos, sin=sin, status=ctx.status, **sizes)
+    assert tuple(q.shape) == (0, 4 * d) and q.dtype == dtype
+    ctx.positions = ctx.request_of = none
+    ctx.layout = {"attention": ops.attention_step_layout([])[1]}
+    for table in (group.block_table, group.block_table[:0]):
+        group.block_table = table
+        out = ops.attention_e4m3(ctx, q, cache, group, scale=0.1, **sizes)
+        assert tuple(out.shape) == (0, 4 * d) and out.dtype == dtype
+    assert all(torch.equal(a, getattr(cache, n).view(torch.uint8)) for a, n in zip(before, ("k", "v", "k_scale", "v_scale"))) and int(ctx.status) == 0
+
+
 def test_calls_that_are_refused():
     ctx, group, pages = plain.step([2, 40], [5, 0], 16)
     cache = ops.PagedE4M3.zeros(pages, 2, 16, 64)

@@ -696,10 +696,10 @@ VOSTI_API int vosti_attention_e4m3_simt(const void* q, const void* k, const void
                                         const int* positions, const int* request_of, const int* block_table, int max_pages, int page_size,
                                         int num_pages, int nq, int nkv, int d, float scale, int window, int is_f32, unsigned* status,
                                         cudaStream_t stream) {
-  if (int bad = check_cache(k, v, k_scale, v_scale, block_table, max_pages, page_size, num_pages, nq, nkv, scale, window)) return bad;
-  VOSTI_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "attention_e4m3: head_dim %d must be a multiple of 16, at most 256", d);
   VOSTI_REQUIRE(tokens >= 0 && nq <= 65535, "attention_e4m3: bad sizes");
-  if (tokens == 0) return VOSTI_OK;
+  VOSTI_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "attention_e4m3: head_dim %d must be a multiple of 16, at most 256", d);
+  if (tokens == 0) return VOSTI_OK;                              // (arrays of nothing are null)
+  if (int bad = check_cache(k, v, k_scale, v_scale, block_table, max_pages, page_size, num_pages, nq, nkv, scale, window)) return bad;
   const CacheArgs c = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, max_pages, page_size, num_pages};
   const dim3 grid(tokens, nq);
   const cudaError_t e = is_f32 ? vosti_launch(attention_e4m3_simt_kernel<float>, grid, dim3(SIMT_THREADS), 0, stream, (const float*)q, (float*)out, c, positions,

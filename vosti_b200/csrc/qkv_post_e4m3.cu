@@ -542,6 +542,7 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
   VOSTI_REQUIRE(tokens >= 0 && nq > 0 && nkv > 0, "qkv_post_e4m3: bad sizes");
   VOSTI_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "qkv_post_e4m3: head_dim %d must be a multiple of 16, at most 256", d);
   VOSTI_REQUIRE(page_size > 0 && page_size % E4M3_BLOCK == 0, "qkv_post_e4m3: page_size %d must be a multiple of 16", page_size);
+  if (tokens == 0) return VOSTI_OK;                              // (arrays of nothing are null)
   VOSTI_REQUIRE((qkv != nullptr) != (partial != nullptr), "qkv_post_e4m3: give the projection or its partial sums");
   VOSTI_REQUIRE(partial == nullptr || splits >= 1, "qkv_post_e4m3: bad split count");
   VOSTI_REQUIRE(num_slots >= 0 && num_slots <= 0x7fffffff, "qkv_post_e4m3: a cache of %lld slots is too large", (long long)num_slots);
@@ -551,7 +552,6 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
                 "qkv_post_e4m3: rotary_dim %d must be even and between 2 and head_dim %d", rotary_dim, d);
   VOSTI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qkv_post_e4m3: the cache must start on 16 bytes");
   VOSTI_REQUIRE(slot_mapping != nullptr && k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr, "qkv_post_e4m3: the cache is missing");
-  if (tokens == 0) return VOSTI_OK;
   VOSTI_REQUIRE((int64_t)tokens * (nq + 2 * nkv) <= 0x7fffffff - 4096, "qkv_post_e4m3: too many tokens and heads for one launch");
   // Neighbouring tokens whose runs a CTA takes: few tokens one, so that none waits for another's run; more of them four, a run a warp in a batch of
   // single tokens; many, as prompts bring them, eight or sixteen, which hold a run or two. us with tiles of 1, 4, 8, 16 (8B sizes): 8 single tokens 3.3, 3.5, 5.2,
