@@ -555,3 +555,22 @@ def test_calls_that_are_refused():
             ops.attention_e4m3(ctx, q, cache, group, **good)
         setattr(owner, name, kept)
     assert int(ctx.status) == 0
+
+
+def test_arrays_with_too_few_requests_are_refused():
+    """Portions read where the request behind theirs begins; nothing is launched on shorter arrays."""
+    for new in ([5, 40], [2, 40], [40, 2]):
+        ctx, group, pages = plain.step(new, [5, 0], 16)
+        cache = plain.random_cache(pages, 1, 16, 64, torch.Generator().manual_seed(1))
+        q = torch.zeros(sum(new), 2 * 64, dtype=torch.bfloat16, device=DEVICE)
+        sizes = dict(nq=2, nkv=1, head_dim=64, scale=0.1)
+        ops.attention_e4m3(ctx, q, cache, group, **sizes)
+        for owner, name, bad in ((ctx, "cu_q", ctx.cu_q[:-1]), (ctx, "kv_len", ctx.kv_len[:-1]), (group, "block_table", group.block_table[:-1]),
+                                 (ctx, "layout", {"attention": {**ctx.layout["attention"], "num_long_rows": 3}}),
+                                 (ctx, "layout", {"attention": {**ctx.layout["attention"], "num_short_tokens": sum(new) + 1}}), (ctx, "num_tokens", sum(new) + 1)):
+            kept = getattr(owner, name)
+            setattr(owner, name, bad)
+            with pytest.raises(ops.KernelError):
+                ops.attention_e4m3(ctx, q, cache, group, **sizes)
+            setattr(owner, name, kept)
+        assert int(ctx.status) == 0

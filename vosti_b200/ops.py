@@ -2441,11 +2441,14 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
     if nq <= 0 or nkv <= 0 or nq % nkv or cache.heads != nkv or cache.head_dim != head_dim or group.page_size != cache.page_size:
         raise KernelError("attention_e4m3: head counts, page size and cache do not match")
     table, status = group.block_table, ctx.status
-    if table.dim() != 2 or table.dtype != torch.int32:
-        raise KernelError("attention_e4m3: the block table is int32 [requests, pages]")
+    tokens = q.shape[0]
+    requests = ctx.num_requests if tokens else 0
+    if tokens not in (0, ctx.num_tokens):
+        raise KernelError(f"attention_e4m3: {tokens} queries of a step of {ctx.num_tokens} tokens")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] < requests:
+        raise KernelError(f"attention_e4m3: the block table is int32 [requests, pages] of {requests} requests, got {table.dtype} {tuple(table.shape)}")
     if window < 0 or appended < 0 or not scale > 0:
         raise KernelError("attention_e4m3: the score scale must be positive, the window and the appended tokens not negative")
-    tokens = q.shape[0]
     _ints("attention_e4m3", tokens, positions=ctx.positions, request_of=ctx.request_of)
     _ints("attention_e4m3", 1, status=status)
     stream = _here("attention_e4m3", q, cache.k, ctx.positions, ctx.request_of, table, status)
@@ -2462,9 +2465,14 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
         count, long_rows, short = tokens, 0, None
     else:
         short = ctx.extras.get("attention.short_tokens")
+    if count > tokens or long_rows > requests:
+        raise KernelError(f"attention_e4m3: the step's layout names {count} single tokens and {long_rows} portions, it has {tokens} tokens of {requests} requests")
     if long_rows:
         rows = ctx.extras.get("attention.long_rows")
-        _ints("attention_e4m3", long_rows, cu_q=ctx.cu_q, kv_len=ctx.kv_len, **({} if rows is None else {"long_rows": rows}))
+        _ints("attention_e4m3", requests + 1, cu_q=ctx.cu_q)             # (a request's tokens end where the next one's begin)
+        _ints("attention_e4m3", requests, kv_len=ctx.kv_len)
+        if rows is not None:
+            _ints("attention_e4m3", long_rows, long_rows=rows)
         _here("attention_e4m3", rows, ctx.cu_q, ctx.kv_len)
         _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iiifipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
