@@ -290,6 +290,21 @@ def test_portions_behind_long_caches(new, past, nq, nkv, d, page, window):
     attention(new, past, nq=nq, nkv=nkv, d=d, page=page, window=window, seed=4)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_long_cache_beside_a_portion_does_not_cut_its_keys(d):
+    """How a portion's keys are cut goes by the portions of a step: the same bits beside a single token that sees many more."""
+    gen = torch.Generator().manual_seed(6)
+    ctx, group, pages = plain.step([300, 1], [0, 3500], 16)
+    cache = plain.random_cache(pages, 1, 16, d, gen)
+    q = torch.randn(301, 4 * d, generator=gen).bfloat16().to(DEVICE)
+    sizes = dict(nq=4, nkv=1, head_dim=d, scale=d ** -0.5)
+    both = ops.attention_e4m3(ctx, q, cache, group, **sizes)
+    check_attention(q, cache, ctx, group, both, nq=4, nkv=1, d=d, window=0, scale=d ** -0.5)
+    alone, view, _ = plain.step([300], [0], 16)
+    view.block_table = group.block_table[:1]
+    assert torch.equal(ops.attention_e4m3(alone, q[:300], cache, view, **sizes), both[:300]) and int(ctx.status) == int(alone.status) == 0
+
+
 def test_segments_of_both_head_sizes():
     """One token of few heads behind many keys, for each head size first or after the other."""
     for d in (64, 128, 64):

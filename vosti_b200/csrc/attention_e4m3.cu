@@ -583,6 +583,8 @@ attention_e4m3_simt_kernel(const T* __restrict__ q, T* __restrict__ out, const C
 // Segments of a token's keys: as many as find an SM at once, each of a tile a warp at least, eight at most (what a cluster always may have); sixteen
 // where they are few and long. us at 1, 4, 8 and 16 segments: 8 kv heads, one token at 2,048 keys 18.7, 7.8, 6.1 and 7.2, at 8,192 67, 20, 12.3 and
 // 10.5; four at 8,192 72, 24, 18.8 and 25; eight at 8,192 with 4, 6 and 8 31, 28 and 37; sixteen at 2,048 with 1, 3 and 4 21.7, 17.6 and 23.8.
+// A window is left out of it: what it leaves is read sooner by more CTAs than have a tile for every warp (one token, a window of 512 behind 16,384 keys: 16
+// segments 6.3, the two of nine tiles 7.3; a window of 4,096 7.9 and, in eight, 9.0; eight tokens, 512: six segments 7.3, two 8.3).
 int segments_of(int64_t items, int max_kv_len) {
   const int64_t room = 148 * RESIDENT / items, work = (max_kv_len + TILE - 1) / TILE / WARPS;
   if (items * MAX_SEGMENTS <= 2 * 148 && work >= 2 * MAX_SEGMENTS) return MAX_SEGMENTS;
