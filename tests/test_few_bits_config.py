@@ -5,7 +5,7 @@ import torch
 from tiny_configs import TINY_A
 from vosti_b200 import Engine
 from vosti_b200.cache import CacheManager
-from vosti_b200.config import ConfigError, PartSpec, in_few_bits, model_spec_from_config
+from vosti_b200.config import ConfigError, PartSpec, in_few_bits, model_spec_from_config, serves_few_bits
 from vosti_b200.models import build_model
 from vosti_b200.parts import build_feed_forward, build_mixer
 
@@ -63,6 +63,17 @@ def test_engine_refuses():
             Engine("nowhere", weights="int4", batch_invariant=mode)
     with pytest.raises(ValueError, match="bfloat16"):
         Engine("nowhere", weights="int4", dtype="float32")
+
+
+@pytest.mark.parametrize("form", [dict(cache="e4m3"), dict(weights="int4"), dict(cache="e4m3", weights="int4")])
+def test_engine_refuses_a_description_in_few_bits(form):
+    """The same as by the engine's own arguments."""
+    plain = model_spec_from_config(TINY_A)
+    few = in_few_bits(plain, **form)
+    assert serves_few_bits(few) and not serves_few_bits(plain)
+    for mode in (True, "1", "full", "decode"):
+        with pytest.raises(ValueError, match="batch_invariant"):
+            Engine(spec=few, tensors={}, num_blocks=4, batch_invariant=mode)
 
 
 def test_pages_hold_whole_blocks():

@@ -1,7 +1,7 @@
 from .schema import ConfigError, LayerSpec, ModelSpec, PartSpec, RunEntry
 from .registry import (architecture_of, known_architectures, model_spec_from_config,
                        model_spec_from_dir, read_config_json, register_architecture)
-from .few_bits import in_few_bits
+from .few_bits import in_few_bits, serves_few_bits
 from . import qwen3 as _qwen3
 from .qwen3 import Qwen3Config
 from . import mugizen as _mugizen
@@ -22,5 +22,5 @@ register_architecture(_difavik.ARCHITECTURE, _difavik.spec_from_config, replace=
 __all__ = [
     "ConfigError", "LayerSpec", "ModelSpec", "PartSpec", "RunEntry", "Qwen3Config",
     "architecture_of", "in_few_bits", "known_architectures", "model_spec_from_config", "model_spec_from_dir",
-    "read_config_json", "register_architecture",
+    "read_config_json", "register_architecture", "serves_few_bits",
 ]

@@ -19,6 +19,12 @@ def _with(part: PartSpec, **params) -> PartSpec:
     return PartSpec.make(part.kind, **{**part.as_dict(), **params})
 
 
+def serves_few_bits(spec: ModelSpec) -> bool:
+    """Whether any of a description's layers holds its keys and values in 8 bits or matrices in 4."""
+    parts = [part for layer in spec.layers for part in (layer.mixer, layer.feed_forward) if part is not None]
+    return any((part.kind in CACHE_KINDS and part.get("cache") is not None) or (part.kind in WEIGHT_KINDS and part.get("weights") is not None) for part in parts)
+
+
 def in_few_bits(spec: ModelSpec, *, cache: Optional[str] = None, weights: Optional[str] = None, weight_group: int = 128) -> ModelSpec:
     """`cache` "e4m3": keys and values in float8 e4m3 with a power of two per block of 16 tokens and head (ops.PagedE4M3).
     `weights` "int4": the layers' matrices rounded to 4 bits with a scale per `weight_group` neighbouring inputs

@@ -28,6 +28,7 @@ from typing import Dict, Iterable, List, Optional, Sequence
 import numpy as np
 import torch
 
+from ..config import serves_few_bits
 from ..sampling import sample_from_slots, sampler_state_words
 from .batch import StepEntry
 from .request import AdmissionStatus, Request
@@ -76,8 +77,12 @@ class Engine:
         `cuda_graphs`: decode steps are recorded once per shape and replayed; it is switched
         off by itself for a model with a part that declares `capture_safe = False`."""
         from .. import ops
-        if (cache_dtype or weights) and batch_invariant not in (False, None, "off", "0", ""):
-            raise ValueError("serving in few bits rounds keys, values and products by how the work is cut: not with batch_invariant")
+        one_order = batch_invariant not in (False, None, "off", "0", "")
+
+        def refuse_one_order(few_bits):
+            if few_bits and one_order:
+                raise ValueError("serving in few bits rounds keys, values and products by how the work is cut: not with batch_invariant")
+        refuse_one_order(cache_dtype or weights or (spec is not None and serves_few_bits(spec)))
         if weights and not _is_bfloat16(dtype) and str(dtype) != "bf16":
             raise ValueError("weights in 4 bits serve bfloat16 activations only")
         self.invariance = ops.set_invariance(batch_invariant) if _is_bfloat16(dtype) else None
@@ -86,6 +91,7 @@ class Engine:
                                   tensors=tensors, consume_tensors=consume_tensors, cache_dtype=cache_dtype, weights=weights,
                                   weight_group=weight_group)
         spec = self.runner.spec
+        refuse_one_order(serves_few_bits(spec))            # (an architecture of the folder's own)
         self.scheduler = Scheduler(self.runner.cache, SchedulerConfig(
             max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens,
             prefill_chunk_size=prefill_chunk_size, vocab_size=spec.vocab_size, max_context=spec.max_positions))
