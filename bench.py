@@ -248,15 +248,20 @@ def flops_of_prefill(config, tokens):
     return linear + attention
 
 
-def closed_form_weight_bytes(config):
-    """bf16 bytes of every weight a decode step reads whole: per layer the four attention
+def closed_form_weight_bytes(config, weights=None, group=128):
+    """Bytes of every weight a decode step reads whole: per layer the four attention
     projections, two head norms, two norms, three feed-forward matrices; the final norm; the
-    output head (the embedding table is read by rows, one per token)."""
+    output head (the embedding table is read by rows, one per token). All of them bfloat16, or with
+    `weights` "int4" the layers' matrices in 4 bits (features in sixteens, inputs in blocks of 128) and a bfloat16 scale for each `group` inputs."""
     L, H = config["num_hidden_layers"], config["hidden_size"]
     nq, nkv, d, I, V = (config["num_attention_heads"], config["num_key_value_heads"], config["head_dim"],
                         config["intermediate_size"], config["vocab_size"])
-    per_layer = H * (nq + 2 * nkv) * d + nq * d * H + 3 * H * I + 2 * H + 2 * d
-    return 2 * (L * per_layer + H + V * H)
+    matrices = [((nq + 2 * nkv) * d, H), (H, nq * d), (2 * I, H), (H, I)]
+    if weights == "int4":
+        per_layer = sum(-(-f // 16) * 16 * -(-k // 128) * (64 + 128 // group * 2) for f, k in matrices)
+    else:
+        per_layer = sum(2 * f * k for f, k in matrices)
+    return L * (per_layer + 2 * (2 * H + 2 * d)) + 2 * (H + V * H)
 
 
 def reference_main(args) -> int:
@@ -825,8 +830,8 @@ def main() -> int:
     del tensors
     torch.cuda.empty_cache()
     weight_bytes = engine.runner.model.weight_bytes()
-    assert args.weights or abs(weight_bytes - closed_form_weight_bytes(config)) <= 0.002 * weight_bytes, \
-        (weight_bytes, closed_form_weight_bytes(config))
+    expected_bytes = closed_form_weight_bytes(config, args.weights, args.weight_group)
+    assert abs(weight_bytes - expected_bytes) <= 0.002 * weight_bytes, (weight_bytes, expected_bytes)
     kv_bytes_per_token = engine.runner.cache.bytes_per_token()
 
     prefill_ms = float("nan") if args.no_prefill else prefill_run(engine, 5, seed=11)

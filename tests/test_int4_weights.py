@@ -83,3 +83,16 @@ def test_scales_and_types_that_are_refused():
                  (codes.to(torch.complex64), torch.ones(16, 1))):
         with pytest.raises(ops.KernelError):
             ops.Int4Weight.from_codes(*args, 128)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("hidden,heads,kv,d,inter", [(256, 4, 2, 64, 512), (200, 5, 1, 48, 328)])
+def test_bytes_that_the_benchmark_counts(group, hidden, heads, kv, d, inter):
+    """The benchmark's closed form of a step's weight bytes against the weights' own tensors."""
+    import bench
+    config = dict(num_hidden_layers=3, hidden_size=hidden, num_attention_heads=heads, num_key_value_heads=kv, head_dim=d, intermediate_size=inter, vocab_size=300)
+    matrices = [((heads + 2 * kv) * d, hidden), (hidden, heads * d), (2 * inter, hidden), (hidden, inter)]
+    rest = 2 * (3 * (2 * hidden + 2 * d) + hidden + 300 * hidden)
+    packed = [ops.Int4Weight.quantize(torch.ones(shape), group) for shape in matrices]
+    assert bench.closed_form_weight_bytes(config, "int4", group) == rest + 3 * sum(w.codes.numel() + 2 * w.scales.numel() for w in packed)
+    assert bench.closed_form_weight_bytes(config) == rest + 3 * sum(2 * f * k for f, k in matrices)
