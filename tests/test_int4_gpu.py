@@ -167,3 +167,46 @@ def test_gated_products_that_are_refused():
     with pytest.raises(ops.KernelError):
         ops.gemm_int4(odd, w, status, swiglu=True)
     assert tuple(ops.gemm_int4(odd[:0], w, status).shape) == (0, 64) and int(status) == 0
+
+
+@pytest.mark.parametrize("features,k,group", [(16, 128, 128), (130, 640, 32), (257, 96, 32), (333, 264, 64), (4096, 512, 64), (20, 1024, 128)])
+@pytest.mark.parametrize("rows", [5, 16, 17, 64, 128, 129, 300])
+def test_each_weight_alone(features, k, group, rows):
+    """Rows of a single one pick single weights: codes times scales to the bit, rounded once to bfloat16 above 16 rows and not at all below."""
+    w, numbers, _ = weight(features, k, group)
+    numbers = (numbers.float().bfloat16() if rows > 16 else numbers.float()).to(DEVICE)      # (a code of 4 bits times 8 bits is exact in float32)
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    for start in range(0, k, rows):
+        at = torch.arange(start, start + rows, device=DEVICE) * 7 % k
+        x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEVICE)
+        x[torch.arange(rows, device=DEVICE), at] = 1
+        assert torch.equal(ops.gemm_int4(x, w, status, out_dtype=torch.float32), numbers[:, at].T.float())
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("rows", [17, 33, 64, 65, 128, 129, 300])
+@pytest.mark.parametrize("features,k,group", [(1000, 1024, 128), (130, 640, 32), (4096, 512, 64), (257, 96, 32), (640, 200, 32), (300, 8192, 128)])
+def test_products_of_rounded_weights(rows, features, k, group):
+    """More than 16 rows against the weights as they are rounded: what is left are the float32 sums, each addition of which may be cut off
+    below its last bit (2^-23 of at most sum |x||w|), and the result's rounding."""
+    w, numbers, gen = weight(features, k, group, seed=3)
+    rounded = numbers.float().bfloat16().double()
+    x = torch.randn(rows, k, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    want, size = x.double() @ rounded.T, x.double().abs() @ rounded.abs().T
+    for kind, half in ((torch.float32, 2.0 ** -24), (torch.bfloat16, 2.0 ** -8)):
+        y = ops.gemm_int4(x.to(DEVICE), w, status, out_dtype=kind).cpu().double()
+        sums = (k + 8) * 2.0 ** -23 * size
+        assert bool(((y - want).abs() <= sums + half * (want.abs() + sums)).all()) and int(status) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 40])
+@pytest.mark.parametrize("k", [1, 7, 100, 129, 1003])
+def test_rows_that_start_inside_a_word_are_exact(rows, k):
+    """They take the few rows' kernel sixteen at a time, whose codes and scales are not rounded."""
+    w, numbers, gen = weight(70, k, 32)
+    x = torch.randn(rows, k, generator=gen).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    for kind in (torch.float32, torch.bfloat16):
+        check(ops.gemm_int4(x.to(DEVICE), w, status, out_dtype=kind), x, numbers, 16)
+    assert int(status) == 0
