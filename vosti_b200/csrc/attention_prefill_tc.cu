@@ -542,10 +542,8 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const uint32_t bar = edge ? smem_u32(&edge_bar[w]) : smem_u32(&kv_full[stage]);
       if (lane == 0) mbar_expect_tx(bar, (uint32_t)(2 * NB * GROUP_KEYS * 128));
       __syncwarp();
-      if constexpr (!EIGHT) {
       if (lane < 2 * NB)
         tma_load_2d(smem_u32(dst + lane * (KT * 128)), lane < NB ? &map_k : &map_v, (lane < NB ? lane : lane - NB) * 64, row, bar);
-      }
       if (edge) {
         ok = mbar_wait(bar, edges & 1, &abort_flag, status);
         ++edges;
