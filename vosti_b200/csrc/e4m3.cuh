@@ -44,7 +44,8 @@ __device__ __forceinline__ int e4m3_scale_for(float amax) {
   return scale > 0 ? scale : 0;
 }
 
-// ---- payloads as bfloat16
+// ---- payloads as bfloat16: bits in their new places, and a product with a power of two for the difference of the exponents' biases, which takes
+// subnormals with it (published for float16 by F. Giesen, "Half to float done quick", 2012)
 __device__ __forceinline__ uint32_t bf16x2_times(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

@@ -2338,7 +2338,7 @@ class PagedE4M3:
     `v_scale` [pages, kv heads, page / 16]. A block that was handed a value that is not finite, or 2^96
     or more in size (sums of weights times values have to fit float32), has the scale 255 and is no number. A payload 0x7f or 0xff is
     no number either (`qkv_post_e4m3` leaves one in such blocks only): attention's rows that see it in a key are no numbers, those that see it in a
-    value are none in its feature, or in all of theirs. `zeros` makes an empty one; `dequantized` gives keys and values [pages, kv heads, page, d] in float32."""
+    value are none in its feature, or in all of theirs. Sizes in a cache made elsewhere stay below 2^96 too (scales of up to 215). `zeros` makes an empty one; `dequantized` gives keys and values [pages, kv heads, page, d] in float32."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "head_dim", "pointers")
 
