@@ -423,21 +423,18 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     uint32_t edges = 0;
     if constexpr (EIGHT) {
       constexpr int UNITS = D / 32;                      // 16-byte pieces of a block's keys, or values, that a lane moves
-      auto block_of = [&](int key) {                     // the cache's block that begins with the key, -1 where no page holds it
-        const int index = page_shift >= 0 ? key >> page_shift : key / page_size;
-        const int page = index < max_pages ? table[index] : -1;
-        return page < 0 || page >= num_pages ? (int64_t)-1 : ((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (key - index * page_size) / GROUP_KEYS;
-      };
       for (int j = 0; j < tiles && ok; ++j) {
         const int stage = j % STAGES;
         const int lo = tile_key(j) + w * GROUP_KEYS;
         uint4 piece[2][UNITS];
         int k_scale = 0, v_scale = 0, seen = 0;          // tokens of the block before the last visible one's end
         if (lo + GROUP_KEYS - 1 >= first_key && lo < key_end) {
-          const int64_t block = block_of(lo);
-          if (block < 0) {
+          const int index = page_shift >= 0 ? lo >> page_shift : lo / page_size;
+          const int page = index < max_pages ? table[index] : -1;
+          if (page < 0 || page >= num_pages) {
             raise_fault(status, VOSTI_FAULT_PAGE_RANGE);
           } else {
+            const int64_t block = ((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (lo - index * page_size) / GROUP_KEYS;
             seen = min(GROUP_KEYS, key_end - lo);
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
@@ -490,7 +487,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           // zero, and its token's key is none. (Places are worked out again too: kept for this, they spill registers of the loop.)
           int key, me;
           asm volatile("mov.u32 %0, %2;\n\tmov.u32 %1, %%laneid;" : "=r"(key), "=r"(me) : "r"(lo));
-          const int64_t at = block_of(key) * (GROUP_KEYS * D);
+          const int index = key / page_size, page = index < max_pages ? table[index] : -1;
+          const int64_t at = page < 0 || page >= num_pages
+                                 ? -1
+                                 : (((int64_t)page * nkv + g) * (page_size / GROUP_KEYS) + (key - index * page_size) / GROUP_KEYS) * (GROUP_KEYS * D);
           uint32_t tokens = 0;                           // of the block that are no numbers, bit by bit
           __syncwarp();                                  // (every lane's pieces are in their places)
 #pragma unroll 1
