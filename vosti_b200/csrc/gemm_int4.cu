@@ -10,7 +10,8 @@
 // Bringing Large Scale MoE Models into Cloud Scale Production", 2022, there for float16.)
 //
 // Gated: tiles of 16 features are taken in pairs, a gate and what it is for, and Y[t, 16 p + i] = silu(gate) * up of pair p, in float32 (24,576 x 4,096,
-// us without and with it, and with a kernel of its own behind: 8 tokens 14.5, 14.5, 19.3, 64 25.6, 26.1, 33.7, 2,048 309, 350, 380 to 440).
+// us without and with it, and with a kernel of its own behind: 8 tokens 14.5, 14.5, 19.1, 64 25.8, 26.2, 33.8, 2,048 371, 378, 446 under the power cap at
+// 1,520 to 1,660 MHz, 316, 322, 385 after a rest at 1,965).
 //
 // Up to 16 tokens: mma.sync, weights as the 16 rows (int4_few_kernel). What bounds it is the weights' bytes. More tokens: tcgen05
 // (int4_tiles_kernel), weights made bfloat16 in tensor memory.

@@ -12,7 +12,7 @@
 // A value that is not finite, or not below 2^96, makes its block's scale 255: the block is no number from then on.
 //
 // A head of 64, 128 or 256 that turns as a whole in pairs (i, i + d/2), or not at all, is d / 8 lanes with four neighbouring elements of each half;
-// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 17 to 19 us, 40% of the rate its bytes could move
+// any other is a warp with an element pair every 32. A prompt of 2,048 tokens of the 8B sizes takes 19 us, 38% of the rate its bytes could move
 // at: blocks are short, and the latencies of their loads in a row are not hidden by the 24 warps an SM holds of their registers (20 warps with more
 // registers, blocks that walked on over query heads, and a head on a whole warp were slower). Eight tokens take 3 us; a CTA that took a run's keys and
 // values both needed 5.3. Between a model's other kernels, which leave neither the cache nor the turns in L2, they take 4.5 us behind the projection;
@@ -554,8 +554,8 @@ VOSTI_API int vosti_qkv_post_e4m3(const void* qkv, const float* partial, int spl
   VOSTI_REQUIRE(slot_mapping != nullptr && k != nullptr && v != nullptr && k_scale != nullptr && v_scale != nullptr, "qkv_post_e4m3: the cache is missing");
   VOSTI_REQUIRE((int64_t)tokens * (nq + 2 * nkv) <= 0x7fffffff - 4096, "qkv_post_e4m3: too many tokens and heads for one launch");
   // Neighbouring tokens whose runs a CTA takes: few tokens one, so that none waits for another's run; more of them four, a run a warp in a batch of
-  // single tokens; many, as prompts bring them, eight or sixteen, which hold a run or two. us with tiles of 1, 4, 8, 16 (8B sizes): 8 single tokens 3.3, 3.5, 5.2,
-  // 5.2; 64 6.1, 4.3, 5.6, 8.6; 256 12.2, 8.8, 9.3, 12.6; a prompt of 512 14, 7.3, 6.5, 6.1; of 2,048 50, 24, 19.5, 17.1.
+  // single tokens; many, as prompts bring them, eight or sixteen, which hold a run or two. us with tiles of 1, 4, 8, 16 (8B sizes): 8 single tokens 3.0, 3.1, 4.2,
+  // 4.2; 64 5.4, 3.7, 5.0, 8.6; 256 12.3, 9.0, 8.8, 13.0; a prompt of 512 13.3, 6.6, 5.8, 5.4; of 2,048 53, 25.9, 21.0, 18.6; of 4,096 105, 52, 42, 37.5.
   const int tile = tokens <= FEW ? 1 : tokens <= MANY ? 4 : tokens <= 4 * MANY ? 8 : 16;
   const PostArgs a = {qkv, partial, splits, (int64_t)tokens * (nq + 2 * nkv) * d, q_out, (uint8_t*)k, (uint8_t*)v, (uint8_t*)k_scale,
                       (uint8_t*)v_scale, q_norm_w, k_norm_w, norm_w_is_f32, eps, 1.f / (float)d, cos_table, sin_table, max_positions, positions, slot_mapping,
