@@ -445,7 +445,8 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             v_scale = map_v.scale[block];
           }
         }
-        if (j >= STAGES) ok = mbar_wait(smem_u32(&kv_empty[stage]), ((j / STAGES) - 1) & 1, &abort_flag, status);
+        // (all lanes or none: those that go on meet in votes)
+        if (j >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&kv_empty[stage]), ((j / STAGES) - 1) & 1, &abort_flag, status)) != 0;
         if (!ok) break;
         // A block that is no number makes its scores no number: those are left out where they are not visible, while such a
         // value would meet weights of zero in rows that do not see it.
