@@ -589,3 +589,55 @@ def test_arrays_with_too_few_requests_are_refused():
                 ops.attention_e4m3(ctx, q, cache, group, **sizes)
             setattr(owner, name, kept)
         assert int(ctx.status) == 0
+
+
+def test_a_layout_that_takes_short_requests_for_portions():
+    """Which requests are portions is the layout's to say, few tokens or many."""
+    ctx, group, pages = plain.step([3, 1, 2], [20, 500, 70], 16)
+    cache = plain.random_cache(pages, 2, 16, 64, torch.Generator().manual_seed(2))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEVICE)
+    ctx.layout = {"attention": dict(num_short_tokens=1, num_long_rows=2, max_long_q_len=3)}
+    ctx.extras = {"attention.short_tokens": ints(3), "attention.long_rows": ints(0, 2)}
+    q = torch.randn(6, 8 * 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(DEVICE)
+    out = ops.attention_e4m3(ctx, q, cache, group, nq=8, nkv=2, head_dim=64, scale=0.125)
+    assert int(ctx.status) == 0
+    check_attention(q, cache, ctx, group, out, nq=8, nkv=2, d=64, window=0, scale=0.125)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_rows_that_see_nothing_are_zeros(dtype, d, window):
+    """A single token at position -1 (a place of a batch that no request fills) reads no page and comes out as zeros."""
+    ctx, group, pages = plain.step([1] * 5, [10, 300, 2000, 0, 64], 16)
+    cache = plain.random_cache(pages, 2, 16, d, torch.Generator().manual_seed(2))
+    q = torch.randn(5, 4 * d, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEVICE)
+    sizes = dict(nq=4, nkv=2, head_dim=d, scale=0.1, window=window)
+    want = ops.attention_e4m3(ctx, q, cache, group, **sizes)
+    ctx.positions[1] = ctx.positions[4] = -1
+    group.block_table[1] = group.block_table[4] = -1
+    for appended in (0, 1):
+        out = ops.attention_e4m3(ctx, q, cache, group, appended=appended, **sizes)
+        assert torch.equal(out[[0, 2, 3]], want[[0, 2, 3]]) and int(out[[1, 4]].count_nonzero()) == 0 and int(ctx.status) == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: both give what each gives alone."""
+    steps = [plain.step(new, past, 16, seed=i) for i, (new, past) in enumerate((([1] * 8, [900] * 8), ([200, 1, 1], [100, 700, 40])))]
+    gens = [torch.Generator().manual_seed(20 + i) for i in range(2)]
+    caches = [[plain.random_cache(pages, 2, 16, 128, torch.Generator().manual_seed(i)) for _ in range(2)] for i, (_, _, pages) in enumerate(steps)]
+    qkv = [torch.randn(ctx.num_tokens, 12 * 128, generator=g).bfloat16().to(DEVICE) for (ctx, _, _), g in zip(steps, gens)]
+
+    def run(i, cache, turns):
+        ctx, group, _ = steps[i]
+        for _ in range(turns):
+            q = ops.qkv_post_e4m3(qkv[i], cache, nq=8, nkv=2, head_dim=128, slot_mapping=group.slot_mapping, status=ctx.status)
+            out = ops.attention_e4m3(ctx, q, cache, group, nq=8, nkv=2, head_dim=128, scale=0.09, appended=ctx.max_q_len)
+        return out
+    want = [run(i, caches[i][0], 20) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for i, stream in enumerate(streams):
+        with torch.cuda.stream(stream):
+            got[i] = run(i, caches[i][1], 20)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(int(ctx.status) == 0 for ctx, _, _ in steps)

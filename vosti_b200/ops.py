@@ -2475,7 +2475,7 @@ def attention_e4m3(ctx, q: torch.Tensor, cache: PagedE4M3, group, *, nq: int, nk
             _ints("attention_e4m3", long_rows, long_rows=rows)
         _here("attention_e4m3", rows, ctx.cu_q, ctx.kv_len)
         # keys of the portions alone: those of single tokens beside them say nothing of how theirs are best cut
-        longest = ctx.max_kv_len if count == 0 else max(kv for n, kv in zip(ctx.host_q_lens, ctx.host_kv_lens) if n > SHORT_ROW)
+        longest = ctx.max_kv_len if count == 0 else max((kv for n, kv in zip(ctx.host_q_lens, ctx.host_kv_lens) if n > SHORT_ROW), default=ctx.max_kv_len)
         _check(_bound("vosti_attention_prefill_tc_e4m3", "pppppp" "pipp" "piiiiii" "iiifipp")(
             q.data_ptr(), *cache.pointers, out.data_ptr(), _address(rows), long_rows, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), *geometry,
             lists["max_long_q_len"], tokens, longest, scale, window, status.data_ptr(), stream), "attention_prefill_tc_e4m3")
